@@ -399,6 +399,82 @@ SCA2_API int sca2_scan_fwd_bwd_noalloc(const sca2_scan_args* a, sca2_out o, floa
                                        sca2_out dO, const float* dS_final,
                                        const sca2_scan_grads* gr, void* stream);
 
+/* ---- residual join with norms -----------------------------------------------------------------
+ * Per row of width d:
+ *     p = N_post(u) (or u),   y = x + scale * sigmoid(gate) * p,   z = N(y)
+ * the tail of a residual block with the norm after the block, its gate and residual scale, and the
+ * norm before the next block.  N: LayerNorm (as sca2_layer_norm_fwd) or the RMS norm
+ * v * rsqrt(mean(v^2) + eps) * w.  fp32 arithmetic; z is formed from the unrounded y. */
+#define SCA2_RNORM_MAX_D 4096
+enum sca2_norm_kind { SCA2_NORM_LAYER = 0, SCA2_NORM_RMS = 1 };
+
+typedef struct sca2_rnorm_args {
+  const void* x;        /* (rows, d) x_dtype: the residual stream */
+  const void* u;        /* (rows, d) u_dtype: the block's output */
+  const void* gate;     /* u_dtype logits: (rows, d) or (rows, 1), by gate_mode */
+  int64_t sx, su, sg;   /* row strides in values (the rows themselves are contiguous) */
+  const float* w;       /* (d) weight of N, or NULL: no z */
+  const float* b;       /* (d) bias of N or NULL (LayerNorm only) */
+  const float* pw;      /* (d) weight of N_post, or NULL: p = u */
+  const float* pb;      /* (d) bias of N_post or NULL (LayerNorm only) */
+  const float* scale;   /* (d) residual scale, or NULL = 1 */
+  int64_t rows;
+  int32_t d;            /* 1 ... SCA2_RNORM_MAX_D */
+  int32_t x_dtype, u_dtype, z_dtype;
+  int32_t kind;         /* sca2_norm_kind, of both norms */
+  int32_t gate_mode;    /* 0: no gate; 1: one logit a row; 2: one a value */
+  float eps;
+} sca2_rnorm_args;
+
+/* y (rows, d) x_dtype and z (rows, d) z_dtype (or NULL), dense; stats (rows, 4) fp32, 16-byte
+ * aligned, kept for the backward, or NULL.  Replaces the residual line and the following LayerNorm
+ * of the layers (lapa/layer.py:589-590, sca2/ref.py:384-390), which have neither the norm after
+ * the block nor the gate and scale.  y may not alias the inputs. */
+SCA2_API int sca2_residual_norm_fwd(const sca2_rnorm_args* a, void* y, void* z, float* stats, void* stream);
+
+/* Gradients, all written, dense: dx x_dtype, du u_dtype, dgate u_dtype ((rows, d) or (rows)); the
+ * parameters' fp32 gradients or NULL to skip one. */
+typedef struct sca2_rnorm_grads {
+  void *dx, *du, *dgate;
+  float *dw, *db, *dscale, *dpw, *dpb;
+} sca2_rnorm_grads;
+
+SCA2_API int64_t sca2_residual_norm_work_bytes(int64_t rows, int32_t d);
+
+/* dy (x_dtype) and dz (z_dtype) dense, either may be NULL (zero); stats as the forward left them;
+ * work: 16-byte aligned, at least sca2_residual_norm_work_bytes(rows, d). */
+SCA2_API int sca2_residual_norm_bwd(const sca2_rnorm_args* a, const float* stats, const void* dy,
+                   const void* dz, const sca2_rnorm_grads* g, void* work, int64_t work_bytes,
+                   void* stream);
+
+/* ---- gradient norm and clipping ---------------------------------------------------------------
+ * One tensor of the list: n values at src (src_dtype) and, for clipping, their destination
+ * (dst_dtype; src itself for clipping in place).  Both dense; any alignment to their values. */
+typedef struct sca2_grad_tensor {
+  const void* src;
+  void* dst;            /* ignored by sca2_grad_norm */
+  int64_t n;
+  int32_t src_dtype;    /* SCA2_F32 or SCA2_BF16 */
+  int32_t dst_dtype;
+} sca2_grad_tensor;
+
+/* Bytes of the device workspace of the two calls below (the list itself is host memory and is
+ * not kept: its contents travel as kernel parameters). */
+SCA2_API int64_t sca2_clip_grads_work_bytes(const sca2_grad_tensor* list, int32_t count);
+
+/* *norm (device, fp32) = the 2-norm of all values of the list together, summed in 64 bits in a
+ * fixed order.  count = 0 gives 0.  No counterpart in the reference; the semantics are
+ * torch.nn.utils.clip_grad_norm_'s. */
+SCA2_API int sca2_grad_norm(const sca2_grad_tensor* list, int32_t count, float* norm, void* work,
+                   int64_t work_bytes, void* stream);
+
+/* dst = src * min(1, max_norm / (norm + 1e-6)) for every tensor, and *norm the norm before it.
+ * An infinite or NaN norm reaches the values as it does there (0 or NaN).  A destination may be
+ * its own source with the same type; any other overlap of a destination with a tensor of the
+ * list is refused. */
+SCA2_API int sca2_clip_grads(const sca2_grad_tensor* list, int32_t count, float max_norm, float* norm,
+                   void* work, int64_t work_bytes, void* stream);
+
 /* Read and clear the device fault word of the tensor-core kernels (synchronises the
  * device).  Bit 0: an internal wait on the tensor core timed out; the kernel left early
  * and its outputs are not valid.  Kernels never trap: this word is how a device-side

@@ -82,6 +82,28 @@ class DScanGrads(C.Structure):
     ]
 
 
+class RNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("u", C.c_void_p), ("gate", C.c_void_p),
+        ("sx", C.c_int64), ("su", C.c_int64), ("sg", C.c_int64),
+        ("w", C.c_void_p), ("b", C.c_void_p), ("pw", C.c_void_p), ("pb", C.c_void_p), ("scale", C.c_void_p),
+        ("rows", C.c_int64), ("d", C.c_int32), ("x_dtype", C.c_int32), ("u_dtype", C.c_int32),
+        ("z_dtype", C.c_int32), ("kind", C.c_int32), ("gate_mode", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class RNormGrads(C.Structure):
+    _fields_ = [
+        ("dx", C.c_void_p), ("du", C.c_void_p), ("dgate", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p),
+        ("dscale", C.c_void_p), ("dpw", C.c_void_p), ("dpb", C.c_void_p),
+    ]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("n", C.c_int64), ("src_dtype", C.c_int32),
+                ("dst_dtype", C.c_int32)]
+
+
 # (name, restype, argtypes) of every exported symbol, in header order
 SIGNATURES = [
     ("sca2_scan_fwd", C.c_int, [C.POINTER(ScanArgs), Out, C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -133,6 +155,13 @@ SIGNATURES = [
                                  C.POINTER(ShortGrads), C.c_void_p, C.c_void_p]),
     ("sca2_scan_fwd_bwd_noalloc", C.c_int, [C.POINTER(ScanArgs), Out, C.c_void_p, Out, C.c_void_p,
                                             C.POINTER(ScanGrads), C.c_void_p]),
+    ("sca2_residual_norm_fwd", C.c_int, [C.POINTER(RNormArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("sca2_residual_norm_work_bytes", C.c_int64, [C.c_int64, C.c_int32]),
+    ("sca2_residual_norm_bwd", C.c_int, [C.POINTER(RNormArgs), C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.POINTER(RNormGrads), C.c_void_p, C.c_int64, C.c_void_p]),
+    ("sca2_clip_grads_work_bytes", C.c_int64, [C.c_void_p, C.c_int32]),
+    ("sca2_grad_norm", C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    ("sca2_clip_grads", C.c_int, [C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     ("sca2_fault_status", C.c_int, [C.POINTER(C.c_uint32)]),
     ("sca2_last_error", C.c_char_p, []),
     ("sca2_version", C.c_char_p, []),

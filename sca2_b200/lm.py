@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
 from .heads import LaplaceConfig
 from .layers import GatedLayer, LaplaceAttention, LayerCfg, LayerNorm
 
@@ -232,11 +233,14 @@ def lm_loss(model: nn.Module, tokens: torch.Tensor) -> torch.Tensor:
 
 
 def train_step(model: nn.Module, opt: torch.optim.Optimizer, tokens: torch.Tensor,
-               dtype: Optional[torch.dtype] = torch.bfloat16) -> torch.Tensor:
-    """One optimizer step (bf16 autocast by default); returns the loss (device scalar)."""
+               dtype: Optional[torch.dtype] = torch.bfloat16, max_norm: Optional[float] = None) -> torch.Tensor:
+    """One optimizer step (bf16 autocast by default); returns the loss (device scalar).  max_norm:
+    the gradients are clipped to that global norm before the optimizer's step (ops.clip_grads)."""
     with torch.autocast("cuda", dtype=dtype, enabled=dtype is not None):
         loss = lm_loss(model, tokens)
     loss.backward()
+    if max_norm is not None:
+        ops.clip_grads([p.grad for p in model.parameters() if p.grad is not None], max_norm)
     opt.step()
     opt.zero_grad(set_to_none=True)
     return loss.detach()

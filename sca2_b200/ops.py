@@ -10,6 +10,8 @@
     rms_heads(o)                                          multi-head read gathered + RMS
     layer_norm(x, w, b, eps)                              the layers' LayerNorm (fwd + bwd kernels)
     linear16(x, w, sizes)                                 x w^T to 16 bits on bf16 tensor cores
+    residual_norm(x, u, weight, ...) -> (y, z)            residual join with the norms on both sides
+    grad_norm(grads), clip_grads(grads, max_norm, out)    global gradient norm, clipping
 
 Every op runs the CUDA kernels of libsca2b200.so on the current stream.  There is no
 CPU path: a CPU tensor or a missing library raises.  Device memory (outputs, saved
@@ -18,9 +20,12 @@ allocates nothing.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import contextlib
+import struct
+from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import Out, ScanArgs, ScanGrads, Tok
@@ -34,6 +39,14 @@ def _stream():
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Context in which `dev` is the current device (launches go to the current device's stream)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _need_cuda(*ts):
@@ -1284,6 +1297,291 @@ def linear16(x: torch.Tensor, w: torch.Tensor, sizes: Tuple[int, ...]) -> Tuple[
 # ======================================================================================
 #  preallocated plans (benchmarks, CUDA-graph capture)
 # ======================================================================================
+# ======================================================================================
+#  residual join with the norms on both sides of it
+# ======================================================================================
+_NORM_KIND = {"layer": 0, "rms": 1}
+
+
+def _row_view(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
+    """t (..., d) as rows of contiguous values with one row stride (a copy only where its strides
+    do not allow that), and the stride."""
+    if t.is_contiguous():
+        return t, d
+    if t.stride(-1) == 1 or d == 1:
+        try:
+            v = t.view(-1, d)
+            if v.size(0) <= 1 or v.stride(0) >= d:
+                return v, max(v.stride(0), d)
+        except RuntimeError:
+            pass
+    return t.contiguous(), d
+
+
+def _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
+    a = _lib.RNormArgs()
+    d = x.shape[-1]
+    (x, a.sx), (u, a.su) = _row_view(x, d), _row_view(u, d)
+    a.x, a.u = x.data_ptr(), u.data_ptr()
+    if gate is not None:
+        a.gate_mode = 2 if gate.shape[-1] == d else 1
+        gate, a.sg = _row_view(gate, gate.shape[-1])
+        a.gate = gate.data_ptr()
+    a.w, a.b, a.pw, a.pb, a.scale = _ptr(w), _ptr(b), _ptr(pw), _ptr(pb), _ptr(scale)
+    a.rows, a.d = x.numel() // d, d
+    a.x_dtype, a.u_dtype, a.z_dtype = _DT[x.dtype], _DT[u.dtype], _DT[zdt]
+    a.kind, a.eps = kind, eps
+    return a, (x, u, gate)  # the tensors stay alive until the launch is queued
+
+
+def _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, save: bool):
+    dev = x.device
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    z = torch.empty(x.shape if w is not None else (0,), device=dev, dtype=zdt)
+    stats = torch.empty(x.numel() // x.shape[-1] if save else 0, 4, device=dev)
+    a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
+    with _on(dev):
+        _lib.check(_lib.load().sca2_residual_norm_fwd(a, y.data_ptr(), z.data_ptr() if w is not None else None,
+                                                      stats.data_ptr() if save else None, _stream()), "residual_norm")
+    return y, z, stats
+
+
+def _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, stats, dy, dz):
+    dev, d = x.device, x.shape[-1]
+    dense = lambda t, ty: None if t is None else t.to(ty).contiguous()
+    dy, dz = dense(dy, x.dtype), dense(dz, zdt)
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    du = torch.empty(u.shape, device=dev, dtype=u.dtype)
+    dgate = torch.empty(gate.shape, device=dev, dtype=gate.dtype) if gate is not None else None
+    dpar = [torch.empty(d, device=dev) if t is not None else None for t in (w, b, scale, pw, pb)]
+    a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
+    lib = _lib.load()
+    n = lib.sca2_residual_norm_work_bytes(a.rows, d)
+    work = torch.empty(n, device=dev, dtype=torch.uint8)
+    g = _lib.RNormGrads(dx.data_ptr(), du.data_ptr(), _ptr(dgate), *[_ptr(t) for t in dpar])
+    with _on(dev):
+        _lib.check(lib.sca2_residual_norm_bwd(a, stats.data_ptr(), _ptr(dy), _ptr(dz), g, work.data_ptr(), n, _stream()),
+                   "residual_norm_bwd")
+    return dx, du, dpar[0], dpar[1], dgate, dpar[2], dpar[3], dpar[4]
+
+
+@torch.library.custom_op("sca2b200::residual_norm_fwd", mutates_args=())
+def _residual_norm_fwd(x: torch.Tensor, u: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor],
+                       gate: Optional[torch.Tensor], scale: Optional[torch.Tensor], pw: Optional[torch.Tensor],
+                       pb: Optional[torch.Tensor], kind: int, eps: float, zdt: torch.dtype, save: bool
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """sca2_residual_norm_fwd: y, z (empty without w) and, with save, the rows' means and deviations."""
+    return _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, save)
+
+
+@_residual_norm_fwd.register_fake
+def _(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, save):
+    return (x.new_empty(x.shape), x.new_empty(x.shape if w is not None else (0,), dtype=zdt),
+            x.new_empty(x.numel() // x.shape[-1] if save else 0, 4, dtype=torch.float32))
+
+
+@torch.library.custom_op("sca2b200::residual_norm_bwd", mutates_args=())
+def _residual_norm_bwd(x: torch.Tensor, u: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor],
+                       gate: Optional[torch.Tensor], scale: Optional[torch.Tensor], pw: Optional[torch.Tensor],
+                       pb: Optional[torch.Tensor], kind: int, eps: float, zdt: torch.dtype, stats: torch.Tensor,
+                       dy: Optional[torch.Tensor], dz: Optional[torch.Tensor]
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                  torch.Tensor, torch.Tensor]:
+    """sca2_residual_norm_bwd: dx, du, dw, db, dgate, dscale, dpw, dpb (empty where there is no input)."""
+    out = _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, stats, dy, dz)
+    return tuple(x.new_empty(0) if t is None else t for t in out)
+
+
+@_residual_norm_bwd.register_fake
+def _(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, stats, dy, dz):
+    like = lambda t: x.new_empty(0) if t is None else t.new_empty(t.shape)
+    return tuple(like(t) for t in (x, u, w, b, gate, scale, pw, pb))
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    x, u, w, b, gate, scale, pw, pb, ctx.kind, ctx.eps, ctx.zdt, _ = inputs
+    ctx.save_for_backward(x, u, w, b, gate, scale, pw, pb, output[2])
+
+
+def _residual_norm_backward(ctx, dy, dz, _dstats):
+    x, u, w, b, gate, scale, pw, pb, stats = ctx.saved_tensors
+    out = torch.ops.sca2b200.residual_norm_bwd(x, u, w, b, gate, scale, pw, pb, ctx.kind, ctx.eps, ctx.zdt, stats, dy,
+                                               dz if w is not None else None)
+    return (*[None if t is None else g for t, g in zip((x, u, w, b, gate, scale, pw, pb), out)], None, None, None, None)
+
+
+_residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """The eager path of residual_norm: the same two calls without the operator dispatch."""
+
+    @staticmethod
+    def forward(ctx, x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
+        y, z, stats = _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, True)
+        ctx.save_for_backward(x, u, w, b, gate, scale, pw, pb, stats)
+        ctx.opts = kind, eps, zdt
+        ctx.set_materialize_grads(False)
+        return y, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dz):
+        *ins, stats = ctx.saved_tensors
+        return (*_residual_norm_bwd_run(*ins, *ctx.opts, stats, dy, dz if ins[2] is not None else None),
+                None, None, None)
+
+
+def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, *, gate: Optional[torch.Tensor] = None,
+                  scale: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, kind: str = "layer", eps: float = 1e-5,
+                  out_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The join of a block's output u to the residual stream x, with the norm after the block, its
+    gate and residual scale, and the norm before the next block, in one kernel each way:
+
+        p = N_post(u) if post_weight is given, else u
+        y = x + scale * sigmoid(gate) * p          z = N(y) if weight is given, else None
+
+    x, u (..., d) fp32 or bf16 (their types may differ), d <= 4096; gate (..., d) or (..., 1) logits;
+    weight, bias, post_weight, post_bias, scale (d) (computed with in fp32).  kind: "layer"
+    (LayerNorm) or "rms" (no bias), for both norms.  y has x's type, z out_dtype (default: x's);
+    arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
+    dev = _need_cuda(x, u, weight, bias, gate, scale, post_weight, post_bias)
+    E, d = _lib.Sca2Error, x.shape[-1] if x.dim() else 0
+    if kind not in _NORM_KIND:
+        raise E(f"residual_norm: kind must be 'layer' or 'rms', not {kind!r}")
+    if d < 1 or u.shape != x.shape:
+        raise E(f"residual_norm: x and u must have one shape (..., d), got {tuple(x.shape)} and {tuple(u.shape)}")
+    if gate is not None and (gate.shape[:-1] != x.shape[:-1] or gate.dim() != x.dim() or gate.shape[-1] not in (1, d)):
+        raise E(f"residual_norm: gate must be (..., d) or (..., 1), got {tuple(gate.shape)}")
+    zdt = x.dtype if out_dtype is None else out_dtype
+    if x.dtype not in _DT or u.dtype not in _DT or zdt not in _DT:
+        raise E("residual_norm: x, u and out_dtype must be float32 or bfloat16")
+    if (bias is not None and weight is None) or (post_bias is not None and post_weight is None):
+        raise E("residual_norm: a bias needs its weight")
+    par = []
+    for t in (weight, bias, scale, post_weight, post_bias):
+        if t is not None and t.shape != (d,):
+            raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
+        par.append(None if t is None else t.float().contiguous())
+    if gate is not None and gate.dtype != u.dtype:
+        gate = gate.to(u.dtype)
+    w, b, sc, pw, pb = par
+    kid, eps = _NORM_KIND[kind], float(eps)
+    if torch.compiler.is_compiling():
+        y, z, _ = torch.ops.sca2b200.residual_norm_fwd(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt,
+                                                       _wants_grad(x, u, w, b, gate, sc, pw, pb))
+    elif _wants_grad(x, u, w, b, gate, sc, pw, pb):
+        y, z = _ResidualNorm.apply(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt)
+    else:
+        y, z, _ = _residual_norm_run(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt, False)
+    return y, (z if w is not None else None)
+
+
+# ======================================================================================
+#  global gradient norm and clipping
+# ======================================================================================
+def _grad_list(what: str, grads, out=None):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
+    E = _lib.Sca2Error
+    if len(outs) != len(grads):
+        raise E(f"{what}: {len(grads)} gradients and {len(outs)} destinations")
+    for t in grads if out is None else grads + outs:
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _DT:
+            raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
+    dev = _need_cuda(*grads, *(outs if out is not None else ()))
+    if out is not None:
+        for g, o in zip(grads, outs):
+            if g.shape != o.shape or not o.is_contiguous():
+                raise E(f"{what}: a destination must be contiguous, with its gradient's shape")
+    return grads, outs, dev
+
+
+def _grad_table(src, dst):
+    """The sca2_grad_tensor list as bytes (host memory; the library copies it into the launch)."""
+    flat = [v for s, d in zip(src, dst)
+            for v in (s.data_ptr(), d.data_ptr(), s.numel(), _DT[s.dtype], _DT[d.dtype])]
+    return struct.pack("=" + "QQqii" * len(src), *flat)
+
+
+def _clip_run(grads, outs, max_norm: Optional[float], dev) -> torch.Tensor:
+    # a gradient that is not contiguous goes through a contiguous copy
+    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dst = [s if o is g else o for s, g, o in zip(src, grads, outs)]
+    table, n, lib = _grad_table(src, dst), len(src), _lib.load()
+    with _on(dev):
+        norm = torch.empty((), device=dev)
+        nb = lib.sca2_clip_grads_work_bytes(table, n)
+        work = torch.empty(max(nb, 8), device=dev, dtype=torch.uint8)
+        if max_norm is None:
+            _lib.check(lib.sca2_grad_norm(table, n, norm.data_ptr(), work.data_ptr(), nb, _stream()), "grad_norm")
+        else:
+            _lib.check(lib.sca2_clip_grads(table, n, max_norm, norm.data_ptr(), work.data_ptr(), nb, _stream()),
+                       "clip_grads")
+    if max_norm is not None:
+        for g, s, o in zip(grads, src, outs):
+            if o is g and s is not g:
+                g.copy_(s)
+    return norm
+
+
+@torch.library.custom_op("sca2b200::grad_norm", mutates_args=())
+def _grad_norm_op(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """sca2_grad_norm over a list of tensors."""
+    return _clip_run(list(grads), list(grads), None, grads[0].device)
+
+
+@_grad_norm_op.register_fake
+def _(grads):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.custom_op("sca2b200::clip_grads_", mutates_args=("grads",))
+def _clip_grads_op(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """sca2_clip_grads in place over a list of tensors; returns the norm before."""
+    return _clip_run(list(grads), list(grads), max_norm, grads[0].device)
+
+
+@_clip_grads_op.register_fake
+def _(grads, max_norm):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.no_grad()
+def grad_norm(grads) -> torch.Tensor:
+    """2-norm of all values of the tensors together (fp32 scalar on their device; summed in 64 bits
+    in a fixed order).  grads: a tensor or a list of float32 / bfloat16 tensors on one device; no
+    tensor gives 0 (on the current CUDA device)."""
+    grads, outs, dev = _grad_list("grad_norm", grads)
+    if not grads:
+        return torch.zeros((), device="cuda")
+    if torch.compiler.is_compiling():
+        return torch.ops.sca2b200.grad_norm(grads)
+    return _clip_run(grads, outs, None, dev)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
+    """Scale the gradients so that their global 2-norm is at most max_norm, and return the norm
+    before (fp32 scalar; nothing waits for the device): g * min(1, max_norm / (norm + 1e-6)), as
+    torch.nn.utils.clip_grad_norm_.  In place, or into the contiguous tensors `out` (float32 or
+    bfloat16, one for each gradient).  A tensor that is written may not share memory with another
+    of the call (refused)."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise _lib.Sca2Error("clip_grads: max_norm must be >= 0")
+    grads, outs, dev = _grad_list("clip_grads", grads, out)
+    if not grads:
+        return torch.zeros((), device="cuda")
+    if torch.compiler.is_compiling() and out is None:
+        return torch.ops.sca2b200.clip_grads_(grads, max_norm)
+    norm = _clip_run(grads, outs, max_norm, dev)
+    torch.autograd.graph.increment_version(outs)
+    return norm
+
+
 class PhaseScanPlan:
     """A phase-flavour scan with every output / saved / gradient buffer allocated once, so
     fwd() and bwd() are exactly one library call each and can be timed or captured in a CUDA

@@ -1,0 +1,136 @@
+"""The residual join, gradient clipping and gated feed-forward without a GPU: refusals of the
+Python functions and of the C entry points (host checks, before any launch), struct layouts, fake
+implementations."""
+import ctypes
+import os
+import shutil
+import subprocess
+import tempfile
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from sca2_b200 import _lib, ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 1 << 20  # an address that is never read: every call below is refused first
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+def test_struct_layouts():
+    fields = {"sca2_rnorm_args": (_lib.RNormArgs, ["gate", "sx", "w", "scale", "rows", "d", "z_dtype", "gate_mode", "eps"]),
+              "sca2_rnorm_grads": (_lib.RNormGrads, ["du", "dw", "dpb"]),
+              "sca2_grad_tensor": (_lib.GradTensor, ["dst", "n", "src_dtype", "dst_dtype"])}
+    body = "".join(f'printf("%zu\\n", sizeof({t}));' + "".join(f'printf("%zu\\n", offsetof({t}, {f}));' for f in fs)
+                   for t, (_, fs) in fields.items())
+    with tempfile.TemporaryDirectory() as d:
+        c = os.path.join(d, "p.c")
+        open(c, "w").write('#include <stddef.h>\n#include <stdio.h>\n#include "sca2b200.h"\nint main(void){' + body + "return 0;}")
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", c + ".x"], check=True)
+        got = [int(x) for x in subprocess.run([c + ".x"], capture_output=True, text=True, check=True).stdout.split()]
+    want = [v for cls, fs in fields.values() for v in [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in fs]]
+    assert got == want
+    assert len(ops._grad_table([torch.zeros(3)] * 2, [torch.zeros(3)] * 2)) == 2 * ctypes.sizeof(_lib.GradTensor)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 8)
+    for call in (lambda: ops.residual_norm(x, x, torch.ones(8)), lambda: ops.grad_norm([x]),
+                 lambda: ops.clip_grads([x], 1.0)):
+        with pytest.raises(_lib.Sca2Error, match="CUDA"):
+            call()
+
+
+def test_residual_norm_refusals():
+    with FakeTensorMode():
+        x, w = torch.empty(4, 8, device="cuda"), torch.empty(8, device="cuda")
+        half, long = torch.empty(4, 8, device="cuda", dtype=torch.float16), torch.empty(4, 9, device="cuda")
+        bad = [dict(u=long), dict(u=x[:3]), dict(weight=torch.empty(9, device="cuda")), dict(bias=w), dict(post_bias=w),
+               dict(weight=w, kind="batch"), dict(weight=w, out_dtype=torch.float16), dict(u=half),
+               dict(gate=torch.empty(4, 2, device="cuda")), dict(gate=torch.empty(4, device="cuda")),
+               dict(gate=torch.empty(3, 8, device="cuda")), dict(scale=torch.empty(1, device="cuda"))]
+        for kw in bad:
+            kw = dict(kw)
+            u = kw.pop("u", x)
+            with pytest.raises(_lib.Sca2Error):
+                ops.residual_norm(x, u, kw.pop("weight", None), kw.pop("bias", None), **kw)
+        with pytest.raises(_lib.Sca2Error):
+            ops.residual_norm(torch.empty((), device="cuda"), torch.empty((), device="cuda"))
+
+
+def test_residual_norm_entry_refusals():
+    lib = _lib.load()
+
+    def args(**kw):
+        a = _lib.RNormArgs()
+        a.x = a.u = a.w = P
+        a.sx = a.su = a.rows = a.d = 8
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+    bad = [dict(d=0), dict(rows=-1), dict(x=None), dict(u=None), dict(sx=7), dict(su=0), dict(x_dtype=2), dict(u_dtype=-1),
+           dict(z_dtype=5), dict(kind=2), dict(gate_mode=3), dict(gate_mode=1), dict(gate_mode=2, gate=P, sg=7),
+           dict(eps=-1.0), dict(eps=float("nan")), dict(pb=P), dict(b=P, w=None), dict(b=P, kind=1), dict(pb=P, pw=P, kind=1)]
+    g = _lib.RNormGrads(P, P, P, P, P, P, P, P)
+    for kw in bad:
+        assert lib.sca2_residual_norm_fwd(args(**kw), P, P, None, None) == _lib.SCA2_ERR_ARG, kw
+        assert lib.sca2_residual_norm_bwd(args(**kw), P, P, P, g, P, 1 << 40, None) == _lib.SCA2_ERR_ARG, kw
+        assert lib.sca2_last_error().startswith(b"residual_norm")
+    assert lib.sca2_residual_norm_fwd(args(d=4097, sx=4097, su=4097), P, P, None, None) == _lib.SCA2_ERR_UNSUPPORTED
+    assert lib.sca2_residual_norm_fwd(None, P, P, None, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_residual_norm_fwd(args(), None, P, None, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_residual_norm_fwd(args(w=None), P, P, None, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_residual_norm_fwd(args(), P, P, P + 4, None) == _lib.SCA2_ERR_ARG
+    n = lib.sca2_residual_norm_work_bytes(8, 8)
+    assert n > 0 and lib.sca2_residual_norm_work_bytes(0, 8) == 0 and lib.sca2_residual_norm_work_bytes(8, 5000) == 0
+    bwd = lambda a=None, st=P, dz=P, gr=g, wk=P, nb=n: lib.sca2_residual_norm_bwd(a or args(), st, P, dz, gr, wk, nb, None)
+    for kw in (dict(st=None), dict(st=P + 4), dict(gr=None), dict(wk=None), dict(wk=P + 8), dict(nb=n - 1),
+               dict(a=args(w=None)), dict(gr=_lib.RNormGrads(None, P)), dict(gr=_lib.RNormGrads(P, None)),
+               dict(a=args(gate_mode=1, gate=P, sg=1), gr=_lib.RNormGrads(P, P, None))):
+        assert bwd(**kw) == _lib.SCA2_ERR_ARG, kw
+
+
+def test_clip_refusals():
+    with FakeTensorMode():
+        t, h = torch.empty(8, device="cuda"), torch.empty(8, device="cuda", dtype=torch.float16)
+        for call in (lambda: ops.clip_grads([t], -1.0), lambda: ops.clip_grads([t], float("nan")),
+                     lambda: ops.clip_grads([h], 1.0), lambda: ops.grad_norm([h]), lambda: ops.grad_norm([None]),
+                     lambda: ops.clip_grads([t], 1.0, out=[]), lambda: ops.clip_grads([t], 1.0, out=[h]),
+                     lambda: ops.clip_grads([t], 1.0, out=[t[:4]]),
+                     lambda: ops.clip_grads([t.view(2, 4)], 1.0, out=[torch.empty(4, 2, device="cuda").t()])):
+            with pytest.raises(_lib.Sca2Error):
+                call()
+
+
+def test_clip_entry_refusals():
+    import struct
+    lib = _lib.load()
+    one = lambda s=P, d=P, n=8, a=0, b=0: struct.pack("=QQqii", s, d, n, a, b)
+    big = 1 << 40
+    for t in (one(s=0), one(d=0), one(n=-1), one(n=(1 << 41) + 1), one(a=2), one(b=3), one(s=P + 2), one(d=P + 2),
+              one(a=1), one(d=P + 4), one() + one(), one(d=P + 4096) + one(s=P + 4096, d=P + 8192)):
+        assert lib.sca2_clip_grads(t, len(t) // 32, 1.0, P, P, big, None) == _lib.SCA2_ERR_ARG, t
+    t = one()
+    assert lib.sca2_clip_grads(t, -1, 1.0, P, P, big, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads(None, 1, 1.0, P, P, big, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads(t, 1, -1.0, P, P, big, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads(t, 1, 1.0, None, P, big, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads(t, 1, 1.0, P, None, big, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads(t, 1, 1.0, P, P + 4, big, None) == _lib.SCA2_ERR_ARG
+    n = lib.sca2_clip_grads_work_bytes(t, 1)
+    assert n >= 8 and lib.sca2_clip_grads(t, 1, 1.0, P, P, n - 1, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_grad_norm(t, 1, P, P, n - 1, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_clip_grads_work_bytes(one(n=-1), 1) == 0
+
+
+def test_fake_shapes():
+    with FakeTensorMode():
+        x, u = torch.empty(2, 3, 40, device="cuda"), torch.empty(2, 3, 40, device="cuda", dtype=torch.bfloat16)
+        w, g = torch.empty(40, device="cuda"), torch.empty(2, 3, 1, device="cuda", dtype=torch.bfloat16)
+        y, z, st = torch.ops.sca2b200.residual_norm_fwd(x, u, w, None, g, w, None, None, 0, 1e-5, torch.bfloat16, True)
+        assert y.shape == z.shape == x.shape and y.dtype == x.dtype and z.dtype == u.dtype and st.shape == (6, 4)
+        out = torch.ops.sca2b200.residual_norm_bwd(x, u, w, None, g, w, None, None, 0, 1e-5, torch.bfloat16, st, y, z)
+        assert [tuple(t.shape) for t in out] == [(2, 3, 40), (2, 3, 40), (40,), (0,), (2, 3, 1), (40,), (0,), (0,)]
+        assert torch.ops.sca2b200.grad_norm([x, w]).shape == ()
+        assert torch.ops.sca2b200.clip_grads_([x, w], 1.0).shape == ()
