@@ -399,6 +399,35 @@ SCA2_API int sca2_scan_fwd_bwd_noalloc(const sca2_scan_args* a, sca2_out o, floa
                                        sca2_out dO, const float* dS_final,
                                        const sca2_scan_grads* gr, void* stream);
 
+/* ---- gated feed-forward ------------------------------------------------------------------------
+ *     g = x w_gate^T,  u = x w_up^T,  h = act(g) * u
+ * the two projections of a gated feed-forward block, the activation and the product in one kernel
+ * (bf16 operands, fp32 accumulators, h rounded once).  The layers' FFN of the reference has one
+ * projection and GELU (lapa/layer.py:564-566); this is its gated form.  All tensors bf16; d and f
+ * multiples of 8, rows 16-byte aligned. */
+enum sca2_act { SCA2_ACT_SILU = 0, SCA2_ACT_GELU = 1 };   /* gelu: the exact form (erf) */
+
+typedef struct sca2_ffn_args {
+  const void* x;        /* (rows, d), row stride ldx */
+  const void* w_gate;   /* (f, d), row stride ldg */
+  const void* w_up;     /* (f, d), row stride ldu */
+  int64_t ldx, ldg, ldu;  /* in values, multiples of 8 */
+  int64_t rows;
+  int32_t d, f;
+  int32_t act;          /* sca2_act */
+} sca2_ffn_args;
+
+/* h (rows, f) dense. */
+SCA2_API int sca2_gated_ffn_fwd(const sca2_ffn_args* a, void* h, void* stream);
+
+/* Workspace of the backward: bf16 dg and du (rows, f), and fp32 parts of the weight gradients. */
+SCA2_API int64_t sca2_gated_ffn_work_bytes(int64_t rows, int32_t d, int32_t f);
+
+/* Gradients from dh (rows, f) dense: dx (rows, d) dense or NULL, dw_gate and dw_up (f, d) dense or
+ * both NULL, all written.  g and u are recomputed.  work 256-byte aligned. */
+SCA2_API int sca2_gated_ffn_bwd(const sca2_ffn_args* a, const void* dh, void* dx, void* dw_gate, void* dw_up,
+                   void* work, int64_t work_bytes, void* stream);
+
 /* ---- residual join with norms -----------------------------------------------------------------
  * Per row of width d:
  *     p = N_post(u) (or u),   y = x + scale * sigmoid(gate) * p,   z = N(y)

@@ -82,6 +82,13 @@ class DScanGrads(C.Structure):
     ]
 
 
+class FfnArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("ldx", C.c_int64), ("ldg", C.c_int64),
+        ("ldu", C.c_int64), ("rows", C.c_int64), ("d", C.c_int32), ("f", C.c_int32), ("act", C.c_int32),
+    ]
+
+
 class RNormArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("u", C.c_void_p), ("gate", C.c_void_p),
@@ -155,6 +162,10 @@ SIGNATURES = [
                                  C.POINTER(ShortGrads), C.c_void_p, C.c_void_p]),
     ("sca2_scan_fwd_bwd_noalloc", C.c_int, [C.POINTER(ScanArgs), Out, C.c_void_p, Out, C.c_void_p,
                                             C.POINTER(ScanGrads), C.c_void_p]),
+    ("sca2_gated_ffn_fwd", C.c_int, [C.POINTER(FfnArgs), C.c_void_p, C.c_void_p]),
+    ("sca2_gated_ffn_work_bytes", C.c_int64, [C.c_int64, C.c_int32, C.c_int32]),
+    ("sca2_gated_ffn_bwd", C.c_int, [C.POINTER(FfnArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_int64, C.c_void_p]),
     ("sca2_residual_norm_fwd", C.c_int, [C.POINTER(RNormArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     ("sca2_residual_norm_work_bytes", C.c_int64, [C.c_int64, C.c_int32]),
     ("sca2_residual_norm_bwd", C.c_int, [C.POINTER(RNormArgs), C.c_void_p, C.c_void_p, C.c_void_p,

@@ -79,6 +79,8 @@ cudaError_t cp_read_faults(unsigned int* out);
 // phase_cp.cu
 cudaError_t pcp_read_faults(unsigned int* out);
 bool pcp_value_tma(const sca2_scan_args& p, const float* cstates);
+// gated_ffn.cu
+cudaError_t ffn_read_faults(unsigned int* out);
 // phase_proj.cu
 size_t proj_work_floats(int B, int T, int H, int Mh);
 cudaError_t proj_bwd(int B, int T, int H, int Mh, int dtype, const float* work, const sca2_tok& kh,
@@ -160,14 +162,15 @@ const char* sca2_version(void) { return "sca2b200 0.1.0 (sm_100a)"; }
 int sca2_fault_status(uint32_t* faults) {
   if (!faults) return fail(SCA2_ERR_ARG, "null output");
   unsigned int f = 0;
-  unsigned int fb = 0, fp = 0, fc = 0, fq = 0;
+  unsigned int fb = 0, fp = 0, fc = 0, fq = 0, ff = 0;
   cudaError_t e = sca2::tc_read_faults(&f);
   if (e == cudaSuccess) e = sca2::tc_read_faults_bwd(&fb);
   if (e == cudaSuccess) e = sca2::tc_read_faults_prep(&fp);
   if (e == cudaSuccess) e = sca2::cp_read_faults(&fc);
   if (e == cudaSuccess) e = sca2::pcp_read_faults(&fq);
+  if (e == cudaSuccess) e = sca2::ffn_read_faults(&ff);
   if (e != cudaSuccess) return cuda_fail(e, "sca2_fault_status");
-  *faults = f | fb | fp | fc | fq;
+  *faults = f | fb | fp | fc | fq | ff;
   return SCA2_OK;
 }
 

@@ -688,7 +688,7 @@ bool pcp_covers(const sca2_scan_args& p, const float* cstates) {
 
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime (no link against
 // the driver library); nullptr where the driver does not provide it
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static std::once_flag once;
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   std::call_once(once, [] {

@@ -10,6 +10,7 @@
     rms_heads(o)                                          multi-head read gathered + RMS
     layer_norm(x, w, b, eps)                              the layers' LayerNorm (fwd + bwd kernels)
     linear16(x, w, sizes)                                 x w^T to 16 bits on bf16 tensor cores
+    gated_ffn(x, w_gate, w_up, act)                       act(x w_gate^T) * (x w_up^T), bf16
     residual_norm(x, u, weight, ...) -> (y, z)            residual join with the norms on both sides
     grad_norm(grads), clip_grads(grads, max_norm, out)    global gradient norm, clipping
 
@@ -1297,6 +1298,137 @@ def linear16(x: torch.Tensor, w: torch.Tensor, sizes: Tuple[int, ...]) -> Tuple[
 # ======================================================================================
 #  preallocated plans (benchmarks, CUDA-graph capture)
 # ======================================================================================
+# ======================================================================================
+#  gated feed-forward projections
+# ======================================================================================
+_ACT = {"silu": 0, "gelu": 1}
+
+
+def _ffn_rows(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+    """t (..., width) as 16-byte aligned rows with a stride of a multiple of 8 values (a copy only
+    where it is not laid out so), and the stride."""
+    v, ld = _row_view(t, width)
+    if v.data_ptr() % 16 or ld % 8:
+        v, ld = v.clone(memory_format=torch.contiguous_format), width
+    return v, ld
+
+
+def _ffn_args(x, wg, wu, act):
+    a = _lib.FfnArgs()
+    d = x.shape[-1]
+    (x, a.ldx), (wg, a.ldg), (wu, a.ldu) = _ffn_rows(x, d), _ffn_rows(wg, d), _ffn_rows(wu, d)
+    a.x, a.w_gate, a.w_up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
+    a.rows, a.d, a.f, a.act = x.numel() // d, d, wg.shape[0], act
+    return a, (x, wg, wu)  # the tensors stay alive until the launch is queued
+
+
+def _gated_ffn_run(x, wg, wu, act: int):
+    dev = x.device
+    h = torch.empty(*x.shape[:-1], wg.shape[0], device=dev, dtype=torch.bfloat16)
+    a, hold = _ffn_args(x, wg, wu, act)
+    with _on(dev):
+        _lib.check(_lib.load().sca2_gated_ffn_fwd(a, h.data_ptr(), _stream()), "gated_ffn")
+    return h
+
+
+def _gated_ffn_bwd_run(x, wg, wu, act: int, dh, need_x: bool, need_w: bool):
+    dev = x.device
+    a, hold = _ffn_args(x, wg, wu, act)
+    dh, _ = _ffn_rows(dh.to(torch.bfloat16).contiguous(), a.f)
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_x else None
+    dwg, dwu = (torch.empty(wg.shape, device=dev, dtype=wg.dtype) if need_w else None for _ in range(2))
+    lib = _lib.load()
+    n = lib.sca2_gated_ffn_work_bytes(a.rows, a.d, a.f)
+    work = torch.empty(n, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        _lib.check(lib.sca2_gated_ffn_bwd(a, dh.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu), work.data_ptr(), n,
+                                          _stream()), "gated_ffn_bwd")
+    return dx, dwg, dwu
+
+
+@torch.library.custom_op("sca2b200::gated_ffn_fwd", mutates_args=())
+def _gated_ffn_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, act: int) -> torch.Tensor:
+    """sca2_gated_ffn_fwd: h (..., f)."""
+    return _gated_ffn_run(x, wg, wu, act)
+
+
+@_gated_ffn_fwd.register_fake
+def _(x, wg, wu, act):
+    return x.new_empty(*x.shape[:-1], wg.shape[0])
+
+
+@torch.library.custom_op("sca2b200::gated_ffn_bwd", mutates_args=())
+def _gated_ffn_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, act: int, dh: torch.Tensor, need_x: bool,
+                   need_w: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """sca2_gated_ffn_bwd: dx, dw_gate, dw_up (empty where not needed)."""
+    return tuple(x.new_empty(0) if t is None else t for t in _gated_ffn_bwd_run(x, wg, wu, act, dh, need_x, need_w))
+
+
+@_gated_ffn_bwd.register_fake
+def _(x, wg, wu, act, dh, need_x, need_w):
+    e = lambda t, need: t.new_empty(t.shape) if need else t.new_empty(0)
+    return e(x, need_x), e(wg, need_w), e(wu, need_w)
+
+
+def _gated_ffn_setup(ctx, inputs, output):
+    x, wg, wu, ctx.act = inputs
+    ctx.save_for_backward(x, wg, wu)
+
+
+def _gated_ffn_backward(ctx, dh):
+    nx, nw = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+    dx, dwg, dwu = torch.ops.sca2b200.gated_ffn_bwd(*ctx.saved_tensors, ctx.act, dh, nx, nw)
+    return dx if nx else None, dwg if nw else None, dwu if nw else None, None
+
+
+_gated_ffn_fwd.register_autograd(_gated_ffn_backward, setup_context=_gated_ffn_setup)
+
+
+class _GatedFFN(torch.autograd.Function):
+    """The eager path of gated_ffn: the same two calls without the operator dispatch."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, act):
+        ctx.save_for_backward(x, wg, wu)
+        ctx.act = act
+        return _gated_ffn_run(x, wg, wu, act)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        need = ctx.needs_input_grad
+        return (*_gated_ffn_bwd_run(*ctx.saved_tensors, ctx.act, dh, need[0], need[1] or need[2]), None)
+
+
+def gated_ffn_supported(d: int, f: int) -> bool:
+    """Widths that gated_ffn takes: multiples of 8."""
+    return d >= 8 and f >= 8 and d % 8 == 0 and f % 8 == 0
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu") -> torch.Tensor:
+    """h = act(x w_gate^T) * (x w_up^T): both projections of a gated feed-forward block, the
+    activation ("silu", or "gelu" in its exact form) and the product in one kernel.  x (..., d),
+    weights (f, d), all bf16 with fp32 accumulation, d and f multiples of 8; returns h (..., f).
+    Differentiable once in all three; the backward recomputes the projections, so nothing but the
+    inputs is kept.  The weights may be the halves of one (2 f, d) tensor."""
+    _need_cuda(x, w_gate, w_up)
+    E = _lib.Sca2Error
+    if act not in _ACT:
+        raise E(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
+    if any(t.dtype != torch.bfloat16 for t in (x, w_gate, w_up)):
+        raise E("gated_ffn: x and the weights must be bfloat16")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1]:
+        raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(w_gate.shape)} and "
+                f"{tuple(w_up.shape)}")
+    if not gated_ffn_supported(x.shape[-1], w_gate.shape[0]):
+        raise E(f"gated_ffn: d and f must be multiples of 8, got {x.shape[-1]} and {w_gate.shape[0]}")
+    if torch.compiler.is_compiling():
+        return torch.ops.sca2b200.gated_ffn_fwd(x, w_gate, w_up, _ACT[act])
+    if _wants_grad(x, w_gate, w_up):
+        return _GatedFFN.apply(x, w_gate, w_up, _ACT[act])
+    return _gated_ffn_run(x, w_gate, w_up, _ACT[act])
+
+
 # ======================================================================================
 #  residual join with the norms on both sides of it
 # ======================================================================================

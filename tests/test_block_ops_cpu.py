@@ -19,7 +19,8 @@ P = 1 << 20  # an address that is never read: every call below is refused first
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
 def test_struct_layouts():
-    fields = {"sca2_rnorm_args": (_lib.RNormArgs, ["gate", "sx", "w", "scale", "rows", "d", "z_dtype", "gate_mode", "eps"]),
+    fields = {"sca2_ffn_args": (_lib.FfnArgs, ["w_up", "ldx", "ldu", "rows", "d", "f", "act"]),
+              "sca2_rnorm_args": (_lib.RNormArgs, ["gate", "sx", "w", "scale", "rows", "d", "z_dtype", "gate_mode", "eps"]),
               "sca2_rnorm_grads": (_lib.RNormGrads, ["du", "dw", "dpb"]),
               "sca2_grad_tensor": (_lib.GradTensor, ["dst", "n", "src_dtype", "dst_dtype"])}
     body = "".join(f'printf("%zu\\n", sizeof({t}));' + "".join(f'printf("%zu\\n", offsetof({t}, {f}));' for f in fs)
@@ -37,7 +38,7 @@ def test_struct_layouts():
 def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 8)
     for call in (lambda: ops.residual_norm(x, x, torch.ones(8)), lambda: ops.grad_norm([x]),
-                 lambda: ops.clip_grads([x], 1.0)):
+                 lambda: ops.clip_grads([x], 1.0), lambda: ops.gated_ffn(x.bfloat16(), x.bfloat16(), x.bfloat16())):
         with pytest.raises(_lib.Sca2Error, match="CUDA"):
             call()
 
@@ -124,8 +125,50 @@ def test_clip_entry_refusals():
     assert lib.sca2_clip_grads_work_bytes(one(n=-1), 1) == 0
 
 
+def test_gated_ffn_refusals():
+    assert ops.gated_ffn_supported(8, 16) and not ops.gated_ffn_supported(12, 16) and not ops.gated_ffn_supported(8, 4)
+    with FakeTensorMode():
+        e = lambda *s, t=torch.bfloat16: torch.empty(*s, device="cuda", dtype=t)
+        x, w = e(4, 16), e(24, 16)
+        for args in ((x, w, e(24, 8)), (x, w, e(32, 16)), (e(4, 8), w, w), (x, e(16), e(16)), (x, e(20, 16), e(20, 16)),
+                     (e(4, 12), e(24, 12), e(24, 12)), (e(1).squeeze(0), w, w), (x, w, w, "relu"), (e(4, 16, t=torch.float32), w, w),
+                     (x, w, e(24, 16, t=torch.float32)), (x, w, e(24, 16, t=torch.float16))):
+            with pytest.raises(_lib.Sca2Error):
+                ops.gated_ffn(*args)
+
+
+def test_gated_ffn_entry_refusals():
+    lib = _lib.load()
+
+    def args(**kw):
+        a = _lib.FfnArgs(P, P, P, 16, 16, 16, 300, 16, 24, 0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+    bad = [dict(x=None), dict(w_gate=None), dict(w_up=None), dict(rows=-1), dict(d=0), dict(f=0), dict(act=2), dict(ldx=8),
+           dict(ldx=20), dict(ldg=8), dict(ldu=12), dict(x=P + 8), dict(w_gate=P + 2), dict(w_up=P + 4)]
+    wide = [dict(d=12), dict(f=20), dict(rows=(1 << 30) + 1), dict(f=1 << 21), dict(rows=1 << 30, f=1 << 20)]
+    n = lib.sca2_gated_ffn_work_bytes(300, 16, 24)
+    assert n > 0 and lib.sca2_gated_ffn_work_bytes(0, 16, 24) == 0
+    for kw, code in [(b, _lib.SCA2_ERR_ARG) for b in bad] + [(b, _lib.SCA2_ERR_UNSUPPORTED) for b in wide]:
+        assert lib.sca2_gated_ffn_fwd(args(**kw), P, None) == code, kw
+        assert lib.sca2_gated_ffn_bwd(args(**kw), P, P, P, P, P, n, None) == code, kw
+    assert lib.sca2_gated_ffn_fwd(None, P, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_gated_ffn_fwd(args(), None, None) == _lib.SCA2_ERR_ARG
+    assert lib.sca2_gated_ffn_fwd(args(), P + 2, None) == _lib.SCA2_ERR_ARG
+    bwd = lambda dh=P, dx=P, g=P, u=P, w=P, nb=n: lib.sca2_gated_ffn_bwd(args(), dh, dx, g, u, w, nb, None)
+    for kw in (dict(dh=None), dict(dh=P + 8), dict(dx=P + 8), dict(g=None), dict(u=None), dict(g=P + 2), dict(w=None),
+               dict(w=P + 128), dict(nb=n - 1)):
+        assert bwd(**kw) == _lib.SCA2_ERR_ARG, kw
+
+
 def test_fake_shapes():
     with FakeTensorMode():
+        b, w2 = torch.empty(2, 3, 16, device="cuda", dtype=torch.bfloat16), torch.empty(24, 16, device="cuda", dtype=torch.bfloat16)
+        h = torch.ops.sca2b200.gated_ffn_fwd(b, w2, w2, 0)
+        assert h.shape == (2, 3, 24) and h.dtype == torch.bfloat16
+        out = torch.ops.sca2b200.gated_ffn_bwd(b, w2, w2, 0, h, True, False)
+        assert [tuple(t.shape) for t in out] == [(2, 3, 16), (0,), (0,)]
         x, u = torch.empty(2, 3, 40, device="cuda"), torch.empty(2, 3, 40, device="cuda", dtype=torch.bfloat16)
         w, g = torch.empty(40, device="cuda"), torch.empty(2, 3, 1, device="cuda", dtype=torch.bfloat16)
         y, z, st = torch.ops.sca2b200.residual_norm_fwd(x, u, w, None, g, w, None, None, 0, 1e-5, torch.bfloat16, True)
