@@ -24,9 +24,18 @@ constructors:
 
 Parameter and state names follow those layers (n, <slots>, mix, fn, ff.0, ff.2, cw), so a
 reference layer's state_dict loads with strict=True and decode states are interchangeable;
-LayerCfg is the reference's configuration record field for field.  The heads run on the
-sm_100a kernels; norms, the mix projection and the FFN are torch modules (cuBLAS under
-autocast).
+LayerCfg is the reference's configuration record field for field, with one field of this package's
+own (`tail`).  The heads run on the sm_100a kernels; norms, the mix projection and the FFN are torch
+modules (cuBLAS under autocast).
+
+The block's tail has options that the reference's layers lack (TailCfg, off by default; then
+parameters, names and results are the reference layers'): a gated FFN, a norm after each of the two
+branches, a gate and a residual scale.  With any of the last three on, each branch joins the
+residual stream through one kernel (ops.residual_norm), which also forms the norm before the FFN;
+with the gated FFN its two projections, activation and product are one kernel (ops.gated_ffn):
+
+    y = x + s1 * sigmoid(G1 z) * N1(mix(concat_s u_s)),   f = LN(y)         join1
+    y = y + s2 * sigmoid(G2 f) * N2(W_down(act(W_gate f) * (W_up f)))       join2, ff
 """
 from __future__ import annotations
 
@@ -44,7 +53,7 @@ from .heads import LaplaceConfig
 
 @dataclass
 class LayerCfg:
-    """Field for field the reference's LayerCfg (sca2/ref.py:281-331)."""
+    """Field for field the reference's LayerCfg (sca2/ref.py:281-331), and `tail`."""
     d: int = 128
     Mc: int = 64
     Md: int = 16
@@ -69,6 +78,27 @@ class LayerCfg:
     gdn_heads: int = 3
     gdn_head_k: int = 60
     gdn_expand_v: float = 1.0
+    tail: Optional["TailCfg"] = None  # not the reference's: options of the block's tail
+
+
+@dataclass
+class TailCfg:
+    """Options of a block's tail (module docstring).  ffn_act: "silu" or "gelu" for the gated FFN,
+    "" for the plain one.  post_norm: a LayerNorm on each branch's output.  gate: "token" or
+    "channel" for a learned sigmoid gate on it, from the branch's normed input.  res_scale: > 0 for
+    a learned residual scale for each channel that begins there."""
+    ffn_act: str = ""
+    post_norm: bool = False
+    gate: str = ""
+    res_scale: float = 0.0
+
+    def __post_init__(self):
+        if self.ffn_act not in ("", "silu", "gelu") or self.gate not in ("", "token", "channel") or self.res_scale < 0:
+            raise ValueError(f"bad tail options: {self}")
+
+    @property
+    def joined(self) -> bool:
+        return self.post_norm or bool(self.gate) or self.res_scale > 0
 
 
 class LayerNorm(nn.LayerNorm):
@@ -84,13 +114,55 @@ class LayerNorm(nn.LayerNorm):
         return super().forward(x)
 
 
+class GatedFFN(nn.Module):
+    """down(act(gate(x)) * up(x)), no biases.  In bf16 (autocast, or bf16 modules) the two
+    projections, the activation and the product run as one kernel (ops.gated_ffn) for widths that
+    it covers; in fp32 they are torch's."""
+
+    def __init__(self, d: int, ff: int, act: str = "silu"):
+        super().__init__()
+        self.act = act
+        self.gate = nn.Linear(d, ff, bias=False)
+        self.up = nn.Linear(d, ff, bias=False)
+        self.down = nn.Linear(ff, d, bias=False)
+
+    def forward(self, x):
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else x.dtype
+        if x.is_cuda and dt == torch.bfloat16 and ops.gated_ffn_supported(x.shape[-1], self.gate.out_features):
+            h = ops.gated_ffn(x.to(dt), self.gate.weight.to(dt), self.up.weight.to(dt), self.act)
+        else:
+            h = (F.silu if self.act == "silu" else F.gelu)(self.gate(x)) * self.up(x)
+        return self.down(h)
+
+
+class ResidualJoin(nn.Module):
+    """x + scale * sigmoid(gate(z)) * norm(u) for a branch's output u and its normed input z, and
+    the norm of the sum for the next branch, in one kernel (ops.residual_norm)."""
+
+    def __init__(self, d: int, tail: TailCfg, eps: float):
+        super().__init__()
+        self.norm = nn.LayerNorm(d, eps) if tail.post_norm else None
+        self.gate = nn.Linear(d, d if tail.gate == "channel" else 1) if tail.gate else None
+        self.scale = nn.Parameter(torch.full((d,), float(tail.res_scale))) if tail.res_scale > 0 else None
+        self.eps = eps
+
+    def forward(self, x, u, z, next_norm: Optional[nn.LayerNorm] = None):
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else x.dtype
+        w, b = (next_norm.weight, next_norm.bias) if next_norm is not None else (None, None)
+        pw, pb = (self.norm.weight, self.norm.bias) if self.norm is not None else (None, None)
+        return ops.residual_norm(x, u, w, b, gate=self.gate(z) if self.gate is not None else None, scale=self.scale,
+                                 post_weight=pw, post_bias=pb, eps=self.eps,
+                                 out_dtype=dt if dt == torch.bfloat16 else x.dtype)
+
+
 Slot = Tuple[str, str]  # (module attribute, state key)
 
 
 class MixerLayer(nn.Module):
     """One pre-norm residual block over a table of parallel head slots (module docstring)."""
 
-    def __init__(self, d: int, slots: Sequence[Tuple[str, str, nn.Module]], mix_in: int, ff: int, conv: int = 0):
+    def __init__(self, d: int, slots: Sequence[Tuple[str, str, nn.Module]], mix_in: int, ff: int, conv: int = 0,
+                 tail: Optional[TailCfg] = None):
         super().__init__()
         self.d = d
         self.n = LayerNorm(d)
@@ -99,7 +171,13 @@ class MixerLayer(nn.Module):
             self.add_module(attr, module)
         self.mix = nn.Linear(mix_in, d)
         self.fn = LayerNorm(d)
-        self.ff = nn.Sequential(nn.Linear(d, ff), nn.GELU(), nn.Linear(ff, d))
+        if tail is not None and tail.ffn_act:
+            self.ff = GatedFFN(d, ff, tail.ffn_act)
+        else:
+            self.ff = nn.Sequential(nn.Linear(d, ff), nn.GELU(), nn.Linear(ff, d))
+        self.joined = tail is not None and tail.joined
+        if self.joined:
+            self.join1, self.join2 = (ResidualJoin(d, tail, self.fn.eps) for _ in range(2))
         self.k = conv
         if conv:
             w = torch.zeros(d, 1, conv)
@@ -118,13 +196,16 @@ class MixerLayer(nn.Module):
         return st
 
     # ---- the residual tail shared by prefill and step ---------------------------------
-    def _tail(self, x: torch.Tensor, us) -> torch.Tensor:
+    def _tail(self, x: torch.Tensor, z: torch.Tensor, us) -> torch.Tensor:
         if torch.is_autocast_enabled() and x.is_cuda:
             # the mix product reads its input in the autocast dtype: cast each slot's read-out
             # before joining them (the same elementwise rounding as casting the joined fp32
             # tensor, without materialising it; the gradients come back per slot, contiguous)
             dt = torch.get_autocast_dtype("cuda")
             us = [u.to(dt) for u in us]
+        if self.joined:
+            y, f = self.join1(x, self.mix(torch.cat(us, -1)), z, self.fn)
+            return self.join2(y, self.ff(f), f)[0]
         y = x + self.mix(torch.cat(us, -1))
         return y + self.ff(self.fn(y))
 
@@ -145,7 +226,7 @@ class MixerLayer(nn.Module):
             u, new[key] = getattr(self, attr).prefill(z, h, st[key])
             us.append(u)
         new["z_prev"] = z[:, -1]
-        return self._tail(x, us), new
+        return self._tail(x, z, us), new
 
     def step(self, x_t: torch.Tensor, state: Dict):
         z = self.n(x_t)
@@ -160,7 +241,7 @@ class MixerLayer(nn.Module):
             u, new[key] = getattr(self, attr).step(z, h, state[key])
             us.append(u)
         new["z_prev"] = z
-        return self._tail(x_t, us), new
+        return self._tail(x_t, z, us), new
 
 
 # ---- the reference's layer families as slot tables --------------------------------------
@@ -185,7 +266,7 @@ class SCA2Layer(MixerLayer):
         dv = _dv(cfg)
         c = _c_head(cfg, c_cls or heads.CHeadRef, cfg.d, dv)
         dh = _d_head(cfg, d_cls or heads.DHeadRef, cfg.d, dv)
-        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, conv)
+        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, conv, cfg.tail)
         self.cfg = cfg
 
 
@@ -213,7 +294,7 @@ class ShortLayer(MixerLayer):
         dv = _dv(cfg)
         c = _c_head(cfg, self.C_CLS, cfg.d, dv)
         dh = heads.CHeadShort(cfg.d, cfg.Ls, dv, theta_scale=cfg.theta_scale or 0.02)
-        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff)
+        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, tail=cfg.tail)
         self.cfg = cfg
         if hasattr(c, "lam_raw"):
             c.LAM_MAX = cfg.lam_max if cfg.lam_max is not None else 1.0 / cfg.Ls
@@ -229,11 +310,12 @@ class ShortLayerDampH(ShortLayer):
 
 
 class LaplaceAttention(MixerLayer):
-    """Long head || short head (lapa/layer.py:551-600), configured by a LaplaceConfig."""
+    """Long head || short head (lapa/layer.py:551-600), configured by a LaplaceConfig and the
+    options of its tail."""
 
-    def __init__(self, cfg: LaplaceConfig = LaplaceConfig()):
+    def __init__(self, cfg: LaplaceConfig = LaplaceConfig(), tail: Optional[TailCfg] = None):
         super().__init__(cfg.d, [("long", "long", heads.LongHead(cfg)), ("short", "short", heads.ShortHead(cfg))],
-                         4 * cfg.dv, cfg.ff)
+                         4 * cfg.dv, cfg.ff, tail=tail)
         self.cfg = cfg
 
     def _head_state(self, head, B, device, dtype):

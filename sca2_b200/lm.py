@@ -22,7 +22,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .heads import LaplaceConfig
-from .layers import GatedLayer, LaplaceAttention, LayerCfg, LayerNorm
+from .layers import GatedLayer, LaplaceAttention, LayerCfg, LayerNorm, TailCfg
 
 
 class LM(nn.Module):
@@ -105,11 +105,13 @@ def next_token(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, g
 
 
 class LaplaceLM(LM):
-    """lapa/model.py LaplaceLM: LaplaceAttention layers with LaplaceConfig(d=d, **cfg)."""
+    """lapa/model.py LaplaceLM: LaplaceAttention layers with LaplaceConfig(d=d, **cfg); `tail`:
+    options of their tails (layers.TailCfg)."""
 
-    def __init__(self, vocab: int, d: int = 128, n_layers: int = 4, tie_embeddings: bool = False, **cfg):
+    def __init__(self, vocab: int, d: int = 128, n_layers: int = 4, tie_embeddings: bool = False,
+                 tail: Optional[TailCfg] = None, **cfg):
         c = LaplaceConfig(d=d, **cfg)
-        super().__init__(lambda i: LaplaceAttention(c), n_layers, vocab, d, tie_embeddings)
+        super().__init__(lambda i: LaplaceAttention(c, tail), n_layers, vocab, d, tie_embeddings)
 
 
 class GatedLM(LM):

@@ -177,3 +177,17 @@ def test_fake_shapes():
         assert [tuple(t.shape) for t in out] == [(2, 3, 40), (2, 3, 40), (40,), (0,), (2, 3, 1), (40,), (0,), (0,)]
         assert torch.ops.sca2b200.grad_norm([x, w]).shape == ()
         assert torch.ops.sca2b200.clip_grads_([x, w], 1.0).shape == ()
+
+
+def test_tail_options():
+    """The tail's parameters by option, the reference's names without any; bad options refused."""
+    from sca2_b200 import layers
+    cfg = lambda **t: layers.LayerCfg(d=32, Mc=16, Md=4, G=4, ff=48, freq="rope", dv=32, tail=layers.TailCfg(**t) if t else None)
+    plain = set(layers.SCA2Layer(cfg()).state_dict())
+    assert set(layers.SCA2Layer(cfg(res_scale=0.0, gate="")).state_dict()) == plain
+    full = set(layers.SCA2Layer(cfg(ffn_act="silu", post_norm=True, gate="token", res_scale=0.1)).state_dict())
+    assert {"ff.gate.weight", "ff.up.weight", "ff.down.weight", "join1.norm.weight", "join2.gate.bias", "join1.scale"} <= full
+    assert {k for k in plain if not k.startswith("ff.")} <= full
+    for bad in (dict(ffn_act="relu"), dict(gate="row"), dict(res_scale=-1.0)):
+        with pytest.raises(ValueError):
+            layers.TailCfg(**bad)
