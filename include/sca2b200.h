@@ -487,9 +487,9 @@ typedef struct sca2_grad_tensor {
   int32_t dst_dtype;
 } sca2_grad_tensor;
 
-/* Bytes of the device workspace of the two calls below (the list itself is host memory and is
- * not kept: its contents travel as kernel parameters). */
-SCA2_API int64_t sca2_clip_grads_work_bytes(const sca2_grad_tensor* list, int32_t count);
+/* Bytes of the device workspace of the two calls below for a list of `count` tensors (the list
+ * itself is host memory and is not kept: its contents travel as kernel parameters). */
+SCA2_API int64_t sca2_clip_grads_work_bytes(int32_t count);
 
 /* *norm (device, fp32) = the 2-norm of all values of the list together, summed in 64 bits in a
  * fixed order.  count = 0 gives 0.  No counterpart in the reference; the semantics are

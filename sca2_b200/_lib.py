@@ -170,7 +170,7 @@ SIGNATURES = [
     ("sca2_residual_norm_work_bytes", C.c_int64, [C.c_int64, C.c_int32]),
     ("sca2_residual_norm_bwd", C.c_int, [C.POINTER(RNormArgs), C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.POINTER(RNormGrads), C.c_void_p, C.c_int64, C.c_void_p]),
-    ("sca2_clip_grads_work_bytes", C.c_int64, [C.c_void_p, C.c_int32]),
+    ("sca2_clip_grads_work_bytes", C.c_int64, [C.c_int32]),
     ("sca2_grad_norm", C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     ("sca2_clip_grads", C.c_int, [C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     ("sca2_fault_status", C.c_int, [C.POINTER(C.c_uint32)]),
@@ -189,6 +189,8 @@ class Sca2Error(RuntimeError):
 def load(path: str = LIB_PATH):
     """Load (once) and return the library handle with typed symbols."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

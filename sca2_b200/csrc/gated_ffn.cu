@@ -49,9 +49,9 @@ enum Act { SILU, GELU };
 
 constexpr int BK = 64;               // contraction steps of a stage: 128 bytes, one swizzle row
 constexpr int HALF = 128 * BK * 2;   // one operand of one CTA's stage, 16 KB
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;        // four to a quarter of the rows, each a quarter of the columns
 constexpr int NT = 128 + 32 * EPI_WARPS;
-constexpr int STG = 4096;            // one staged output block: 32 rows of 128 bytes
+constexpr int STG = 2048;            // one staged output block: 32 rows of 64 bytes
 constexpr uint64_t WAIT_NS = 4000000000ull;  // a wait gives up after this
 
 template <int MODE>
@@ -60,7 +60,7 @@ struct Layout {
   static constexpr int NSTG = MODE == FWD ? 1 : 2;  // staged output blocks of a warp
   static constexpr int RING = STAGES * 2 * HALF;
   static constexpr int BARS = RING + EPI_WARPS * NSTG * STG;
-  static constexpr int TOTAL = BARS + 256 + 1024;  // 1024: room to align the ring
+  static constexpr int TOTAL = BARS + 320 + 1024;  // 1024: room to align the ring
 };
 
 struct Geo {
@@ -217,9 +217,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
 
-// 16-byte chunk c of row r of a staged 128-byte swizzled block
+// 16-byte chunk c of row r of a staged block, in the 64-byte swizzle (8 rows' stores of one chunk
+// fall on 8 different 16-byte columns of the banks)
 __device__ __forceinline__ uint32_t chunk(uint32_t base, int r, int c) {
-  return base + (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+  return base + (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 __device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -336,8 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
         if (ok) commit2(tfull + 8 * acc);
       }
     }
-  } else if (warp >= 4) {  // ---- epilogue: 32 rows (the warp's quarter of TMEM) x half the columns
-    const int e = warp - 4, q = warp & 3, half = e >> 2;
+  } else if (warp >= 4) {  // ---- epilogue: 32 rows (the warp's quarter of TMEM) x a quarter of the columns
+    const int e = warp - 4, q = warp & 3, part = e >> 2;
     const uint32_t stg = stg0 + e * L::NSTG * STG, dhb = dhbar + 8 * e, tempty0 = map_to(tempty, 0);
     int n = 0;
     for (int u = pair; u < g.units; u += pairs, ++n) {
@@ -345,7 +346,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
       const int acc = n & 1;
       const int row = t.m * 256 + 128 * rank + 32 * q;
       const uint32_t tm = umma::taddr(tmem, 32 * q, 256 * acc);
-      const int hc = t.n * 128 + 64 * half;  // FWD, BACK: first of the warp's 64 columns of h
+      const int hc = t.n * 128 + 32 * part;  // FWD, BACK: first of the warp's 32 columns of h
       if constexpr (MODE == BACK) {
         if (lane == 0) {
           stores_read<0>();
@@ -356,6 +357,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
       if (!__all_sync(0xffffffffu, wait_for(tfull + 8 * acc, (n >> 1) & 1))) break;
       umma::fence_after_sync();
       if constexpr (MODE == FWD || MODE == BACK) {
+        uint32_t rg[32], ru[32];
+        float vg[32], vu[32];
+        ld32(tm + 32 * part, rg);
+        ld32(tm + 128 + 32 * part, ru);
+        umma::ld_wait();
+        umma::take<32>(rg, vg);
+        umma::take<32>(ru, vu);
+        // the accumulator is in registers: the products of the tile after next may have it
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(tempty0 + 8 * acc);
         if constexpr (MODE == BACK) {
           if (!__all_sync(0xffffffffu, wait_for(dhb, n & 1))) break;
         } else {
@@ -363,44 +375,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           __syncwarp();
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t rg[32], ru[32];
-          float vg[32], vu[32];
-          ld32(tm + 64 * half + 32 * c, rg);
-          ld32(tm + 128 + 64 * half + 32 * c, ru);
-          umma::ld_wait();
-          umma::take<32>(rg, vg);
-          umma::take<32>(ru, vu);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t at = chunk(stg, lane, j);
+          if constexpr (MODE == FWD) {
+            float h[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t at = chunk(stg, lane, 4 * c + j);
-            if constexpr (MODE == FWD) {
-              float h[8];
+            for (int i = 0; i < 8; ++i) h[i] = act_of<ACT>(vg[8 * j + i]) * vu[8 * j + i];
+            sts4(at, pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
+          } else {
+            const uint4 w = lds4(at);
+            const float dh[8] = {lo(w.x), hi(w.x), lo(w.y), hi(w.y), lo(w.z), hi(w.z), lo(w.w), hi(w.w)};
+            float dg[8], du[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) h[i] = act_of<ACT>(vg[8 * j + i]) * vu[8 * j + i];
-              sts4(at, pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
-            } else {
-              const uint4 w = lds4(at);
-              const float dh[8] = {lo(w.x), hi(w.x), lo(w.y), hi(w.y), lo(w.z), hi(w.z), lo(w.w), hi(w.w)};
-              float dg[8], du[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float a, da;
-                act_grad<ACT>(vg[8 * j + i], a, da);
-                dg[i] = dh[i] * vu[8 * j + i] * da;
-                du[i] = dh[i] * a;
-              }
-              sts4(chunk(stg + STG, lane, 4 * c + j), pack2(dg[0], dg[1]), pack2(dg[2], dg[3]), pack2(dg[4], dg[5]),
-                   pack2(dg[6], dg[7]));
-              sts4(at, pack2(du[0], du[1]), pack2(du[2], du[3]), pack2(du[4], du[5]), pack2(du[6], du[7]));
+            for (int i = 0; i < 8; ++i) {
+              float a, da;
+              act_grad<ACT>(vg[8 * j + i], a, da);
+              dg[i] = dh[i] * vu[8 * j + i] * da;
+              du[i] = dh[i] * a;
             }
+            sts4(chunk(stg + STG, lane, j), pack2(dg[0], dg[1]), pack2(dg[2], dg[3]), pack2(dg[4], dg[5]),
+                 pack2(dg[6], dg[7]));
+            sts4(at, pack2(du[0], du[1]), pack2(du[2], du[3]), pack2(du[4], du[5]), pack2(du[6], du[7]));
           }
         }
-        umma::fence_before_sync();
         umma::fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          arrive_cluster(tempty0 + 8 * acc);
           if (row < g.rows && hc < g.f) {
             if constexpr (MODE == FWD) {
               store2d(&maps.o0, stg, hc, row);
@@ -415,51 +415,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
         const int limit = MODE == DX ? g.rows : g.f;
         const bool parts = MODE == DW && g.splits > 1;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // 32 columns at a time
+        for (int c = 0; c < 2; ++c) {  // 32 columns at a time
           uint32_t r[32];
           float v[32];
-          ld32(tm + 128 * half + 32 * c, r);
+          ld32(tm + 64 * part + 32 * c, r);
           umma::ld_wait();
           umma::take<32>(r, v);
-          const int col = t.n * 256 + 128 * half + 32 * c;
-          if (parts) {  // 32 fp32 columns fill a staged block
-            const uint32_t sb = stg + (c & 1) * STG;
-            if (lane == 0) stores_read<1>();
+          if (c == 1) {
+            umma::fence_before_sync();
             __syncwarp();
+            if (lane == 0) arrive_cluster(tempty0 + 8 * acc);
+          }
+          const int col = t.n * 256 + 64 * part + 32 * c;
+          if (parts) {  // 16 fp32 columns fill a staged block
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              sts4(chunk(sb, lane, j), __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                   __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-            umma::fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (row < limit && col < g.d) store3d(&maps.o0, sb, col, row, t.split * 2 + t.slice);
-              stores_commit();
-            }
-          } else {  // 64 bf16 columns do
-            const uint32_t sb = stg + (c >> 1) * STG;
-            if ((c & 1) == 0) {
+            for (int k = 0; k < 2; ++k) {
               if (lane == 0) stores_read<1>();
               __syncwarp();
-            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              sts4(chunk(sb, lane, 4 * (c & 1) + j), pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
-                   pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
-            if (c & 1) {
+              for (int j = 0; j < 4; ++j)
+                sts4(chunk(stg + k * STG, lane, j), __float_as_uint(v[16 * k + 4 * j]), __float_as_uint(v[16 * k + 4 * j + 1]),
+                     __float_as_uint(v[16 * k + 4 * j + 2]), __float_as_uint(v[16 * k + 4 * j + 3]));
               umma::fence_async_smem();
               __syncwarp();
               if (lane == 0) {
-                if (row < limit && col - 32 < g.d)
-                  store2d(MODE == DW && t.slice ? &maps.o1 : &maps.o0, sb, col - 32, row);
+                if (row < limit && col + 16 * k < g.d)
+                  store3d(&maps.o0, stg + k * STG, col + 16 * k, row, t.split * 2 + t.slice);
                 stores_commit();
               }
             }
+          } else {  // 32 bf16 columns do
+            if (lane == 0) stores_read<1>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              sts4(chunk(stg + c * STG, lane, j), pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
+                   pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
+            umma::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (row < limit && col < g.d) store2d(MODE == DW && t.slice ? &maps.o1 : &maps.o0, stg + c * STG, col, row);
+              stores_commit();
+            }
           }
         }
-        umma::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(tempty0 + 8 * acc);
       }
     }
     if (lane == 0) stores_done();
@@ -578,21 +577,22 @@ int cuda_fail(cudaError_t e, const char* where) {
   return SCA2_ERR_CUDA;
 }
 
-// map of a (rows, cols) matrix with row stride ld values; boxes of 128 bytes x `box` rows, swizzled
+// map of a (rows, cols) matrix with row stride ld values; swizzled boxes: 64 columns x `box` rows of
+// an operand, 32 x 32 of what the epilogue stages (box = 0)
 bool map2(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, int64_t ld, int box) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t bx[2] = {64, (cuuint32_t)box}, es[2] = {1, 1};
+  const cuuint32_t bx[2] = {box ? 64u : 32u, box ? (cuuint32_t)box : 32u}, es[2] = {1, 1};
   return tensor_map_encoder()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, bx, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // map of the fp32 parts (splits * 2, f, d)
 bool map3(CUtensorMap* m, const void* p, int64_t slices, int64_t f, int64_t d) {
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)f, (cuuint64_t)slices};
   const cuuint64_t strides[2] = {(cuuint64_t)d * 4, (cuuint64_t)(f * d * 4)};
-  const cuuint32_t bx[3] = {32, 32, 1}, es[3] = {1, 1, 1};
+  const cuuint32_t bx[3] = {16, 32, 1}, es[3] = {1, 1, 1};
   return tensor_map_encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides, bx, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -715,7 +715,7 @@ int sca2_gated_ffn_fwd(const sca2_ffn_args* a, void* h, void* stream) {
     Maps m;
     memset(&m, 0, sizeof(m));
     if (!map2(&m.a0, a->x, a->rows, a->d, a->ldx, 128) || !map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 128) ||
-        !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) || !map2(&m.o0, h, a->rows, a->f, a->f, 32))
+        !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) || !map2(&m.o0, h, a->rows, a->f, a->f, 0))
       return fail(SCA2_ERR_CUDA, "gated_ffn: tensor map refused");
     e = launch_act<FWD>(a->act, m, geo_proj(*a), st);
   }
@@ -759,15 +759,15 @@ int sca2_gated_ffn_bwd(const sca2_ffn_args* a, const void* dh, void* dx, void* d
   Maps m;
   memset(&m, 0, sizeof(m));
   if (!map2(&m.a0, a->x, n, a->d, a->ldx, 128) || !map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 128) ||
-      !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) || !map2(&m.o0, dg, n, a->f, a->f, 32) ||
-      !map2(&m.o1, du, n, a->f, a->f, 32) || !map2(&m.dh, dh, n, a->f, a->f, 32))
+      !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) || !map2(&m.o0, dg, n, a->f, a->f, 0) ||
+      !map2(&m.o1, du, n, a->f, a->f, 0) || !map2(&m.dh, dh, n, a->f, a->f, 0))
     return fail(SCA2_ERR_CUDA, refused);
   e = launch_act<BACK>(a->act, m, geo_proj(*a), st);
   if (e == cudaSuccess && dx) {
     memset(&m, 0, sizeof(m));
     if (!map2(&m.a0, dg, n, a->f, a->f, 128) || !map2(&m.a1, du, n, a->f, a->f, 128) ||
         !map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 64) || !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 64) ||
-        !map2(&m.o0, dx, n, a->d, a->d, 32))
+        !map2(&m.o0, dx, n, a->d, a->d, 0))
       return fail(SCA2_ERR_CUDA, refused);
     e = launch<DX, SILU>(m, geo_dx(*a), st);
   }
@@ -777,7 +777,7 @@ int sca2_gated_ffn_bwd(const sca2_ffn_args* a, const void* dh, void* dx, void* d
     bool ok = map2(&m.a0, dg, n, a->f, a->f, 64) && map2(&m.a1, du, n, a->f, a->f, 64) &&
               map2(&m.b0, a->x, n, a->d, a->ldx, 64);
     if (g.splits > 1) ok = ok && map3(&m.o0, part, 2 * g.splits, a->f, a->d);
-    else ok = ok && map2(&m.o0, dw_gate, a->f, a->d, a->d, 32) && map2(&m.o1, dw_up, a->f, a->d, a->d, 32);
+    else ok = ok && map2(&m.o0, dw_gate, a->f, a->d, a->d, 0) && map2(&m.o1, dw_up, a->f, a->d, a->d, 0);
     if (!ok) return fail(SCA2_ERR_CUDA, refused);
     e = launch<DW, SILU>(m, g, st);
     if (e == cudaSuccess && g.splits > 1) {

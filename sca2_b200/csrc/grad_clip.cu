@@ -34,8 +34,8 @@ struct Entry {
   int16_t sdt, ddt;   // SCA2_F32 or SCA2_BF16
 };
 
-// The launch's tensors.  Kernel parameters hold up to 32 764 bytes: 1000 entries, or 100 where
-// they suffice (the parameters are copied at each launch).
+// The launch's tensors.  Kernel parameters hold up to 32 764 bytes: 1000 entries, or a smaller table
+// where it suffices (the parameters are copied at each launch).
 template <int N>
 struct Table {
   int32_t count, chunks;
@@ -58,27 +58,80 @@ __device__ __forceinline__ float2 unpack(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
 
-// f(j, v) for the 16 values of this thread in the chunk [c0, c0 + CHUNK) of a tensor of n values
-// that lies on a 16-byte boundary and has the whole chunk: group k of 4 (fp32) or 8 (bf16) consecutive values.
-template <class F>
-__device__ __forceinline__ void vec_f32(const float* p, F f) {
-  float4 q[4];
+// The 16 values of a chunk that thread t takes: groups of consecutive values where the chunk is
+// whole and on a 16-byte boundary, every NT-th value otherwise.  All loads are issued before the
+// first value is used.
+template <class T>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[16]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) q[k] = reinterpret_cast<const float4*>(p)[threadIdx.x + NT * k];
+    for (int k = 0; k < 4; ++k) {
+      const float4 q = reinterpret_cast<const float4*>(p)[threadIdx.x + NT * k];
+      v[4 * k] = q.x, v[4 * k + 1] = q.y, v[4 * k + 2] = q.z, v[4 * k + 3] = q.w;
+    }
+  } else {
+    uint4 q[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f(4 * (threadIdx.x + NT * k), q[k]);
+    for (int k = 0; k < 2; ++k) q[k] = reinterpret_cast<const uint4*>(p)[threadIdx.x + NT * k];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float2 a = unpack(q[k].x), b = unpack(q[k].y), c = unpack(q[k].z), d = unpack(q[k].w);
+      v[8 * k] = a.x, v[8 * k + 1] = a.y, v[8 * k + 2] = b.x, v[8 * k + 3] = b.y;
+      v[8 * k + 4] = c.x, v[8 * k + 5] = c.y, v[8 * k + 6] = d.x, v[8 * k + 7] = d.y;
+    }
+  }
 }
-template <class F>
-__device__ __forceinline__ void vec_bf16(const __nv_bfloat16* p, F f) {
-  uint4 q[2];
+__device__ __forceinline__ float value(float v) { return v; }
+__device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ void load_each(const T* p, int m, float (&v)[16]) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) q[k] = reinterpret_cast<const uint4*>(p)[threadIdx.x + NT * k];
+  for (int k = 0; k < 16; ++k) {
+    const int j = threadIdx.x + NT * k;
+    v[k] = j < m ? value(p[j]) : 0.f;
+  }
+}
+// vec: the source is whole and aligned (its groups: 4 values of fp32, 8 of bf16)
+template <class T>
+__device__ __forceinline__ void load16(const void* src, int64_t at, int m, bool vec, float (&v)[16]) {
+  const T* p = reinterpret_cast<const T*>(src) + at;
+  if (vec) load_vec(p, v);
+  else load_each(p, m, v);
+}
+// the first value's place and the distance of the groups, as load_vec<T> took them
+template <class TS, class TD>
+__device__ __forceinline__ void store_vec(TD* p, const float (&v)[16]) {
+  constexpr int G = sizeof(TS) == 4 ? 4 : 8;  // values of a group
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int j = 8 * (threadIdx.x + NT * k);
-    const float2 a = unpack(q[k].x), b = unpack(q[k].y), c = unpack(q[k].z), d = unpack(q[k].w);
-    f(j, make_float4(a.x, a.y, b.x, b.y));
-    f(j + 4, make_float4(c.x, c.y, d.x, d.y));
+  for (int k = 0; k < 16; k += 4) {
+    const int j = G * (threadIdx.x + NT * (k / G)) + k % G;
+    if constexpr (sizeof(TD) == 4) {
+      __stcs(reinterpret_cast<float4*>(p + j), make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+    } else {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[k], v[k + 1]), b = __floats2bfloat162_rn(v[k + 2], v[k + 3]);
+      __stcs(reinterpret_cast<uint2*>(p + j), make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                                         *reinterpret_cast<const uint32_t*>(&b)));
+    }
+  }
+}
+__device__ __forceinline__ void put(float* p, float v) { __stcs(p, v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <class TS, class TD>
+__device__ __forceinline__ void scale_chunk(const Entry& e, int64_t at, int m, bool vec, float coef) {
+  float v[16];
+  load16<TS>(e.src, at, m, vec, v);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] *= coef;
+  TD* p = reinterpret_cast<TD*>(e.dst) + at;
+  if (vec) {
+    store_vec<TS>(p, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int j = threadIdx.x + NT * k;
+      if (j < m) put(p + j, v[k]);
+    }
   }
 }
 
@@ -105,21 +158,15 @@ __global__ void __launch_bounds__(NT) norm_kernel(const __grid_constant__ Table<
     while (ti + 1 < t.count && t.e[ti + 1].first <= c) ++ti;
     const Entry& e = t.e[ti];
     const int64_t at = (c - e.first) * CHUNK;
-    const int64_t left = e.n - at;
-    const auto add = [&](int, float4 q) {
-      s0 = fma((double)q.x, (double)q.x, s0), s1 = fma((double)q.y, (double)q.y, s1);
-      s2 = fma((double)q.z, (double)q.z, s2), s3 = fma((double)q.w, (double)q.w, s3);
-    };
-    if (left >= CHUNK && aligned16(e.src)) {
-      if (e.sdt == SCA2_F32) vec_f32(reinterpret_cast<const float*>(e.src) + at, add);
-      else vec_bf16(reinterpret_cast<const __nv_bfloat16*>(e.src) + at, add);
-    } else {
-      const int m = (int)(left < CHUNK ? left : CHUNK);
-#pragma unroll 4
-      for (int j = threadIdx.x; j < m; j += NT) {
-        const double v = ld_io(e.src, at + j, e.sdt);
-        s0 = fma(v, v, s0);
-      }
+    const int m = (int)(e.n - at < CHUNK ? e.n - at : CHUNK);
+    const bool vec = m == CHUNK && aligned16(e.src);
+    float v[16];
+    if (e.sdt == SCA2_F32) load16<float>(e.src, at, m, vec, v);
+    else load16<__nv_bfloat16>(e.src, at, m, vec, v);
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      s0 = fma((double)v[k], (double)v[k], s0), s1 = fma((double)v[k + 1], (double)v[k + 1], s1);
+      s2 = fma((double)v[k + 2], (double)v[k + 2], s2), s3 = fma((double)v[k + 3], (double)v[k + 3], s3);
     }
   }
   const double s = cta_sum((s0 + s1) + (s2 + s3));
@@ -152,25 +199,14 @@ __global__ void __launch_bounds__(NT) clip_kernel(const __grid_constant__ Table<
     const Entry& e = t.e[ti];
     if (coef == 1.f && e.dst == e.src) continue;  // in place, and every value keeps its bits
     const int64_t at = (c - e.first) * CHUNK;
-    const int64_t left = e.n - at;
-    if (left >= CHUNK && aligned16(e.src) && aligned16(e.dst)) {
-      const auto put = [&](int j, float4 q) {
-        q.x *= coef, q.y *= coef, q.z *= coef, q.w *= coef;
-        if (e.ddt == SCA2_F32) {
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(e.dst) + at + j) = q;
-        } else {
-          __nv_bfloat162 a = __floats2bfloat162_rn(q.x, q.y), b = __floats2bfloat162_rn(q.z, q.w);
-          uint2 o;
-          o.x = *reinterpret_cast<uint32_t*>(&a), o.y = *reinterpret_cast<uint32_t*>(&b);
-          *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(e.dst) + at + j) = o;
-        }
-      };
-      if (e.sdt == SCA2_F32) vec_f32(reinterpret_cast<const float*>(e.src) + at, put);
-      else vec_bf16(reinterpret_cast<const __nv_bfloat16*>(e.src) + at, put);
+    const int m = (int)(e.n - at < CHUNK ? e.n - at : CHUNK);
+    const bool vec = m == CHUNK && aligned16(e.src) && aligned16(e.dst);
+    if (e.sdt == SCA2_F32) {
+      if (e.ddt == SCA2_F32) scale_chunk<float, float>(e, at, m, vec, coef);
+      else scale_chunk<float, __nv_bfloat16>(e, at, m, vec, coef);
     } else {
-      const int m = (int)(left < CHUNK ? left : CHUNK);
-#pragma unroll 4
-      for (int j = threadIdx.x; j < m; j += NT) st_io(e.dst, at + j, ld_io(e.src, at + j, e.sdt) * coef, e.ddt);
+      if (e.ddt == SCA2_F32) scale_chunk<__nv_bfloat16, float>(e, at, m, vec, coef);
+      else scale_chunk<__nv_bfloat16, __nv_bfloat16>(e, at, m, vec, coef);
     }
   }
 }
@@ -180,7 +216,7 @@ __global__ void __launch_bounds__(NT) finish_kernel(const double* __restrict__ p
   if (threadIdx.x == 0) *norm = nrm;
 }
 
-constexpr int SMALL = 100, LARGE = 1000;
+constexpr int SMALL = 64, MIDDLE = 256, LARGE = 1000;
 static_assert(sizeof(Table<LARGE>) <= 32764 - 64, "kernel parameters are limited to 32764 bytes");
 
 int grid_of(int chunks) { return std::max(1, std::min(chunks, 148 * CTAS_PER_SM)); }
@@ -227,25 +263,22 @@ int fail(int code, const char* msg) {
   return code;
 }
 
-// launches of LARGE tensors each, and of at most 2^30 chunks
-std::vector<Group> groups_of(const sca2_grad_tensor* list, int count) {
-  std::vector<Group> v;
+constexpr int64_t PARTS = 148 * CTAS_PER_SM;  // partials of one launch, at most
+
+// launches of LARGE tensors each; false where one would have 2^30 chunks or more
+bool groups_of(const sca2_grad_tensor* list, int count, std::vector<Group>& v) {
   int part = 0;
-  for (int i = 0; i < count;) {
-    Group g{i, i, 0, 0, part};
+  for (int i = 0; i < count; i += LARGE) {
+    Group g{i, std::min(count, i + LARGE), 0, 0, part};
     int64_t chunks = 0;
-    while (g.end < count && g.end - g.begin < LARGE) {
-      const int64_t c = (list[g.end].n + CHUNK - 1) / CHUNK;
-      if (chunks + c > (1LL << 30)) break;
-      chunks += c, ++g.end;
-    }
+    for (int k = g.begin; k < g.end; ++k) chunks += (list[k].n + CHUNK - 1) / CHUNK;
+    if (chunks >= (1LL << 30)) return false;
     g.chunks = (int)chunks, g.grid = grid_of(g.chunks);
-    i = g.end;
     if (!g.chunks) continue;
     part += g.grid;
     v.push_back(g);
   }
-  return v;
+  return true;
 }
 
 int width(int dt) { return dt == SCA2_BF16 ? 2 : 4; }
@@ -297,17 +330,19 @@ int go(const sca2_grad_tensor* list, int32_t count, float max_norm, bool write, 
   if (int rc = check(list, count, write)) return rc;
   if (!norm || !work || (reinterpret_cast<uintptr_t>(work) & 7u))
     return fail(SCA2_ERR_ARG, "clip_grads: norm and an 8-byte aligned workspace are needed");
+  if (work_bytes < sca2_clip_grads_work_bytes(count)) return fail(SCA2_ERR_ARG, "clip_grads: workspace too small");
   if (write && !(max_norm >= 0.f)) return fail(SCA2_ERR_ARG, "clip_grads: max_norm must be >= 0");
   try {
     if (write && overlaps(list, count))
       return fail(SCA2_ERR_ARG, "clip_grads: a destination overlaps another tensor of the list");
-    const std::vector<Group> groups = groups_of(list, count);
+    std::vector<Group> groups;
+    if (!groups_of(list, count, groups)) return fail(SCA2_ERR_UNSUPPORTED, "clip_grads: too many values");
     const int nparts = groups.empty() ? 0 : groups.back().part + groups.back().grid;
-    if (work_bytes < (int64_t)nparts * 8) return fail(SCA2_ERR_ARG, "clip_grads: workspace too small");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     double* part = static_cast<double*>(work);
     const cudaError_t e = count <= SMALL ? run<SMALL>(list, groups, nparts, max_norm, write, norm, part, st)
-                                         : run<LARGE>(list, groups, nparts, max_norm, write, norm, part, st);
+                          : count <= MIDDLE ? run<MIDDLE>(list, groups, nparts, max_norm, write, norm, part, st)
+                                            : run<LARGE>(list, groups, nparts, max_norm, write, norm, part, st);
     if (e != cudaSuccess) {
       set_last_error(std::string("sca2_clip_grads: ") + cudaGetErrorString(e));
       return SCA2_ERR_CUDA;
@@ -323,14 +358,8 @@ int go(const sca2_grad_tensor* list, int32_t count, float max_norm, bool write, 
 
 extern "C" {
 
-int64_t sca2_clip_grads_work_bytes(const sca2_grad_tensor* list, int32_t count) {
-  if (sca2::clip::check(list, count, false)) return 0;
-  try {
-    const auto groups = sca2::clip::groups_of(list, count);
-    return 8 * (int64_t)(groups.empty() ? 1 : groups.back().part + groups.back().grid);
-  } catch (const std::exception&) {
-    return 0;
-  }
+int64_t sca2_clip_grads_work_bytes(int32_t count) {
+  return count < 0 ? 0 : 8 * sca2::clip::PARTS * std::max<int64_t>(1, ((int64_t)count + sca2::clip::LARGE - 1) / sca2::clip::LARGE);
 }
 
 int sca2_grad_norm(const sca2_grad_tensor* list, int32_t count, float* norm, void* work, int64_t work_bytes,

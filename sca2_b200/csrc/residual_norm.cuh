@@ -36,7 +36,7 @@ struct Args {
 
 enum { PART_W, PART_B, PART_SCALE, PART_PW, PART_PB, NPART };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
 __device__ __forceinline__ void unpack2(uint32_t u, float* v) {
   v[0] = __uint_as_float(u << 16), v[1] = __uint_as_float(u & 0xFFFF0000u);
@@ -124,7 +124,7 @@ __device__ __forceinline__ float row_sum(float v, int& flip) {
 }
 
 template <int NT, int NV, int VEC, class TX, class TU>
-__global__ void __launch_bounds__(FT) fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(const Args a) {
   const int t = threadIdx.x % NT;
   const int d = a.d;
   const float inv = 1.f / (float)d;
@@ -244,10 +244,13 @@ __device__ __forceinline__ void warp_sums(float* v, int lane) {
 }
 constexpr int halvings(int n) { return n % 2 == 0 ? 1 + halvings(n / 2) : 0; }
 
-// CTA sums of N values; `s` has (N, W) floats whose unused warps hold zeros
+// CTA sums of N values over at most W warps; `s` has (N, W) floats whose unused warps hold zeros.
+// After the barrier every warp adds the warps' parts itself, W lanes to a value, and hands the
+// totals round: few instructions, and no second barrier.
 template <int N, int W>
 __device__ __forceinline__ void cta_sums(float* v, float* s) {
   constexpr int H = halvings(N) < 5 ? halvings(N) : 5, LEFT = N >> H;
+  constexpr int P = 32 / W, J = (N + P - 1) / P;  // values of one pass over the warp, passes
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   warp_sums<N, 16>(v, lane);
   if ((lane & ((1 << (5 - H)) - 1)) == 0) {
@@ -259,27 +262,27 @@ __device__ __forceinline__ void cta_sums(float* v, float* s) {
     for (int i = 0; i < LEFT; ++i) s[(first + i) * W + warp] = v[i];
   }
   __syncthreads();
+  float q[J];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float q = 0.f;
+  for (int j = 0; j < J; ++j) {
+    const int at = P * W * j + lane;
+    q[j] = at < N * W ? s[at] : 0.f;
 #pragma unroll
-    for (int w = 0; w < W; w += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(s + i * W + w);
-      q += (f.x + f.y) + (f.z + f.w);
-    }
-    v[i] = q;
+    for (int o = W / 2; o > 0; o >>= 1) q[j] += __shfl_xor_sync(0xffffffffu, q[j], o);
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, q[i / P], (i % P) * W);
 }
 
-template <int MAXT, int R, bool CONTIG, class TX, class TU>
-__global__ void __launch_bounds__(MAXT) bwd_kernel(const Args a) {
-  constexpr int W = MAXT / 32;
+template <int MAXT, int R, int MINB, bool CONTIG, class TX, class TU>
+__global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
+  constexpr int W = MAXT <= 256 ? 8 : MAXT / 32;
   __shared__ __align__(16) float red[2][3 * R * W];
   const int t = threadIdx.x, T = blockDim.x, d = a.d;
   const float inv = 1.f / (float)d;
   for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
   __syncthreads();
-  const auto col = [&](int k) { return CONTIG ? 4 * t + k : t + T * k; };
+  const auto col = [&](int k) { return CONTIG ? 4 * t : t + T * k; };  // CONTIG: d % 4 == 0, all four or none
   const auto load = [&](const auto* p, float* v) {
     if constexpr (CONTIG) {
       if (4 * t < d) loadv<4>(p + 4 * t, v);
@@ -298,9 +301,11 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const Args a) {
         if (col(k) < d) storev<1>(p + col(k), v + k);
     }
   };
+  // Columns past d get parameters of 0, which keep whatever a row's statistics make of them out of
+  // the row's sums.
   const auto param = [&](const float* p, float fill, float* v) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = fill;
+    for (int k = 0; k < 4; ++k) v[k] = col(k) < d ? fill : 0.f;
     if (p) load(p, v);
   };
   const bool post = a.pw != nullptr, token = a.gate_mode == 1, chan = a.gate_mode == 2, has_z = a.dz != nullptr;
@@ -346,10 +351,9 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const Args a) {
       for (int k = 0; k < 4; ++k) {
         if (post) un[i][k] = (un[i][k] - st[i][0]) * st[i][1];
         s[i][k] = a.gate_mode ? sigmoid(s[i][k]) : 1.f;
-        const bool ok = col(k) < d;
         if (has_z) {
           const float y = fmaf(sc[k] * s[i][k], fmaf(un[i][k], pw[k], pb[k]), yn[i][k]);
-          yn[i][k] = ok ? (y - st[i][2]) * st[i][3] : 0.f;
+          yn[i][k] = (y - st[i][2]) * st[i][3];
           aw[k] = fmaf(dn[i][k], yn[i][k], aw[k]);
           ab[k] += dn[i][k];
           dn[i][k] *= w[k];
@@ -375,8 +379,7 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const Args a) {
       float q0 = 0.f, q1 = 0.f, q2 = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const bool ok = col(k) < d && r < a.rows;
-        const float e = ok ? dy[i][k] : 0.f;
+        const float e = dy[i][k];
         const float p = fmaf(un[i][k], pw[k], pb[k]);
         as[k] = fmaf(e * s[i][k], p, as[k]);
         dg[k] = e * sc[k] * p * s[i][k] * (1.f - s[i][k]);
@@ -418,12 +421,12 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const Args a) {
   if (post && a.pb) store(part + PART_PB * d, apb);
 }
 
-// rows of partials for a call of `rows` rows: the CTAs of the backward, two to an SM
-inline int bwd_rows_per_step(int64_t rows, int d) { return d > 2048 ? 1 : d > 1024 ? 2 : rows >= 148 * 8 ? 4 : 1; }
+// rows in flight in a CTA, and the CTAs (each leaves one row of partials)
+inline int bwd_rows_per_step(int64_t rows, int d) { return d > 1024 ? 1 : rows >= 148 * 6 ? 2 : 1; }
 inline int bwd_grid(int64_t rows, int d) {
-  const int R = bwd_rows_per_step(rows, d);
+  const int R = bwd_rows_per_step(rows, d), most = 148 * (d > 2048 ? 1 : d > 1024 ? 2 : 3);
   const int64_t want = (rows + R - 1) / R;
-  return (int)(want < 148 * 2 ? want : 148 * 2);
+  return (int)(want < most ? want : most);
 }
 
 template <class TX, class TU>
@@ -453,10 +456,11 @@ template <bool CONTIG, class TX, class TU>
 cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
   const int d = a.d, R = bwd_rows_per_step(a.rows, d), grid = bwd_grid(a.rows, d);
   const int T = ((d + 3) / 4 + 31) / 32 * 32;
-  if (d > 2048) bwd_kernel<1024, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (d > 1024) bwd_kernel<512, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (R == 4) bwd_kernel<256, 4, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else bwd_kernel<256, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  if (d > 2048) bwd_kernel<1024, 1, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (d > 1024) bwd_kernel<512, 1, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (R == 2 && T <= 192) bwd_kernel<192, 2, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (R == 2) bwd_kernel<256, 2, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   return cudaGetLastError();
 }
 template <class TX, class TU>

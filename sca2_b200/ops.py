@@ -22,6 +22,7 @@ allocates nothing.
 from __future__ import annotations
 
 import contextlib
+import operator
 import struct
 from typing import Optional, Sequence, Tuple
 
@@ -45,9 +46,13 @@ def _ptr(t: Optional[torch.Tensor]):
 _HERE = contextlib.nullcontext()
 
 
-def _on(dev: torch.device):
-    """Context in which `dev` is the current device (launches go to the current device's stream)."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _on(dev: int):
+    """Context in which CUDA device `dev` is the current one (a launch needs its stream's device)."""
+    return _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _stream_of(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _need_cuda(*ts):
@@ -61,6 +66,19 @@ def _need_cuda(*ts):
             dev = t.device
         elif t.device != dev:
             raise _lib.Sca2Error("all tensors must be on the same CUDA device")
+    return dev
+
+
+def _device_of(*ts) -> int:
+    """The index of the CUDA device that all the tensors (None: absent) are on; raises as _need_cuda."""
+    dev = -2
+    for t in ts:
+        if t is not None:
+            i = t.get_device()
+            if i != dev:
+                if dev != -2 or i < 0:
+                    return _need_cuda(*ts).index
+                dev = i
     return dev
 
 
@@ -1307,42 +1325,44 @@ _ACT = {"silu": 0, "gelu": 1}
 def _ffn_rows(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
     """t (..., width) as 16-byte aligned rows with a stride of a multiple of 8 values (a copy only
     where it is not laid out so), and the stride."""
-    v, ld = _row_view(t, width)
+    v, ld = (t, width) if t.is_contiguous() else _row_view(t, width)
     if v.data_ptr() % 16 or ld % 8:
         v, ld = v.clone(memory_format=torch.contiguous_format), width
     return v, ld
 
 
 def _ffn_args(x, wg, wu, act):
-    a = _lib.FfnArgs()
-    d = x.shape[-1]
-    (x, a.ldx), (wg, a.ldg), (wu, a.ldu) = _ffn_rows(x, d), _ffn_rows(wg, d), _ffn_rows(wu, d)
-    a.x, a.w_gate, a.w_up = x.data_ptr(), wg.data_ptr(), wu.data_ptr()
-    a.rows, a.d, a.f, a.act = x.numel() // d, d, wg.shape[0], act
+    f, d = wg.shape
+    (x, ldx), (wg, ldg), (wu, ldu) = _ffn_rows(x, d), _ffn_rows(wg, d), _ffn_rows(wu, d)
+    a = _lib.FfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ldx, ldg, ldu, x.numel() // d, d, f, act)
     return a, (x, wg, wu)  # the tensors stay alive until the launch is queued
 
 
 def _gated_ffn_run(x, wg, wu, act: int):
-    dev = x.device
-    h = torch.empty(*x.shape[:-1], wg.shape[0], device=dev, dtype=torch.bfloat16)
+    dev = x.get_device()
+    h = x.new_empty((*x.shape[:-1], wg.shape[0]))
     a, hold = _ffn_args(x, wg, wu, act)
     with _on(dev):
-        _lib.check(_lib.load().sca2_gated_ffn_fwd(a, h.data_ptr(), _stream()), "gated_ffn")
+        rc = _lib.load().sca2_gated_ffn_fwd(a, h.data_ptr(), _stream_of(dev))
+    if rc:
+        _lib.check(rc, "gated_ffn")
     return h
 
 
 def _gated_ffn_bwd_run(x, wg, wu, act: int, dh, need_x: bool, need_w: bool):
-    dev = x.device
+    dev = x.get_device()
     a, hold = _ffn_args(x, wg, wu, act)
     dh, _ = _ffn_rows(dh.to(torch.bfloat16).contiguous(), a.f)
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_x else None
-    dwg, dwu = (torch.empty(wg.shape, device=dev, dtype=wg.dtype) if need_w else None for _ in range(2))
+    dense = torch.contiguous_format
+    dx = torch.empty_like(x, memory_format=dense) if need_x else None
+    dwg, dwu = (torch.empty_like(w, memory_format=dense) if need_w else None for w in (wg, wu))
     lib = _lib.load()
     n = lib.sca2_gated_ffn_work_bytes(a.rows, a.d, a.f)
-    work = torch.empty(n, device=dev, dtype=torch.uint8)
+    work = x.new_empty(n, dtype=torch.uint8)
     with _on(dev):
-        _lib.check(lib.sca2_gated_ffn_bwd(a, dh.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu), work.data_ptr(), n,
-                                          _stream()), "gated_ffn_bwd")
+        rc = lib.sca2_gated_ffn_bwd(a, dh.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu), work.data_ptr(), n, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "gated_ffn_bwd")
     return dx, dwg, dwu
 
 
@@ -1411,11 +1431,11 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
     weights (f, d), all bf16 with fp32 accumulation, d and f multiples of 8; returns h (..., f).
     Differentiable once in all three; the backward recomputes the projections, so nothing but the
     inputs is kept.  The weights may be the halves of one (2 f, d) tensor."""
-    _need_cuda(x, w_gate, w_up)
+    _device_of(x, w_gate, w_up)
     E = _lib.Sca2Error
     if act not in _ACT:
         raise E(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
-    if any(t.dtype != torch.bfloat16 for t in (x, w_gate, w_up)):
+    if not x.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16:
         raise E("gated_ffn: x and the weights must be bfloat16")
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1]:
         raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(w_gate.shape)} and "
@@ -1451,50 +1471,49 @@ def _row_view(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
 
 
 def _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
-    a = _lib.RNormArgs()
     d = x.shape[-1]
-    (x, a.sx), (u, a.su) = _row_view(x, d), _row_view(u, d)
-    a.x, a.u = x.data_ptr(), u.data_ptr()
+    (x, sx), (u, su) = _row_view(x, d), _row_view(u, d)
+    mode = sg = g = 0
     if gate is not None:
-        a.gate_mode = 2 if gate.shape[-1] == d else 1
-        gate, a.sg = _row_view(gate, gate.shape[-1])
-        a.gate = gate.data_ptr()
-    a.w, a.b, a.pw, a.pb, a.scale = _ptr(w), _ptr(b), _ptr(pw), _ptr(pb), _ptr(scale)
-    a.rows, a.d = x.numel() // d, d
-    a.x_dtype, a.u_dtype, a.z_dtype = _DT[x.dtype], _DT[u.dtype], _DT[zdt]
-    a.kind, a.eps = kind, eps
+        mode = 2 if gate.shape[-1] == d else 1
+        gate, sg = _row_view(gate, gate.shape[-1])
+        g = gate.data_ptr()
+    a = _lib.RNormArgs(x.data_ptr(), u.data_ptr(), g, sx, su, sg, _ptr(w), _ptr(b), _ptr(pw), _ptr(pb), _ptr(scale),
+                       x.numel() // d, d, _DT[x.dtype], _DT[u.dtype], _DT[zdt], kind, mode, eps)
     return a, (x, u, gate)  # the tensors stay alive until the launch is queued
 
 
 def _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, save: bool):
-    dev = x.device
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    z = torch.empty(x.shape if w is not None else (0,), device=dev, dtype=zdt)
-    stats = torch.empty(x.numel() // x.shape[-1] if save else 0, 4, device=dev)
+    dev, dense = x.get_device(), torch.contiguous_format
+    y = torch.empty_like(x, memory_format=dense)
+    z = torch.empty_like(x, dtype=zdt, memory_format=dense) if w is not None else x.new_empty(0, dtype=zdt)
+    stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if save else None
     a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
     with _on(dev):
-        _lib.check(_lib.load().sca2_residual_norm_fwd(a, y.data_ptr(), z.data_ptr() if w is not None else None,
-                                                      stats.data_ptr() if save else None, _stream()), "residual_norm")
+        rc = _lib.load().sca2_residual_norm_fwd(a, y.data_ptr(), z.data_ptr() if w is not None else None, _ptr(stats),
+                                                _stream_of(dev))
+    if rc:
+        _lib.check(rc, "residual_norm")
     return y, z, stats
 
 
 def _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, stats, dy, dz):
-    dev, d = x.device, x.shape[-1]
-    dense = lambda t, ty: None if t is None else t.to(ty).contiguous()
-    dy, dz = dense(dy, x.dtype), dense(dz, zdt)
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    du = torch.empty(u.shape, device=dev, dtype=u.dtype)
-    dgate = torch.empty(gate.shape, device=dev, dtype=gate.dtype) if gate is not None else None
-    dpar = [torch.empty(d, device=dev) if t is not None else None for t in (w, b, scale, pw, pb)]
+    dev, dense = x.get_device(), torch.contiguous_format
+    dy = None if dy is None else dy.to(x.dtype).contiguous()
+    dz = None if dz is None else dz.to(zdt).contiguous()
+    dx, du = torch.empty_like(x, memory_format=dense), torch.empty_like(u, memory_format=dense)
+    dgate = torch.empty_like(gate, memory_format=dense) if gate is not None else None
+    dw, db, dscale, dpw, dpb = (None if t is None else torch.empty_like(t) for t in (w, b, scale, pw, pb))
     a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
     lib = _lib.load()
-    n = lib.sca2_residual_norm_work_bytes(a.rows, d)
-    work = torch.empty(n, device=dev, dtype=torch.uint8)
-    g = _lib.RNormGrads(dx.data_ptr(), du.data_ptr(), _ptr(dgate), *[_ptr(t) for t in dpar])
+    n = lib.sca2_residual_norm_work_bytes(a.rows, a.d)
+    work = x.new_empty(n, dtype=torch.uint8)
+    g = _lib.RNormGrads(dx.data_ptr(), du.data_ptr(), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dscale), _ptr(dpw), _ptr(dpb))
     with _on(dev):
-        _lib.check(lib.sca2_residual_norm_bwd(a, stats.data_ptr(), _ptr(dy), _ptr(dz), g, work.data_ptr(), n, _stream()),
-                   "residual_norm_bwd")
-    return dx, du, dpar[0], dpar[1], dgate, dpar[2], dpar[3], dpar[4]
+        rc = lib.sca2_residual_norm_bwd(a, stats.data_ptr(), _ptr(dy), _ptr(dz), g, work.data_ptr(), n, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "residual_norm_bwd")
+    return dx, du, dw, db, dgate, dscale, dpw, dpb
 
 
 @torch.library.custom_op("sca2b200::residual_norm_fwd", mutates_args=())
@@ -1503,7 +1522,8 @@ def _residual_norm_fwd(x: torch.Tensor, u: torch.Tensor, w: Optional[torch.Tenso
                        pb: Optional[torch.Tensor], kind: int, eps: float, zdt: torch.dtype, save: bool
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """sca2_residual_norm_fwd: y, z (empty without w) and, with save, the rows' means and deviations."""
-    return _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, save)
+    y, z, stats = _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, save)
+    return y, z, x.new_empty((0, 4), dtype=torch.float32) if stats is None else stats
 
 
 @_residual_norm_fwd.register_fake
@@ -1579,13 +1599,14 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
     weight, bias, post_weight, post_bias, scale (d) (computed with in fp32).  kind: "layer"
     (LayerNorm) or "rms" (no bias), for both norms.  y has x's type, z out_dtype (default: x's);
     arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
-    dev = _need_cuda(x, u, weight, bias, gate, scale, post_weight, post_bias)
-    E, d = _lib.Sca2Error, x.shape[-1] if x.dim() else 0
+    _device_of(x, u, weight, bias, gate, scale, post_weight, post_bias)
+    E, shape = _lib.Sca2Error, x.shape
+    d = shape[-1] if shape else 0
     if kind not in _NORM_KIND:
         raise E(f"residual_norm: kind must be 'layer' or 'rms', not {kind!r}")
-    if d < 1 or u.shape != x.shape:
-        raise E(f"residual_norm: x and u must have one shape (..., d), got {tuple(x.shape)} and {tuple(u.shape)}")
-    if gate is not None and (gate.shape[:-1] != x.shape[:-1] or gate.dim() != x.dim() or gate.shape[-1] not in (1, d)):
+    if d < 1 or u.shape != shape:
+        raise E(f"residual_norm: x and u must have one shape (..., d), got {tuple(shape)} and {tuple(u.shape)}")
+    if gate is not None and gate.shape != shape and gate.shape != (*shape[:-1], 1):
         raise E(f"residual_norm: gate must be (..., d) or (..., 1), got {tuple(gate.shape)}")
     zdt = x.dtype if out_dtype is None else out_dtype
     if x.dtype not in _DT or u.dtype not in _DT or zdt not in _DT:
@@ -1594,9 +1615,12 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
         raise E("residual_norm: a bias needs its weight")
     par = []
     for t in (weight, bias, scale, post_weight, post_bias):
-        if t is not None and t.shape != (d,):
-            raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
-        par.append(None if t is None else t.float().contiguous())
+        if t is not None:
+            if t.shape != (d,):
+                raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                t = t.float().contiguous()
+        par.append(t)
     if gate is not None and gate.dtype != u.dtype:
         gate = gate.to(u.dtype)
     w, b, sc, pw, pb = par
@@ -1614,55 +1638,69 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
 # ======================================================================================
 #  global gradient norm and clipping
 # ======================================================================================
+_shape, _dtype, _layout = (operator.attrgetter(n) for n in ("shape", "dtype", "layout"))
+_T = torch.Tensor
+
+
 def _grad_list(what: str, grads, out=None):
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
+    grads = [grads] if isinstance(grads, _T) else list(grads)
+    outs = grads if out is None else ([out] if isinstance(out, _T) else list(out))
     E = _lib.Sca2Error
     if len(outs) != len(grads):
         raise E(f"{what}: {len(grads)} gradients and {len(outs)} destinations")
-    for t in grads if out is None else grads + outs:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _DT:
-            raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
-    dev = _need_cuda(*grads, *(outs if out is not None else ()))
-    if out is not None:
-        for g, o in zip(grads, outs):
-            if g.shape != o.shape or not o.is_contiguous():
-                raise E(f"{what}: a destination must be contiguous, with its gradient's shape")
+    every = grads if out is None else grads + outs
+    if not all([isinstance(t, _T) for t in every]) or not set(map(_dtype, every)) <= _DT.keys() \
+            or set(map(_layout, every)) - {torch.strided}:
+        raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
+    if not every:
+        return grads, outs, None
+    dev = set(map(_T.get_device, every))
+    dev = dev.pop() if len(dev) == 1 and min(dev) >= 0 else _need_cuda(*every).index
+    if out is not None and (list(map(_shape, grads)) != list(map(_shape, outs)) or not all(map(_T.is_contiguous, outs))):
+        raise E(f"{what}: a destination must be contiguous, with its gradient's shape")
     return grads, outs, dev
 
 
 def _grad_table(src, dst):
     """The sca2_grad_tensor list as bytes (host memory; the library copies it into the launch)."""
-    flat = [v for s, d in zip(src, dst)
-            for v in (s.data_ptr(), d.data_ptr(), s.numel(), _DT[s.dtype], _DT[d.dtype])]
-    return struct.pack("=" + "QQqii" * len(src), *flat)
+    n = len(src)
+    flat = [0] * (5 * n)
+    flat[0::5] = map(_T.data_ptr, src)
+    flat[1::5] = map(_T.data_ptr, dst) if dst is not src else flat[0::5]
+    flat[2::5] = map(_T.numel, src)
+    flat[3::5] = map(_DT.__getitem__, map(_dtype, src))
+    flat[4::5] = map(_DT.__getitem__, map(_dtype, dst)) if dst is not src else flat[3::5]
+    return struct.pack("=" + "QQqii" * n, *flat)
 
 
-def _clip_run(grads, outs, max_norm: Optional[float], dev) -> torch.Tensor:
+def _clip_run(grads, outs, max_norm: Optional[float], dev: int) -> torch.Tensor:
     # a gradient that is not contiguous goes through a contiguous copy
-    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    dst = [s if o is g else o for s, g, o in zip(src, grads, outs)]
-    table, n, lib = _grad_table(src, dst), len(src), _lib.load()
+    src, back = grads, ()
+    if not all(map(_T.is_contiguous, grads)):
+        src = [g.contiguous() for g in grads]
+        if outs is grads:
+            back = [(g, s) for g, s in zip(grads, src) if g is not s]
+    table, n, lib = _grad_table(src, src if outs is grads else outs), len(src), _lib.load()
+    norm = src[0].new_empty((), dtype=torch.float32)
+    nb = lib.sca2_clip_grads_work_bytes(n)
+    work = src[0].new_empty(nb, dtype=torch.uint8)
     with _on(dev):
-        norm = torch.empty((), device=dev)
-        nb = lib.sca2_clip_grads_work_bytes(table, n)
-        work = torch.empty(max(nb, 8), device=dev, dtype=torch.uint8)
         if max_norm is None:
-            _lib.check(lib.sca2_grad_norm(table, n, norm.data_ptr(), work.data_ptr(), nb, _stream()), "grad_norm")
+            rc = lib.sca2_grad_norm(table, n, norm.data_ptr(), work.data_ptr(), nb, _stream_of(dev))
         else:
-            _lib.check(lib.sca2_clip_grads(table, n, max_norm, norm.data_ptr(), work.data_ptr(), nb, _stream()),
-                       "clip_grads")
+            rc = lib.sca2_clip_grads(table, n, max_norm, norm.data_ptr(), work.data_ptr(), nb, _stream_of(dev))
+    if rc:
+        _lib.check(rc, "grad_norm" if max_norm is None else "clip_grads")
     if max_norm is not None:
-        for g, s, o in zip(grads, src, outs):
-            if o is g and s is not g:
-                g.copy_(s)
+        for g, s in back:
+            g.copy_(s)
     return norm
 
 
 @torch.library.custom_op("sca2b200::grad_norm", mutates_args=())
 def _grad_norm_op(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """sca2_grad_norm over a list of tensors."""
-    return _clip_run(list(grads), list(grads), None, grads[0].device)
+    return _clip_run(grads, grads, None, grads[0].get_device())
 
 
 @_grad_norm_op.register_fake
@@ -1673,7 +1711,7 @@ def _(grads):
 @torch.library.custom_op("sca2b200::clip_grads_", mutates_args=("grads",))
 def _clip_grads_op(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
     """sca2_clip_grads in place over a list of tensors; returns the norm before."""
-    return _clip_run(list(grads), list(grads), max_norm, grads[0].device)
+    return _clip_run(grads, grads, max_norm, grads[0].get_device())
 
 
 @_clip_grads_op.register_fake
@@ -1681,35 +1719,35 @@ def _(grads, max_norm):
     return grads[0].new_empty((), dtype=torch.float32)
 
 
-@torch.no_grad()
 def grad_norm(grads) -> torch.Tensor:
     """2-norm of all values of the tensors together (fp32 scalar on their device; summed in 64 bits
     in a fixed order).  grads: a tensor or a list of float32 / bfloat16 tensors on one device; no
-    tensor gives 0 (on the current CUDA device)."""
+    tensor gives 0 (on the current CUDA device).  Not differentiable."""
     grads, outs, dev = _grad_list("grad_norm", grads)
     if not grads:
         return torch.zeros((), device="cuda")
-    if torch.compiler.is_compiling():
-        return torch.ops.sca2b200.grad_norm(grads)
-    return _clip_run(grads, outs, None, dev)
+    with torch.no_grad():
+        if torch.compiler.is_compiling():
+            return torch.ops.sca2b200.grad_norm(grads)
+        return _clip_run(grads, outs, None, dev)
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     """Scale the gradients so that their global 2-norm is at most max_norm, and return the norm
     before (fp32 scalar; nothing waits for the device): g * min(1, max_norm / (norm + 1e-6)), as
     torch.nn.utils.clip_grad_norm_.  In place, or into the contiguous tensors `out` (float32 or
     bfloat16, one for each gradient).  A tensor that is written may not share memory with another
-    of the call (refused)."""
+    of the call (refused).  Not differentiable."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise _lib.Sca2Error("clip_grads: max_norm must be >= 0")
     grads, outs, dev = _grad_list("clip_grads", grads, out)
     if not grads:
         return torch.zeros((), device="cuda")
-    if torch.compiler.is_compiling() and out is None:
-        return torch.ops.sca2b200.clip_grads_(grads, max_norm)
-    norm = _clip_run(grads, outs, max_norm, dev)
+    with torch.no_grad():
+        if torch.compiler.is_compiling() and out is None:
+            return torch.ops.sca2b200.clip_grads_(grads, max_norm)
+        norm = _clip_run(grads, outs, max_norm, dev)
     torch.autograd.graph.increment_version(outs)
     return norm
 

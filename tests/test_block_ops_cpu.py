@@ -119,10 +119,10 @@ def test_clip_entry_refusals():
     assert lib.sca2_clip_grads(t, 1, 1.0, None, P, big, None) == _lib.SCA2_ERR_ARG
     assert lib.sca2_clip_grads(t, 1, 1.0, P, None, big, None) == _lib.SCA2_ERR_ARG
     assert lib.sca2_clip_grads(t, 1, 1.0, P, P + 4, big, None) == _lib.SCA2_ERR_ARG
-    n = lib.sca2_clip_grads_work_bytes(t, 1)
+    n = lib.sca2_clip_grads_work_bytes(1)
     assert n >= 8 and lib.sca2_clip_grads(t, 1, 1.0, P, P, n - 1, None) == _lib.SCA2_ERR_ARG
     assert lib.sca2_grad_norm(t, 1, P, P, n - 1, None) == _lib.SCA2_ERR_ARG
-    assert lib.sca2_clip_grads_work_bytes(one(n=-1), 1) == 0
+    assert lib.sca2_clip_grads_work_bytes(-1) == 0 and lib.sca2_clip_grads_work_bytes(2001) == 3 * n
 
 
 def test_gated_ffn_refusals():
