@@ -68,6 +68,8 @@ struct Geo {
   int tiles_n, tiles_m, slices, splits;  // unit = ((split * slices + slice) * tiles_m + m) * tiles_n + n
   int units;
   int kb, kb_half;                       // contraction blocks of a whole tile; DX: those of one half
+  int kb_split, kb_more;                 // those of a split, and how many splits have one more
+  int sn, sm, ss, sp;                    // the grid's pairs as digits of a unit
 };
 
 struct Maps {
@@ -231,17 +233,31 @@ __device__ __forceinline__ uint4 lds4(uint32_t a) {
   return q;
 }
 
+// A pair's units, `step` apart.  The step is kept as digits (Geo::s*) and added with carries: a
+// division for each tile would stall the one thread that issues the products between two tiles.
 struct Unit {
-  int n, m, slice, split, k0, k1;
+  int n, m, slice, split;
+  __device__ __forceinline__ void first(const Geo& g, int u) {
+    n = u % g.tiles_n, u /= g.tiles_n;
+    m = u % g.tiles_m, u /= g.tiles_m;
+    slice = u % g.slices, split = u / g.slices;
+  }
+  __device__ __forceinline__ void next(const Geo& g) {
+    n += g.sn;
+    const int c = n >= g.tiles_n;
+    n -= c ? g.tiles_n : 0;
+    m += g.sm + c;
+    const int e = m >= g.tiles_m;
+    m -= e ? g.tiles_m : 0;
+    slice += g.ss + e;
+    const int f = slice >= g.slices;
+    slice -= f ? g.slices : 0;
+    split += g.sp + f;
+  }
+  // its contraction blocks: the first `kb_more` splits have one more
+  __device__ __forceinline__ int k0(const Geo& g) const { return split * g.kb_split + (split < g.kb_more ? split : g.kb_more); }
+  __device__ __forceinline__ int k1(const Geo& g) const { return k0(g) + g.kb_split + (split < g.kb_more ? 1 : 0); }
 };
-__device__ __forceinline__ Unit unit_of(const Geo& g, int u) {
-  Unit t;
-  t.n = u % g.tiles_n, u /= g.tiles_n;
-  t.m = u % g.tiles_m, u /= g.tiles_m;
-  t.slice = u % g.slices, t.split = u / g.slices;
-  t.k0 = (int)((int64_t)g.kb * t.split / g.splits), t.k1 = (int)((int64_t)g.kb * (t.split + 1) / g.splits);
-  return t;
-}
 
 template <int MODE, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(const __grid_constant__ Maps maps, const Geo g) {
@@ -279,13 +295,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
   if (warp == 0) {
     if (lane == 0) {  // ---- producer: this CTA's half of both operands
       const uint32_t full0 = map_to(full, 0);
-      int it = 0;
+      int s = 0, ph = 1, issued = 0;
       bool ok = true;
-      for (int u = pair; u < g.units && ok; u += pairs) {
-        const Unit t = unit_of(g, u);
-        for (int k = t.k0; k < t.k1; ++k, ++it) {
-          const int s = it % ST;
-          if (!(ok = wait_for(empty + 8 * s, ((it / ST) & 1) ^ 1))) break;
+      Unit t;
+      t.first(g, pair);
+      for (int u = pair; u < g.units && ok; u += pairs, t.next(g)) {
+        const int k1 = t.k1(g);
+        for (int k = t.k0(g); k < k1; ++k) {
+          if (!(ok = wait_for(empty + 8 * s, ph))) break;
           if (rank == 0) expect(full + 8 * s, 4 * HALF);
           const uint32_t A = base + s * 2 * HALF, B = A + HALF, bar = full0 + 8 * s;
           if constexpr (MODE == FWD || MODE == BACK) {
@@ -306,33 +323,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
             load2(B, &maps.b0, n, k * BK, bar);
             load2(B + HALF / 2, &maps.b0, n + 64, k * BK, bar);
           }
+          if (++s == ST) s = 0, ph ^= 1;
+          issued = issued < ST ? issued + 1 : ST;
         }
       }
       if (!ok && rank == 0)  // leave no copy in flight: both CTAs' copies complete on these
-        for (int i = it > ST ? it - ST : 0; i < it; ++i)
-          if (!wait_for(full + 8 * (i % ST), (i / ST) & 1)) break;
+        for (; issued > 0; --issued) {
+          if (--s < 0) s = ST - 1, ph ^= 1;
+          if (!wait_for(full + 8 * s, ph ^ 1)) break;
+        }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // ---- products of both CTAs
       constexpr bool a_mn = MODE == DW, b_mn = MODE == DX || MODE == DW;
       const uint32_t id = umma::idesc_bf16_t(256, 256, a_mn, b_mn);
-      int it = 0, n = 0;
+      int n = 0, s = 0, ph = 0;
       bool ok = true;
+      Unit t;
+      t.first(g, pair);
       for (int u = pair; u < g.units && ok; u += pairs, ++n) {
-        const Unit t = unit_of(g, u);
-        const int acc = n & 1;
+        const int acc = n & 1, kn = t.k1(g) - t.k0(g);
+        t.next(g);
         if (!(ok = wait_for(tempty + 8 * acc, ((n >> 1) & 1) ^ 1))) break;
         umma::fence_after_sync();
-        for (int k = t.k0; k < t.k1; ++k, ++it) {
-          const int s = it % ST;
-          if (!(ok = wait_for(full + 8 * s, (it / ST) & 1))) break;
+        for (int k = 0; k < kn; ++k) {
+          if (!(ok = wait_for(full + 8 * s, ph))) break;
           umma::fence_after_sync();
           const uint32_t A = base + s * 2 * HALF, B = A + HALF;
           const uint64_t da = a_mn ? desc_mn(A) : desc_k(A), db = b_mn ? desc_mn(B) : desc_k(B);
 #pragma unroll
           for (int j = 0; j < BK / 16; ++j)  // 16 steps on: 2048 / 16 or 32 / 16 in the address field
-            mma2(tmem + 256 * acc, da + (a_mn ? 128 : 2) * j, db + (b_mn ? 128 : 2) * j, id, k > t.k0 || j > 0);
+            mma2(tmem + 256 * acc, da + (a_mn ? 128 : 2) * j, db + (b_mn ? 128 : 2) * j, id, k > 0 || j > 0);
           commit2(empty + 8 * s);
+          if (++s == ST) s = 0, ph ^= 1;
         }
         if (ok) commit2(tfull + 8 * acc);
       }
@@ -341,8 +364,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
     const int e = warp - 4, q = warp & 3, part = e >> 2;
     const uint32_t stg = stg0 + e * L::NSTG * STG, dhb = dhbar + 8 * e, tempty0 = map_to(tempty, 0);
     int n = 0;
-    for (int u = pair; u < g.units; u += pairs, ++n) {
-      const Unit t = unit_of(g, u);
+    Unit t;
+    t.first(g, pair);
+    for (int u = pair; u < g.units; u += pairs, ++n, t.next(g)) {
       const int acc = n & 1;
       const int row = t.m * 256 + 128 * rank + 32 * q;
       const uint32_t tm = umma::taddr(tmem, 32 * q, 256 * acc);
@@ -612,7 +636,13 @@ cudaError_t allow_act(int act) {
 template <int MODE, int ACT>
 cudaError_t launch(const Maps& maps, const Geo& g, cudaStream_t st) {
   const int pairs = g.units < PAIRS ? g.units : PAIRS;
-  ffn_gemm<MODE, ACT><<<2 * pairs, NT, Layout<MODE>::TOTAL, st>>>(maps, g);
+  Geo k = g;
+  k.kb_split = g.kb / g.splits, k.kb_more = g.kb % g.splits;
+  int u = pairs;
+  k.sn = u % g.tiles_n, u /= g.tiles_n;
+  k.sm = u % g.tiles_m, u /= g.tiles_m;
+  k.ss = u % g.slices, k.sp = u / g.slices;
+  ffn_gemm<MODE, ACT><<<2 * pairs, NT, Layout<MODE>::TOTAL, st>>>(maps, k);
   return cudaGetLastError();
 }
 template <int MODE>
