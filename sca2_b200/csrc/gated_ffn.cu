@@ -194,22 +194,38 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t s) {
 }
 
 // ---- activations -----------------------------------------------------------------------------
+// The special function unit's 2^x and 1 / x without the handling of denormals around them: the
+// epilogues run beside the products and are bound by their instructions.  Relative error about
+// 2^-22; an overflow gives inf, and its reciprocal the 0 that the sigmoid has there.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid(float g) { return rcp_fast(1.f + exp2_fast(-LOG2E * g)); }
+
 template <int ACT>
 __device__ __forceinline__ float act_of(float g) {
-  if constexpr (ACT == SILU) return __fdividef(g, 1.f + __expf(-g));
-  else return g * (0.5f + 0.5f * erff(g * 0.70710678f));
+  if constexpr (ACT == SILU) return g * sigmoid(g);
+  else return g * fmaf(0.5f, erff(g * 0.70710678f), 0.5f);
 }
 // the activation and its derivative
 template <int ACT>
 __device__ __forceinline__ void act_grad(float g, float& a, float& da) {
   if constexpr (ACT == SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    const float s = sigmoid(g);
     a = g * s;
-    da = s * fmaf(g, 1.f - s, 1.f);
+    da = fmaf(a, 1.f - s, s);  // s (1 + g (1 - s))
   } else {
-    const float p = 0.5f + 0.5f * erff(g * 0.70710678f);
+    const float p = fmaf(0.5f, erff(g * 0.70710678f), 0.5f);
     a = g * p;
-    da = fmaf(g * 0.39894228f, __expf(-0.5f * g * g), p);
+    da = fmaf(g * 0.39894228f, exp2_fast(-0.5f * LOG2E * g * g), p);
   }
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
