@@ -94,9 +94,11 @@ int sca2_residual_norm_fwd(const sca2_rnorm_args* a, void* y, void* z, float* st
   if (!on(16, {stats})) return fail(SCA2_ERR_ARG, "residual_norm: stats must be 16-byte aligned");
   Args k = args(*a);
   k.y = y, k.z = z, k.stats = stats;
-  const bool vec = strides(*a, 8) && on(16, {k.x, k.u, k.gate_mode == 2 ? k.gate : nullptr, y, z, k.w, k.b, k.pw, k.pb, k.scale});
+  const bool vec = strides(*a, 4) && on(16, {k.x, k.u, k.gate_mode == 2 ? k.gate : nullptr, y, z, k.w, k.b, k.pw, k.pb, k.scale});
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->x_dtype == SCA2_BF16 ? fwd_bf16(k, a->u_dtype, vec, st) : fwd_f32(k, a->u_dtype, vec, st);
+  const auto f = a->x_dtype == SCA2_BF16 ? (a->u_dtype == SCA2_BF16 ? fwd_bf16_bf16 : fwd_bf16_f32)
+                                         : (a->u_dtype == SCA2_BF16 ? fwd_f32_bf16 : fwd_f32_f32);
+  const cudaError_t e = f(k, vec, st);
   return e == cudaSuccess ? SCA2_OK : cuda_fail(e, "sca2_residual_norm_fwd");
 }
 
@@ -130,7 +132,9 @@ int sca2_residual_norm_bwd(const sca2_rnorm_args* a, const float* stats, const v
   k.dy = dy, k.dz = dz, k.dx = g->dx, k.du = g->du, k.dgate = g->dgate, k.part = static_cast<float*>(work);
   const bool contig = strides(*a, 4) && on(16, {k.x, k.u, k.gate_mode == 2 ? k.gate : nullptr, dy, dz, k.dx, k.du,
                                                 k.gate_mode == 2 ? k.dgate : nullptr, k.w, k.b, k.pw, k.pb, k.scale});
-  cudaError_t e = a->x_dtype == SCA2_BF16 ? bwd_bf16(k, a->u_dtype, contig, st) : bwd_f32(k, a->u_dtype, contig, st);
+  const auto f = a->x_dtype == SCA2_BF16 ? (a->u_dtype == SCA2_BF16 ? bwd_bf16_bf16 : bwd_bf16_f32)
+                                         : (a->u_dtype == SCA2_BF16 ? bwd_f32_bf16 : bwd_f32_f32);
+  cudaError_t e = f(k, contig, st);
   if (e == cudaSuccess && (o.p[0] || o.p[1] || o.p[2] || o.p[3] || o.p[4])) {
     reduce_kernel<<<dim3((a->d + 31) / 32, NPART), 256, 0, st>>>(k.part, bwd_grid(a->rows, a->d), a->d, o);
     e = cudaGetLastError();

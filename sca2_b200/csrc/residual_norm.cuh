@@ -5,7 +5,7 @@
 // N is LayerNorm (biased variance, eps inside the root, weight and optional bias) or the RMS norm
 // with weight; gate is one logit for each value or for each row.  All arithmetic in fp32: y and z
 // are rounded once, when stored, and z is formed from the unrounded y.  Instantiated per type of
-// x and u (residual_norm_*.cu); z's type and the options are uniform runtime branches.
+// x and u (residual_norm_*.cu).
 //
 // Bound by memory.  Forward: the row stays in registers between its (up to four) reductions, so
 // everything is read and written once.  Backward: recomputes p, y and the normalised rows from the
@@ -104,32 +104,29 @@ __device__ __forceinline__ void store_dt(void* p, int64_t i, int dt, const float
 }
 
 // ---- forward --------------------------------------------------------------------------------
-// NT threads own a row (a warp, or the whole CTA of 256), each NV groups of VEC values: group k of
-// thread t starts at column VEC (t + NT k).
+// Wide or unaligned rows: the CTA owns a row, each thread NV groups of VEC values: group k of thread t
+// starts at column VEC (t + FT k).  Few registers, so that many CTAs hide each other's barriers.
 constexpr int FT = 256;
 
-template <int NT>
 __device__ __forceinline__ float row_sum(float v, int& flip) {
+  __shared__ float s[2][FT / 32];
   v = warp_sum(v);
-  if constexpr (NT > 32) {
-    __shared__ float s[2][NT / 32];
-    if ((threadIdx.x & 31) == 0) s[flip][threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
+  if ((threadIdx.x & 31) == 0) s[flip][threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) v += s[flip][w];
-    flip ^= 1;  // the next sum's writes pass this one's reads only after its own barrier
-  }
+  for (int w = 0; w < FT / 32; ++w) v += s[flip][w];
+  flip ^= 1;  // the next sum's writes pass this one's reads only after its own barrier
   return v;
 }
 
-template <int NT, int NV, int VEC, class TX, class TU>
-__global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(const Args a) {
-  const int t = threadIdx.x % NT;
+template <int NV, int VEC, class TX, class TU>
+__global__ void __launch_bounds__(FT, NV * VEC <= 4 ? 6 : NV * VEC <= 8 ? 4 : 3) fwd_kernel(const Args a) {
+  const int t = threadIdx.x;
   const int d = a.d;
   const float inv = 1.f / (float)d;
   int flip = 0;
-  const auto col = [&](int k) { return VEC * (t + NT * k); };
+  const auto col = [&](int k) { return VEC * (t + FT * k); };
   // mean and 1 / deviation of v, then v <- (v - mean) / deviation
   const auto normalise = [&](float (&v)[NV][VEC], float& mu, float& rs) {
     mu = 0.f;
@@ -139,7 +136,7 @@ __global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(con
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += v[k][j];  // columns past d hold 0
-      mu = row_sum<NT>(s, flip) * inv;
+      mu = row_sum(s, flip) * inv;
     }
     float q = 0.f;
 #pragma unroll
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(con
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[k][j] -= mu, q = fmaf(v[k][j], v[k][j], q);
       }
-    rs = rsqrtf(row_sum<NT>(q, flip) * inv + a.eps);
+    rs = rsqrtf(row_sum(q, flip) * inv + a.eps);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -166,8 +163,7 @@ __global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(con
     }
   };
 
-  const int64_t step = (int64_t)gridDim.x * (FT / NT);
-  for (int64_t row = (int64_t)blockIdx.x * (FT / NT) + threadIdx.x / NT; row < a.rows; row += step) {
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const TX* xr = reinterpret_cast<const TX*>(a.x) + row * a.sx;
     const TU* ur = reinterpret_cast<const TU*>(a.u) + row * a.su;
     const TU* gr = reinterpret_cast<const TU*>(a.gate) + row * a.sg;
@@ -217,6 +213,147 @@ __global__ void __launch_bounds__(FT, NT == 32 && NV > 2 ? 2 : 3) fwd_kernel(con
         store_dt<VEC>(a.z, row * d + col(k), a.zdt, x[k]);
       }
   }
+}
+
+// ---- asynchronous copies: a thread's own values of the rows to come, into its own slots of shared
+// memory, which no other thread reads: its wait for its copies is the only synchronisation.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Forward for rows of up to 1024 aligned values: a warp owns a row, each lane NG groups of four
+// values, so that every copy, load and store of the warp is one run of whole sectors in either type.
+// The slots hold one row: the next row's u is asked for once this row's is in registers, its x and
+// gate once the join has read this row's, and both travel under the rest of the row's work.
+template <int NG, int GATE, class TX, class TU>
+struct FwdRing {  // bytes of a thread's group in each array; the arrays' slots lie thread by thread
+  static constexpr int BU = 4 * sizeof(TU), BX = 4 * sizeof(TX), BG = GATE == 2 ? BU : 0;
+  static constexpr int OX = NG * BU * FT, OG = OX + NG * BX * FT, BYTES = OG + NG * BG * FT;
+};
+
+template <int NG, int GATE, bool POST, class TX, class TU>
+__global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
+  using L = FwdRing<NG, GATE, TX, TU>;
+  extern __shared__ __align__(16) uint8_t slots[];
+  const int lane = threadIdx.x & 31, d = a.d;
+  const float inv = 1.f / (float)d;
+  const auto col = [&](int k) { return 4 * (lane + 32 * k); };
+  const auto slot = [&](int off, int k, int bytes) { return slots + off + (k * FT + threadIdx.x) * bytes; };
+  const int64_t step = (int64_t)gridDim.x * (FT / 32);
+  int64_t row = (int64_t)blockIdx.x * (FT / 32) + (threadIdx.x >> 5);
+  const auto fetch_u = [&](int64_t r) {
+    if (r < a.rows) {
+      const TU* p = reinterpret_cast<const TU*>(a.u) + r * a.su;
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        if (col(k) < d) copy_async<L::BU>(slot(0, k, L::BU), p + col(k));
+    }
+    copies_commit();
+  };
+  const auto fetch_x = [&](int64_t r) {
+    if (r < a.rows) {
+      const TX* p = reinterpret_cast<const TX*>(a.x) + r * a.sx;
+      const TU* q = reinterpret_cast<const TU*>(a.gate) + r * a.sg;
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        if (col(k) < d) {
+          copy_async<L::BX>(slot(L::OX, k, L::BX), p + col(k));
+          if constexpr (GATE == 2) copy_async<L::BU>(slot(L::OG, k, L::BU), q + col(k));
+        }
+    }
+    copies_commit();
+  };
+  float y[NG][4];
+  const auto normalise = [&](float& mu, float& rs) {  // y <- y - mean
+    mu = 0.f;
+    if (!a.rms) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += y[k][j];  // columns past d hold 0
+      mu = warp_sum(s) * inv;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[k][j] -= mu, q = fmaf(y[k][j], y[k][j], q);
+      }
+    rs = rsqrtf(warp_sum(q) * inv + a.eps);
+  };
+  const auto affine = [&](int k, float rs, const float* w, const float* b) {  // y <- y rs w + b
+    float q[4], c[4] = {0.f, 0.f, 0.f, 0.f};
+    loadv<4>(w + col(k), q);
+    if (b) loadv<4>(b + col(k), c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[k][j] = fmaf(y[k][j] * rs, q[j], c[j]);
+  };
+
+  fetch_u(row), fetch_x(row);
+  for (; row < a.rows; row += step) {
+    float gt = 1.f;
+    if constexpr (GATE == 1) {
+      loadv<1>(reinterpret_cast<const TU*>(a.gate) + row * a.sg, &gt);
+      gt = sigmoid(gt);
+    }
+    copies_wait<1>();
+    float mu = 0.f, rs = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[k][j] = 0.f;
+      if (col(k) < d) loadv<4>(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
+    }
+    fetch_u(row + step);
+    if constexpr (POST) {
+      normalise(mu, rs);
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        if (col(k) < d) affine(k, rs, a.pw, a.pb);
+    }
+    if (a.stats && lane == 0) a.stats[4 * row] = mu, a.stats[4 * row + 1] = rs;
+    copies_wait<1>();
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+        float q[4];
+        if (a.scale) {
+          loadv<4>(a.scale + col(k), q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[k][j] *= q[j];
+        }
+        if constexpr (GATE == 2) {
+          loadv<4>(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[k][j] *= sigmoid(q[j]);
+        }
+        loadv<4>(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[k][j] = GATE == 1 ? fmaf(gt, y[k][j], q[j]) : y[k][j] + q[j];
+        storev<4>(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
+      }
+    fetch_x(row + step);
+    if (!a.z) continue;
+    normalise(mu, rs);
+    if (a.stats && lane == 0) a.stats[4 * row + 2] = mu, a.stats[4 * row + 3] = rs;
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+        affine(k, rs, a.w, a.b);
+        store_dt<4>(a.z, row * d + col(k), a.zdt, y[k]);
+      }
+  }
+  copies_wait<0>();
 }
 
 // ---- backward -------------------------------------------------------------------------------
@@ -421,46 +558,278 @@ __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
   if (post && a.pb) store(part + PART_PB * d, apb);
 }
 
-// rows in flight in a CTA, and the CTAs (each leaves one row of partials)
-inline int bwd_rows_per_step(int64_t rows, int d) { return d > 1024 ? 1 : rows >= 148 * 6 ? 2 : 1; }
+// Backward for rows of up to 1024 aligned values, many of them: as bwd_kernel with the options that
+// cost instructions as template parameters, and the rows to come on their way into shared memory
+// (STAGES - 1 steps ahead) while the present ones are reduced.
+template <int GATE, bool HASZ, class TX, class TU>
+struct BwdRing {
+  static constexpr int R = 2, STAGES = 3, MAXT = 256;
+  // offsets of a row's slots, in bytes of one thread; every array's slots lie thread by thread
+  static constexpr int BX = 4 * sizeof(TX), BU = 4 * sizeof(TU), BZ = 16;
+  static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0),
+                       OST = OZ + (HASZ ? BZ : 0), ROW = OST + 16;
+};
+template <class T>
+__device__ __forceinline__ void slot_read(const uint8_t* p, float (&v)[4]) {
+  loadv<4>(reinterpret_cast<const T*>(p), v);
+}
+
+template <int GATE, bool POST, bool HASZ, class TX, class TU>
+__global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
+  using L = BwdRing<GATE, HASZ, TX, TU>;
+  constexpr int W = 8, R = L::R, ST = L::STAGES;
+  __shared__ __align__(16) float red[2][3 * R * W];
+  extern __shared__ __align__(16) uint8_t slots[];
+  const int t = threadIdx.x, T = blockDim.x, d = a.d;
+  const float inv = 1.f / (float)d;
+  const bool mine = 4 * t < d;
+  for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
+  __syncthreads();
+  const auto param = [&](const float* p, float fill, float (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = mine ? fill : 0.f;  // columns past d: kept out of the sums
+    if (p && mine) loadv<4>(p + 4 * t, v);
+  };
+  float w[4], sc[4], pw[4], pb[4];
+  if constexpr (HASZ) param(a.w, 0.f, w);
+  param(a.scale, 1.f, sc);
+  if constexpr (POST) param(a.pw, 1.f, pw), param(a.pb, 0.f, pb);
+  float aw[4] = {}, ab[4] = {}, as[4] = {}, apw[4] = {}, apb[4] = {};
+
+  const int64_t step = (int64_t)gridDim.x * R;
+  const auto slot = [&](int stage, int i, int off, int bytes) {
+    return slots + (int64_t)(stage * R + i) * L::ROW * T + off * T + bytes * t;
+  };
+  const auto fetch = [&](int64_t r0, int stage) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = r0 + i;
+      if (r < a.rows && mine) {
+        copy_async<L::BU>(slot(stage, i, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su + 4 * t);
+        copy_async<L::BX>(slot(stage, i, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx + 4 * t);
+        if (a.dy) copy_async<L::BX>(slot(stage, i, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d + 4 * t);
+        if constexpr (GATE == 2)
+          copy_async<L::BU>(slot(stage, i, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg + 4 * t);
+        if constexpr (HASZ) {
+          if (a.zdt == SCA2_BF16) copy_async<8>(slot(stage, i, L::OZ, L::BZ), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d + 4 * t);
+          else copy_async<16>(slot(stage, i, L::OZ, L::BZ), reinterpret_cast<const float*>(a.dz) + r * d + 4 * t);
+        }
+        copy_async<16>(slot(stage, i, L::OST, 16), a.stats + 4 * r);
+      }
+    }
+    copies_commit();
+  };
+  int flip = 0;
+  int64_t r0 = (int64_t)blockIdx.x * R;
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) fetch(r0 + s * step, s);
+  for (int stage = 0; r0 < a.rows; r0 += step, stage = stage + 1 == ST ? 0 : stage + 1) {
+    fetch(r0 + (ST - 1) * step, stage == 0 ? ST - 1 : stage - 1);
+    float tok[R];
+    if constexpr (GATE == 1) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        tok[i] = 0.f;
+        if (r0 + i < a.rows) loadv<1>(reinterpret_cast<const TU*>(a.gate) + (r0 + i) * a.sg, &tok[i]);
+      }
+    }
+    copies_wait<ST - 1>();
+    float un[R][4], s[R][4], dy[R][4], yn[R][4], dn[R][4], v[3 * R], ru[R], ry[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float st[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) un[i][k] = dy[i][k] = yn[i][k] = dn[i][k] = st[k] = 0.f, s[i][k] = 1.f;
+      if (r0 + i < a.rows && mine) {
+        slot_read<float>(slot(stage, i, L::OST, 16), st);
+        slot_read<TU>(slot(stage, i, L::OU, L::BU), un[i]);
+        if constexpr (HASZ) slot_read<TX>(slot(stage, i, L::OX, L::BX), yn[i]);
+        if (a.dy) slot_read<TX>(slot(stage, i, L::ODY, L::BX), dy[i]);
+        if constexpr (GATE == 2) slot_read<TU>(slot(stage, i, L::OG, L::BU), s[i]);
+        if constexpr (HASZ) {
+          if (a.zdt == SCA2_BF16) slot_read<__nv_bfloat16>(slot(stage, i, L::OZ, L::BZ), dn[i]);
+          else slot_read<float>(slot(stage, i, L::OZ, L::BZ), dn[i]);
+        }
+      }
+      ru[i] = st[1], ry[i] = st[3];
+      v[2 * i] = v[2 * i + 1] = 0.f;
+      const float g1 = GATE == 1 ? sigmoid(tok[i]) : 1.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (POST) un[i][k] = (un[i][k] - st[0]) * ru[i];
+        if constexpr (GATE == 1) s[i][k] = g1;
+        if constexpr (GATE == 2) s[i][k] = sigmoid(s[i][k]);
+        if constexpr (HASZ) {
+          const float p = POST ? fmaf(un[i][k], pw[k], pb[k]) : un[i][k];
+          const float y = fmaf(GATE ? sc[k] * s[i][k] : sc[k], p, yn[i][k]);
+          yn[i][k] = (y - st[2]) * ry[i];
+          aw[k] = fmaf(dn[i][k], yn[i][k], aw[k]);
+          ab[k] += dn[i][k];
+          dn[i][k] *= w[k];
+          v[2 * i] += dn[i][k];
+          v[2 * i + 1] = fmaf(dn[i][k], yn[i][k], v[2 * i + 1]);
+        }
+      }
+    }
+    if constexpr (HASZ) {
+      cta_sums<2 * R, W>(v, red[flip]);
+      flip ^= 1;
+    }
+    float q[3 * R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = r0 + i;
+      if constexpr (HASZ) {
+        const float m1 = a.rms ? 0.f : v[2 * i] * inv, m2 = v[2 * i + 1] * inv;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dy[i][k] = fmaf(ry[i], dn[i][k] - m1 - yn[i][k] * m2, dy[i][k]);
+      }
+      const bool in = r < a.rows && mine;
+      if (in) storev<4>(reinterpret_cast<TX*>(a.dx) + r * d + 4 * t, dy[i]);
+      float q0 = 0.f, q1 = 0.f, q2 = 0.f, dg[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float p = POST ? fmaf(un[i][k], pw[k], pb[k]) : un[i][k];
+        const float es = GATE ? dy[i][k] * s[i][k] : dy[i][k], dp = es * sc[k];
+        as[k] = fmaf(es, p, as[k]);
+        if constexpr (GATE != 0) {
+          dg[k] = dp * p * (1.f - s[i][k]);
+          if constexpr (GATE == 1) q2 += dg[k];
+        }
+        if constexpr (POST) {
+          apw[k] = fmaf(dp, un[i][k], apw[k]);
+          apb[k] += dp;
+          dn[i][k] = dp * pw[k];
+          q0 += dn[i][k];
+          q1 = fmaf(dn[i][k], un[i][k], q1);
+        } else {
+          dn[i][k] = dp;
+        }
+      }
+      if constexpr (GATE == 2)
+        if (in) storev<4>(reinterpret_cast<TU*>(a.dgate) + r * d + 4 * t, dg);
+      q[3 * i] = q0, q[3 * i + 1] = q1, q[3 * i + 2] = q2;
+    }
+    if constexpr (POST && GATE == 1) {
+      cta_sums<3 * R, W>(q, red[flip]);
+      flip ^= 1;
+    } else if constexpr (POST || GATE == 1) {
+      float h[2 * R];  // two sums a row, or one
+      constexpr int N = POST ? 2 * R : R;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if constexpr (POST) h[2 * i] = q[3 * i], h[2 * i + 1] = q[3 * i + 1];
+        else h[i] = q[3 * i + 2];
+      }
+      cta_sums<N, W>(h, red[flip]);
+      flip ^= 1;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if constexpr (POST) q[3 * i] = h[2 * i], q[3 * i + 1] = h[2 * i + 1];
+        else q[3 * i + 2] = h[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = r0 + i;
+      if (r >= a.rows) continue;
+      if constexpr (POST) {
+        const float m1 = a.rms ? 0.f : q[3 * i] * inv, m2 = q[3 * i + 1] * inv;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dn[i][k] = ru[i] * (dn[i][k] - m1 - un[i][k] * m2);
+      }
+      if (mine) storev<4>(reinterpret_cast<TU*>(a.du) + r * d + 4 * t, dn[i]);
+      if constexpr (GATE == 1)
+        if (t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &q[3 * i + 2]);
+    }
+  }
+  copies_wait<0>();
+  if (!mine) return;
+  float* part = a.part + (int64_t)blockIdx.x * NPART * d + 4 * t;
+  if constexpr (HASZ) {
+    storev<4>(part + PART_W * d, aw);
+    if (a.b) storev<4>(part + PART_B * d, ab);
+  }
+  if (a.scale) storev<4>(part + PART_SCALE * d, as);
+  if constexpr (POST) {
+    storev<4>(part + PART_PW * d, apw);
+    if (a.pb) storev<4>(part + PART_PB * d, apb);
+  }
+}
+
+// Rows in flight in a CTA, and the CTAs (each leaves one row of partials): two to an SM, three of the
+// few-row kernel.  `many`: rows enough that every CTA of bwd_ring (or its unaligned form) has several steps.
+inline bool many(int64_t rows, int d) { return d <= 1024 && rows >= 148 * 8; }
 inline int bwd_grid(int64_t rows, int d) {
-  const int R = bwd_rows_per_step(rows, d), most = 148 * (d > 2048 ? 1 : d > 1024 ? 2 : 3);
-  const int64_t want = (rows + R - 1) / R;
+  const bool m = many(rows, d);
+  const int most = 148 * (d > 2048 ? 1 : d > 1024 || m ? 2 : 3);
+  const int64_t want = m ? (rows + 1) / 2 : rows;
   return (int)(want < most ? want : most);
 }
 
+template <int NG, int GATE, bool POST, class TX, class TU>
+cudaError_t fwd_ring_launch(const Args& a, cudaStream_t st) {
+  constexpr int smem = FwdRing<NG, GATE, TX, TU>::BYTES;
+  const auto k = fwd_ring<NG, GATE, POST, TX, TU>;
+  if (smem > 48 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  const int64_t want = (a.rows + 7) / 8;
+  k<<<(int)(want < 148 * 3 ? want : 148 * 3), FT, smem, st>>>(a);
+  return cudaGetLastError();
+}
+template <int GATE, bool POST, class TX, class TU>
+cudaError_t fwd_ring_width(const Args& a, cudaStream_t st) {
+  switch ((a.d + 255) / 256) {
+    case 1: return fwd_ring_launch<2, GATE, POST, TX, TU>(a, st);
+    case 2: return fwd_ring_launch<4, GATE, POST, TX, TU>(a, st);
+    case 3: return fwd_ring_launch<6, GATE, POST, TX, TU>(a, st);
+    default: return fwd_ring_launch<8, GATE, POST, TX, TU>(a, st);
+  }
+}
+template <bool POST, class TX, class TU>
+cudaError_t fwd_ring_gate(const Args& a, cudaStream_t st) {
+  return a.gate_mode == 0 ? fwd_ring_width<0, POST, TX, TU>(a, st)
+         : a.gate_mode == 1 ? fwd_ring_width<1, POST, TX, TU>(a, st) : fwd_ring_width<2, POST, TX, TU>(a, st);
+}
+// vec: rows and pointers allow groups of four values
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   const int d = a.d;
-  const bool warp = vec && d <= 1024;
-  const int64_t want = warp ? (a.rows + 7) / 8 : a.rows;
-  const int grid = (int)(want < 148 * 8 ? want : 148 * 8);
-  if (warp) {
-    switch ((d + 255) / 256) {
-      case 1: fwd_kernel<32, 1, 8, TX, TU><<<grid, FT, 0, st>>>(a); break;
-      case 2: fwd_kernel<32, 2, 8, TX, TU><<<grid, FT, 0, st>>>(a); break;
-      case 3: fwd_kernel<32, 3, 8, TX, TU><<<grid, FT, 0, st>>>(a); break;
-      default: fwd_kernel<32, 4, 8, TX, TU><<<grid, FT, 0, st>>>(a); break;
-    }
-  } else if (vec) {
-    if (d <= 2048) fwd_kernel<256, 1, 8, TX, TU><<<grid, FT, 0, st>>>(a);
-    else fwd_kernel<256, 2, 8, TX, TU><<<grid, FT, 0, st>>>(a);
+  if (vec && d <= 1024) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
+  const int grid = (int)(a.rows < 148 * 8 ? a.rows : 148 * 8);
+  if (vec) {
+    if (d <= 2048) fwd_kernel<2, 4, TX, TU><<<grid, FT, 0, st>>>(a);
+    else fwd_kernel<4, 4, TX, TU><<<grid, FT, 0, st>>>(a);
   } else {
-    if (d <= 1024) fwd_kernel<256, 4, 1, TX, TU><<<grid, FT, 0, st>>>(a);
-    else fwd_kernel<256, 16, 1, TX, TU><<<grid, FT, 0, st>>>(a);
+    if (d <= 1024) fwd_kernel<4, 1, TX, TU><<<grid, FT, 0, st>>>(a);
+    else fwd_kernel<16, 1, TX, TU><<<grid, FT, 0, st>>>(a);
   }
   return cudaGetLastError();
 }
 
+template <int GATE, bool POST, bool HASZ, class TX, class TU>
+cudaError_t bwd_ring_launch(const Args& a, cudaStream_t st) {
+  using L = BwdRing<GATE, HASZ, TX, TU>;
+  const int T = ((a.d + 3) / 4 + 31) / 32 * 32, smem = L::STAGES * L::R * L::ROW * T;
+  const auto k = bwd_ring<GATE, POST, HASZ, TX, TU>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, L::STAGES * L::R * L::ROW * L::MAXT)) return e;
+  k<<<bwd_grid(a.rows, a.d), T, smem, st>>>(a);
+  return cudaGetLastError();
+}
+template <int GATE, class TX, class TU>
+cudaError_t bwd_ring_gate(const Args& a, cudaStream_t st) {
+  if (a.pw) return a.dz ? bwd_ring_launch<GATE, true, true, TX, TU>(a, st) : bwd_ring_launch<GATE, true, false, TX, TU>(a, st);
+  return a.dz ? bwd_ring_launch<GATE, false, true, TX, TU>(a, st) : bwd_ring_launch<GATE, false, false, TX, TU>(a, st);
+}
 template <bool CONTIG, class TX, class TU>
 cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
-  const int d = a.d, R = bwd_rows_per_step(a.rows, d), grid = bwd_grid(a.rows, d);
+  const int d = a.d, grid = bwd_grid(a.rows, d);
   const int T = ((d + 3) / 4 + 31) / 32 * 32;
   if (d > 2048) bwd_kernel<1024, 1, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   else if (d > 1024) bwd_kernel<512, 1, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (R == 2 && T <= 192) bwd_kernel<192, 2, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (R == 2) bwd_kernel<256, 2, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (!many(a.rows, d)) bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if constexpr (!CONTIG) bwd_kernel<256, 2, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else return a.gate_mode == 0 ? bwd_ring_gate<0, TX, TU>(a, st) : a.gate_mode == 1 ? bwd_ring_gate<1, TX, TU>(a, st) : bwd_ring_gate<2, TX, TU>(a, st);
   return cudaGetLastError();
 }
 template <class TX, class TU>
@@ -468,11 +837,15 @@ cudaError_t bwd_types(const Args& a, bool contig, cudaStream_t st) {
   return contig ? bwd_launch<true, TX, TU>(a, st) : bwd_launch<false, TX, TU>(a, st);
 }
 
-// one translation unit for each type of x
-cudaError_t fwd_f32(const Args& a, int udt, bool vec, cudaStream_t st);
-cudaError_t fwd_bf16(const Args& a, int udt, bool vec, cudaStream_t st);
-cudaError_t bwd_f32(const Args& a, int udt, bool contig, cudaStream_t st);
-cudaError_t bwd_bf16(const Args& a, int udt, bool contig, cudaStream_t st);
+// one translation unit for each pair of types
+cudaError_t fwd_f32_f32(const Args& a, bool vec, cudaStream_t st);
+cudaError_t fwd_f32_bf16(const Args& a, bool vec, cudaStream_t st);
+cudaError_t fwd_bf16_f32(const Args& a, bool vec, cudaStream_t st);
+cudaError_t fwd_bf16_bf16(const Args& a, bool vec, cudaStream_t st);
+cudaError_t bwd_f32_f32(const Args& a, bool contig, cudaStream_t st);
+cudaError_t bwd_f32_bf16(const Args& a, bool contig, cudaStream_t st);
+cudaError_t bwd_bf16_f32(const Args& a, bool contig, cudaStream_t st);
+cudaError_t bwd_bf16_bf16(const Args& a, bool contig, cudaStream_t st);
 
 }  // namespace rnorm
 }  // namespace sca2

@@ -1638,49 +1638,56 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
 # ======================================================================================
 #  global gradient norm and clipping
 # ======================================================================================
-_shape, _dtype, _layout = (operator.attrgetter(n) for n in ("shape", "dtype", "layout"))
+_dtype = operator.attrgetter("dtype")
 _T = torch.Tensor
 
 
 def _grad_list(what: str, grads, out=None):
+    """The call's tensors, the types of the gradients and of the destinations, and the device."""
     grads = [grads] if isinstance(grads, _T) else list(grads)
     outs = grads if out is None else ([out] if isinstance(out, _T) else list(out))
     E = _lib.Sca2Error
     if len(outs) != len(grads):
         raise E(f"{what}: {len(grads)} gradients and {len(outs)} destinations")
-    every = grads if out is None else grads + outs
-    if not all([isinstance(t, _T) for t in every]) or not set(map(_dtype, every)) <= _DT.keys() \
-            or set(map(_layout, every)) - {torch.strided}:
-        raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
-    if not every:
-        return grads, outs, None
-    dev = set(map(_T.get_device, every))
-    dev = dev.pop() if len(dev) == 1 and min(dev) >= 0 else _need_cuda(*every).index
-    if out is not None and (list(map(_shape, grads)) != list(map(_shape, outs)) or not all(map(_T.is_contiguous, outs))):
-        raise E(f"{what}: a destination must be contiguous, with its gradient's shape")
-    return grads, outs, dev
+    dev, types = None, []
+    for ts in (grads,) if out is None else (grads, outs):
+        if not all([isinstance(t, _T) for t in ts]):
+            raise E(f"{what}: gradients must be tensors")
+        types.append(list(map(_dtype, ts)))
+        if not set(types[-1]) <= _DT.keys() or any([t.is_sparse for t in ts]):
+            raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
+        devs = set(map(_T.get_device, ts))
+        if ts and (len(devs) != 1 or min(devs) < 0 or dev not in (None, *devs)):
+            devs = {_need_cuda(*grads, *outs).index}
+        dev = devs.pop() if devs else None
+    if out is not None and not all(map(_T.is_contiguous, outs)):
+        raise E(f"{what}: a destination must be contiguous")
+    return grads, outs, types, dev
 
 
-def _grad_table(src, dst):
-    """The sca2_grad_tensor list as bytes (host memory; the library copies it into the launch)."""
-    n = len(src)
+def _grad_table(src, dst, types):
+    """The sca2_grad_tensor list as bytes (host memory; the library copies it into the launch).  A
+    destination has its gradient's number of values."""
+    n, numel = len(src), list(map(_T.numel, src))
+    if dst is not src and list(map(_T.numel, dst)) != numel:
+        raise _lib.Sca2Error("clip_grads: a destination must have its gradient's shape")
+    codes = [[_DT[t[0]]] * n if len(set(t)) == 1 else [_DT[x] for x in t] for t in types]
     flat = [0] * (5 * n)
-    flat[0::5] = map(_T.data_ptr, src)
-    flat[1::5] = map(_T.data_ptr, dst) if dst is not src else flat[0::5]
-    flat[2::5] = map(_T.numel, src)
-    flat[3::5] = map(_DT.__getitem__, map(_dtype, src))
-    flat[4::5] = map(_DT.__getitem__, map(_dtype, dst)) if dst is not src else flat[3::5]
+    flat[0::5] = ptrs = list(map(_T.data_ptr, src))
+    flat[1::5] = ptrs if dst is src else map(_T.data_ptr, dst)
+    flat[2::5] = numel
+    flat[3::5], flat[4::5] = codes[0], codes[-1]
     return struct.pack("=" + "QQqii" * n, *flat)
 
 
-def _clip_run(grads, outs, max_norm: Optional[float], dev: int) -> torch.Tensor:
+def _clip_run(grads, outs, types, max_norm: Optional[float], dev: int) -> torch.Tensor:
     # a gradient that is not contiguous goes through a contiguous copy
     src, back = grads, ()
     if not all(map(_T.is_contiguous, grads)):
         src = [g.contiguous() for g in grads]
         if outs is grads:
             back = [(g, s) for g, s in zip(grads, src) if g is not s]
-    table, n, lib = _grad_table(src, src if outs is grads else outs), len(src), _lib.load()
+    table, n, lib = _grad_table(src, src if outs is grads else outs, types), len(src), _lib.load()
     norm = src[0].new_empty((), dtype=torch.float32)
     nb = lib.sca2_clip_grads_work_bytes(n)
     work = src[0].new_empty(nb, dtype=torch.uint8)
@@ -1700,7 +1707,8 @@ def _clip_run(grads, outs, max_norm: Optional[float], dev: int) -> torch.Tensor:
 @torch.library.custom_op("sca2b200::grad_norm", mutates_args=())
 def _grad_norm_op(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """sca2_grad_norm over a list of tensors."""
-    return _clip_run(grads, grads, None, grads[0].get_device())
+    grads, outs, types, dev = _grad_list("grad_norm", grads)
+    return _clip_run(grads, outs, types, None, dev)
 
 
 @_grad_norm_op.register_fake
@@ -1711,7 +1719,8 @@ def _(grads):
 @torch.library.custom_op("sca2b200::clip_grads_", mutates_args=("grads",))
 def _clip_grads_op(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
     """sca2_clip_grads in place over a list of tensors; returns the norm before."""
-    return _clip_run(grads, grads, max_norm, grads[0].get_device())
+    grads, outs, types, dev = _grad_list("clip_grads", grads)
+    return _clip_run(grads, outs, types, max_norm, dev)
 
 
 @_clip_grads_op.register_fake
@@ -1723,31 +1732,31 @@ def grad_norm(grads) -> torch.Tensor:
     """2-norm of all values of the tensors together (fp32 scalar on their device; summed in 64 bits
     in a fixed order).  grads: a tensor or a list of float32 / bfloat16 tensors on one device; no
     tensor gives 0 (on the current CUDA device).  Not differentiable."""
-    grads, outs, dev = _grad_list("grad_norm", grads)
+    grads, outs, types, dev = _grad_list("grad_norm", grads)
     if not grads:
         return torch.zeros((), device="cuda")
     with torch.no_grad():
         if torch.compiler.is_compiling():
             return torch.ops.sca2b200.grad_norm(grads)
-        return _clip_run(grads, outs, None, dev)
+        return _clip_run(grads, outs, types, None, dev)
 
 
 def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     """Scale the gradients so that their global 2-norm is at most max_norm, and return the norm
     before (fp32 scalar; nothing waits for the device): g * min(1, max_norm / (norm + 1e-6)), as
     torch.nn.utils.clip_grad_norm_.  In place, or into the contiguous tensors `out` (float32 or
-    bfloat16, one for each gradient).  A tensor that is written may not share memory with another
+    bfloat16, one for each gradient, with as many values).  A tensor that is written may not share memory with another
     of the call (refused).  Not differentiable."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise _lib.Sca2Error("clip_grads: max_norm must be >= 0")
-    grads, outs, dev = _grad_list("clip_grads", grads, out)
+    grads, outs, types, dev = _grad_list("clip_grads", grads, out)
     if not grads:
         return torch.zeros((), device="cuda")
     with torch.no_grad():
         if torch.compiler.is_compiling() and out is None:
             return torch.ops.sca2b200.clip_grads_(grads, max_norm)
-        norm = _clip_run(grads, outs, max_norm, dev)
+        norm = _clip_run(grads, outs, types, max_norm, dev)
     torch.autograd.graph.increment_version(outs)
     return norm
 

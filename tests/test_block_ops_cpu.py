@@ -32,7 +32,8 @@ def test_struct_layouts():
         got = [int(x) for x in subprocess.run([c + ".x"], capture_output=True, text=True, check=True).stdout.split()]
     want = [v for cls, fs in fields.values() for v in [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in fs]]
     assert got == want
-    assert len(ops._grad_table([torch.zeros(3)] * 2, [torch.zeros(3)] * 2)) == 2 * ctypes.sizeof(_lib.GradTensor)
+    t = [torch.zeros(3)] * 2
+    assert len(ops._grad_table(t, t, [[torch.float32] * 2])) == 2 * ctypes.sizeof(_lib.GradTensor)
 
 
 def test_cpu_tensors_are_refused():
