@@ -36,7 +36,53 @@ struct Args {
 
 enum { PART_W, PART_B, PART_SCALE, PART_PW, PART_PB, NPART };
 
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// sigmoid by the special function unit's 2^x and 1 / x (relative error about 2^-22; 2^x overflows to
+// inf, whose reciprocal is the 0 that belongs there)
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid(float v) { return rcp_fast(1.f + exp2_fast(-LOG2E * v)); }
+
+// two fp32 values in one instruction (add, mul, fma of sm_100), each rounded as by itself: the
+// kernels of aligned rows issue about half the instructions with them
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+  return {((uint64_t)__float_as_uint(b) << 32) | __float_as_uint(a)};
+}
+__device__ __forceinline__ F2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ float first(F2 a) { return __uint_as_float((uint32_t)a.v); }
+__device__ __forceinline__ float second(F2 a) { return __uint_as_float((uint32_t)(a.v >> 32)); }
+__device__ __forceinline__ float sum(F2 a) { return first(a) + second(a); }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ F2 sigmoid(F2 v) {
+  const F2 t = v * both(-LOG2E);
+  const F2 e = pair(exp2_fast(first(t)), exp2_fast(second(t))) + both(1.f);
+  return pair(rcp_fast(first(e)), rcp_fast(second(e)));
+}
 
 __device__ __forceinline__ void unpack2(uint32_t u, float* v) {
   v[0] = __uint_as_float(u << 16), v[1] = __uint_as_float(u & 0xFFFF0000u);
@@ -215,6 +261,19 @@ __global__ void __launch_bounds__(FT, NV * VEC <= 4 ? 6 : NV * VEC <= 8 ? 4 : 3)
   }
 }
 
+// four consecutive values as two pairs
+template <class T>
+__device__ __forceinline__ void load2(const T* p, F2 (&v)[2]) {
+  float q[4];
+  loadv<4>(p, q);
+  v[0] = pair(q[0], q[1]), v[1] = pair(q[2], q[3]);
+}
+template <class T>
+__device__ __forceinline__ void store2(T* p, const F2 (&v)[2]) {
+  const float q[4] = {first(v[0]), second(v[0]), first(v[1]), second(v[1])};
+  storev<4>(p, q);
+}
+
 // ---- asynchronous copies: a thread's own values of the rows to come, into its own slots of shared
 // memory, which no other thread reads: its wait for its copies is the only synchronisation.
 template <int BYTES>
@@ -271,32 +330,31 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     }
     copies_commit();
   };
-  float y[NG][4];
+  F2 y[NG][2];
   const auto normalise = [&](float& mu, float& rs) {  // y <- y - mean
     mu = 0.f;
     if (!a.rms) {
-      float s = 0.f;
+      F2 s = both(0.f);
 #pragma unroll
-      for (int k = 0; k < NG; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += y[k][j];  // columns past d hold 0
-      mu = warp_sum(s) * inv;
+      for (int k = 0; k < NG; ++k) s = s + (y[k][0] + y[k][1]);  // columns past d hold 0
+      mu = warp_sum(sum(s)) * inv;
     }
-    float q = 0.f;
+    const F2 m = both(-mu);
+    F2 q0 = both(0.f), q1 = q0;
 #pragma unroll
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[k][j] -= mu, q = fmaf(y[k][j], y[k][j], q);
+        y[k][0] = y[k][0] + m, y[k][1] = y[k][1] + m;
+        q0 = fma(y[k][0], y[k][0], q0), q1 = fma(y[k][1], y[k][1], q1);
       }
-    rs = rsqrtf(warp_sum(q) * inv + a.eps);
+    rs = rsqrtf(warp_sum(sum(q0 + q1)) * inv + a.eps);
   };
   const auto affine = [&](int k, float rs, const float* w, const float* b) {  // y <- y rs w + b
-    float q[4], c[4] = {0.f, 0.f, 0.f, 0.f};
-    loadv<4>(w + col(k), q);
-    if (b) loadv<4>(b + col(k), c);
+    F2 q[2], c[2] = {both(0.f), both(0.f)};
+    load2(w + col(k), q);
+    if (b) load2(b + col(k), c);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[k][j] = fmaf(y[k][j] * rs, q[j], c[j]);
+    for (int j = 0; j < 2; ++j) y[k][j] = fma(y[k][j] * both(rs), q[j], c[j]);
   };
 
   fetch_u(row), fetch_x(row);
@@ -310,9 +368,8 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     float mu = 0.f, rs = 0.f;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[k][j] = 0.f;
-      if (col(k) < d) loadv<4>(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
+      y[k][0] = y[k][1] = both(0.f);
+      if (col(k) < d) load2(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
     }
     fetch_u(row + step);
     if constexpr (POST) {
@@ -326,21 +383,19 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
 #pragma unroll
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
-        float q[4];
+        F2 q[2];
         if (a.scale) {
-          loadv<4>(a.scale + col(k), q);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[k][j] *= q[j];
+          load2(a.scale + col(k), q);
+          y[k][0] = y[k][0] * q[0], y[k][1] = y[k][1] * q[1];
         }
         if constexpr (GATE == 2) {
-          loadv<4>(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[k][j] *= sigmoid(q[j]);
+          load2(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
+          y[k][0] = y[k][0] * sigmoid(q[0]), y[k][1] = y[k][1] * sigmoid(q[1]);
         }
-        loadv<4>(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
+        load2(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[k][j] = GATE == 1 ? fmaf(gt, y[k][j], q[j]) : y[k][j] + q[j];
-        storev<4>(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
+        for (int j = 0; j < 2; ++j) y[k][j] = GATE == 1 ? fma(both(gt), y[k][j], q[j]) : y[k][j] + q[j];
+        store2(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
       }
     fetch_x(row + step);
     if (!a.z) continue;
@@ -350,7 +405,8 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
         affine(k, rs, a.w, a.b);
-        store_dt<4>(a.z, row * d + col(k), a.zdt, y[k]);
+        if (a.zdt == SCA2_BF16) store2(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), y[k]);
+        else store2(reinterpret_cast<float*>(a.z) + row * d + col(k), y[k]);
       }
   }
   copies_wait<0>();
@@ -569,11 +625,6 @@ struct BwdRing {
   static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0),
                        OST = OZ + (HASZ ? BZ : 0), ROW = OST + 16;
 };
-template <class T>
-__device__ __forceinline__ void slot_read(const uint8_t* p, float (&v)[4]) {
-  loadv<4>(reinterpret_cast<const T*>(p), v);
-}
-
 template <int GATE, bool POST, bool HASZ, class TX, class TU>
 __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
   using L = BwdRing<GATE, HASZ, TX, TU>;
@@ -585,16 +636,16 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
   const bool mine = 4 * t < d;
   for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
   __syncthreads();
-  const auto param = [&](const float* p, float fill, float (&v)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = mine ? fill : 0.f;  // columns past d: kept out of the sums
-    if (p && mine) loadv<4>(p + 4 * t, v);
+  const auto param = [&](const float* p, float fill, F2 (&v)[2]) {
+    v[0] = v[1] = both(mine ? fill : 0.f);  // columns past d: kept out of the sums
+    if (p && mine) load2(p + 4 * t, v);
   };
-  float w[4], sc[4], pw[4], pb[4];
+  const F2 zero = both(0.f), one = both(1.f), minus = both(-1.f);
+  F2 w[2], sc[2], pw[2], pb[2];
   if constexpr (HASZ) param(a.w, 0.f, w);
   param(a.scale, 1.f, sc);
   if constexpr (POST) param(a.pw, 1.f, pw), param(a.pb, 0.f, pb);
-  float aw[4] = {}, ab[4] = {}, as[4] = {}, apw[4] = {}, apb[4] = {};
+  F2 aw[2] = {zero, zero}, ab[2] = {zero, zero}, as[2] = {zero, zero}, apw[2] = {zero, zero}, apb[2] = {zero, zero};
 
   const int64_t step = (int64_t)gridDim.x * R;
   const auto slot = [&](int stage, int i, int off, int bytes) {
@@ -634,42 +685,44 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
       }
     }
     copies_wait<ST - 1>();
-    float un[R][4], s[R][4], dy[R][4], yn[R][4], dn[R][4], v[3 * R], ru[R], ry[R];
+    F2 un[R][2], s[R][2], dy[R][2], yn[R][2], dn[R][2];
+    float v[2 * R], ru[R], ry[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      float st[4];
+      float st[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) un[i][k] = dy[i][k] = yn[i][k] = dn[i][k] = st[k] = 0.f, s[i][k] = 1.f;
+      for (int j = 0; j < 2; ++j) un[i][j] = dy[i][j] = yn[i][j] = dn[i][j] = zero, s[i][j] = one;
       if (r0 + i < a.rows && mine) {
-        slot_read<float>(slot(stage, i, L::OST, 16), st);
-        slot_read<TU>(slot(stage, i, L::OU, L::BU), un[i]);
-        if constexpr (HASZ) slot_read<TX>(slot(stage, i, L::OX, L::BX), yn[i]);
-        if (a.dy) slot_read<TX>(slot(stage, i, L::ODY, L::BX), dy[i]);
-        if constexpr (GATE == 2) slot_read<TU>(slot(stage, i, L::OG, L::BU), s[i]);
+        loadv<4>(reinterpret_cast<const float*>(slot(stage, i, L::OST, 16)), st);
+        load2(reinterpret_cast<const TU*>(slot(stage, i, L::OU, L::BU)), un[i]);
+        if constexpr (HASZ) load2(reinterpret_cast<const TX*>(slot(stage, i, L::OX, L::BX)), yn[i]);
+        if (a.dy) load2(reinterpret_cast<const TX*>(slot(stage, i, L::ODY, L::BX)), dy[i]);
+        if constexpr (GATE == 2) load2(reinterpret_cast<const TU*>(slot(stage, i, L::OG, L::BU)), s[i]);
         if constexpr (HASZ) {
-          if (a.zdt == SCA2_BF16) slot_read<__nv_bfloat16>(slot(stage, i, L::OZ, L::BZ), dn[i]);
-          else slot_read<float>(slot(stage, i, L::OZ, L::BZ), dn[i]);
+          if (a.zdt == SCA2_BF16) load2(reinterpret_cast<const __nv_bfloat16*>(slot(stage, i, L::OZ, L::BZ)), dn[i]);
+          else load2(reinterpret_cast<const float*>(slot(stage, i, L::OZ, L::BZ)), dn[i]);
         }
       }
       ru[i] = st[1], ry[i] = st[3];
-      v[2 * i] = v[2 * i + 1] = 0.f;
-      const float g1 = GATE == 1 ? sigmoid(tok[i]) : 1.f;
+      const F2 g1 = both(GATE == 1 ? sigmoid(tok[i]) : 1.f);
+      F2 v0 = zero, v1 = zero;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (POST) un[i][k] = (un[i][k] - st[0]) * ru[i];
-        if constexpr (GATE == 1) s[i][k] = g1;
-        if constexpr (GATE == 2) s[i][k] = sigmoid(s[i][k]);
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (POST) un[i][j] = (un[i][j] + both(-st[0])) * both(ru[i]);
+        if constexpr (GATE == 1) s[i][j] = g1;
+        if constexpr (GATE == 2) s[i][j] = sigmoid(s[i][j]);
         if constexpr (HASZ) {
-          const float p = POST ? fmaf(un[i][k], pw[k], pb[k]) : un[i][k];
-          const float y = fmaf(GATE ? sc[k] * s[i][k] : sc[k], p, yn[i][k]);
-          yn[i][k] = (y - st[2]) * ry[i];
-          aw[k] = fmaf(dn[i][k], yn[i][k], aw[k]);
-          ab[k] += dn[i][k];
-          dn[i][k] *= w[k];
-          v[2 * i] += dn[i][k];
-          v[2 * i + 1] = fmaf(dn[i][k], yn[i][k], v[2 * i + 1]);
+          const F2 p = POST ? fma(un[i][j], pw[j], pb[j]) : un[i][j];
+          const F2 y = fma(GATE ? sc[j] * s[i][j] : sc[j], p, yn[i][j]);
+          yn[i][j] = (y + both(-st[2])) * both(ry[i]);
+          aw[j] = fma(dn[i][j], yn[i][j], aw[j]);
+          ab[j] = ab[j] + dn[i][j];
+          dn[i][j] = dn[i][j] * w[j];
+          v0 = v0 + dn[i][j];
+          v1 = fma(dn[i][j], yn[i][j], v1);
         }
       }
+      v[2 * i] = sum(v0), v[2 * i + 1] = sum(v1);
     }
     if constexpr (HASZ) {
       cta_sums<2 * R, W>(v, red[flip]);
@@ -680,35 +733,35 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
     for (int i = 0; i < R; ++i) {
       const int64_t r = r0 + i;
       if constexpr (HASZ) {
-        const float m1 = a.rms ? 0.f : v[2 * i] * inv, m2 = v[2 * i + 1] * inv;
+        const F2 m1 = both(a.rms ? 0.f : -v[2 * i] * inv), m2 = both(-v[2 * i + 1] * inv), rr = both(ry[i]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dy[i][k] = fmaf(ry[i], dn[i][k] - m1 - yn[i][k] * m2, dy[i][k]);
+        for (int j = 0; j < 2; ++j) dy[i][j] = fma(rr, fma(yn[i][j], m2, dn[i][j] + m1), dy[i][j]);
       }
       const bool in = r < a.rows && mine;
-      if (in) storev<4>(reinterpret_cast<TX*>(a.dx) + r * d + 4 * t, dy[i]);
-      float q0 = 0.f, q1 = 0.f, q2 = 0.f, dg[4];
+      if (in) store2(reinterpret_cast<TX*>(a.dx) + r * d + 4 * t, dy[i]);
+      F2 q0 = zero, q1 = zero, q2 = zero, dg[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float p = POST ? fmaf(un[i][k], pw[k], pb[k]) : un[i][k];
-        const float es = GATE ? dy[i][k] * s[i][k] : dy[i][k], dp = es * sc[k];
-        as[k] = fmaf(es, p, as[k]);
+      for (int j = 0; j < 2; ++j) {
+        const F2 p = POST ? fma(un[i][j], pw[j], pb[j]) : un[i][j];
+        const F2 es = GATE ? dy[i][j] * s[i][j] : dy[i][j], dp = es * sc[j];
+        as[j] = fma(es, p, as[j]);
         if constexpr (GATE != 0) {
-          dg[k] = dp * p * (1.f - s[i][k]);
-          if constexpr (GATE == 1) q2 += dg[k];
+          dg[j] = dp * p * fma(s[i][j], minus, one);
+          if constexpr (GATE == 1) q2 = q2 + dg[j];
         }
         if constexpr (POST) {
-          apw[k] = fmaf(dp, un[i][k], apw[k]);
-          apb[k] += dp;
-          dn[i][k] = dp * pw[k];
-          q0 += dn[i][k];
-          q1 = fmaf(dn[i][k], un[i][k], q1);
+          apw[j] = fma(dp, un[i][j], apw[j]);
+          apb[j] = apb[j] + dp;
+          dn[i][j] = dp * pw[j];
+          q0 = q0 + dn[i][j];
+          q1 = fma(dn[i][j], un[i][j], q1);
         } else {
-          dn[i][k] = dp;
+          dn[i][j] = dp;
         }
       }
       if constexpr (GATE == 2)
-        if (in) storev<4>(reinterpret_cast<TU*>(a.dgate) + r * d + 4 * t, dg);
-      q[3 * i] = q0, q[3 * i + 1] = q1, q[3 * i + 2] = q2;
+        if (in) store2(reinterpret_cast<TU*>(a.dgate) + r * d + 4 * t, dg);
+      q[3 * i] = sum(q0), q[3 * i + 1] = sum(q1), q[3 * i + 2] = sum(q2);
     }
     if constexpr (POST && GATE == 1) {
       cta_sums<3 * R, W>(q, red[flip]);
@@ -734,11 +787,11 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
       const int64_t r = r0 + i;
       if (r >= a.rows) continue;
       if constexpr (POST) {
-        const float m1 = a.rms ? 0.f : q[3 * i] * inv, m2 = q[3 * i + 1] * inv;
+        const F2 m1 = both(a.rms ? 0.f : -q[3 * i] * inv), m2 = both(-q[3 * i + 1] * inv), rr = both(ru[i]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dn[i][k] = ru[i] * (dn[i][k] - m1 - un[i][k] * m2);
+        for (int j = 0; j < 2; ++j) dn[i][j] = rr * fma(un[i][j], m2, dn[i][j] + m1);
       }
-      if (mine) storev<4>(reinterpret_cast<TU*>(a.du) + r * d + 4 * t, dn[i]);
+      if (mine) store2(reinterpret_cast<TU*>(a.du) + r * d + 4 * t, dn[i]);
       if constexpr (GATE == 1)
         if (t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &q[3 * i + 2]);
     }
@@ -747,13 +800,13 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
   if (!mine) return;
   float* part = a.part + (int64_t)blockIdx.x * NPART * d + 4 * t;
   if constexpr (HASZ) {
-    storev<4>(part + PART_W * d, aw);
-    if (a.b) storev<4>(part + PART_B * d, ab);
+    store2(part + PART_W * d, aw);
+    if (a.b) store2(part + PART_B * d, ab);
   }
-  if (a.scale) storev<4>(part + PART_SCALE * d, as);
+  if (a.scale) store2(part + PART_SCALE * d, as);
   if constexpr (POST) {
-    storev<4>(part + PART_PW * d, apw);
-    if (a.pb) storev<4>(part + PART_PB * d, apb);
+    store2(part + PART_PW * d, apw);
+    if (a.pb) store2(part + PART_PB * d, apb);
   }
 }
 

@@ -21,7 +21,6 @@ allocates nothing.
 """
 from __future__ import annotations
 
-import contextlib
 import operator
 import struct
 from typing import Optional, Sequence, Tuple
@@ -43,16 +42,19 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _on(dev: int):
-    """Context in which CUDA device `dev` is the current one (a launch needs its stream's device)."""
-    return _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
-
-
-def _stream_of(dev: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev)
+def _launch(what: str, fn, dev: int, *args):
+    """fn(*args, stream) on the current stream of CUDA device `dev`, which is made the current device
+    where it is not (a launch needs its stream's device); raises on an error code."""
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _need_cuda(*ts):
@@ -1322,47 +1324,43 @@ def linear16(x: torch.Tensor, w: torch.Tensor, sizes: Tuple[int, ...]) -> Tuple[
 _ACT = {"silu": 0, "gelu": 1}
 
 
-def _ffn_rows(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+def _ffn_rows(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int, int]:
     """t (..., width) as 16-byte aligned rows with a stride of a multiple of 8 values (a copy only
-    where it is not laid out so), and the stride."""
+    where it is not laid out so), the stride and the address."""
     v, ld = (t, width) if t.is_contiguous() else _row_view(t, width)
-    if v.data_ptr() % 16 or ld % 8:
+    p = v.data_ptr()
+    if p & 15 or ld & 7:
         v, ld = v.clone(memory_format=torch.contiguous_format), width
-    return v, ld
+        p = v.data_ptr()
+    return v, ld, p
 
 
 def _ffn_args(x, wg, wu, act):
     f, d = wg.shape
-    (x, ldx), (wg, ldg), (wu, ldu) = _ffn_rows(x, d), _ffn_rows(wg, d), _ffn_rows(wu, d)
-    a = _lib.FfnArgs(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ldx, ldg, ldu, x.numel() // d, d, f, act)
+    (x, ldx, px), (wg, ldg, pg), (wu, ldu, pu) = _ffn_rows(x, d), _ffn_rows(wg, d), _ffn_rows(wu, d)
+    a = _lib.FfnArgs(px, pg, pu, ldx, ldg, ldu, x.numel() // d, d, f, act)
     return a, (x, wg, wu)  # the tensors stay alive until the launch is queued
 
 
 def _gated_ffn_run(x, wg, wu, act: int):
-    dev = x.get_device()
     h = x.new_empty((*x.shape[:-1], wg.shape[0]))
     a, hold = _ffn_args(x, wg, wu, act)
-    with _on(dev):
-        rc = _lib.load().sca2_gated_ffn_fwd(a, h.data_ptr(), _stream_of(dev))
-    if rc:
-        _lib.check(rc, "gated_ffn")
+    _launch("gated_ffn", _lib.load().sca2_gated_ffn_fwd, x.get_device(), a, h.data_ptr())
     return h
 
 
 def _gated_ffn_bwd_run(x, wg, wu, act: int, dh, need_x: bool, need_w: bool):
-    dev = x.get_device()
     a, hold = _ffn_args(x, wg, wu, act)
-    dh, _ = _ffn_rows(dh.to(torch.bfloat16).contiguous(), a.f)
+    dh, _, pdh = _ffn_rows(dh if dh.dtype == torch.bfloat16 and dh.is_contiguous() else dh.to(torch.bfloat16).contiguous(), a.f)
     dense = torch.contiguous_format
     dx = torch.empty_like(x, memory_format=dense) if need_x else None
-    dwg, dwu = (torch.empty_like(w, memory_format=dense) if need_w else None for w in (wg, wu))
+    dwg = dwu = None
+    if need_w:
+        dwg, dwu = torch.empty_like(wg, memory_format=dense), torch.empty_like(wu, memory_format=dense)
     lib = _lib.load()
     n = lib.sca2_gated_ffn_work_bytes(a.rows, a.d, a.f)
     work = x.new_empty(n, dtype=torch.uint8)
-    with _on(dev):
-        rc = lib.sca2_gated_ffn_bwd(a, dh.data_ptr(), _ptr(dx), _ptr(dwg), _ptr(dwu), work.data_ptr(), n, _stream_of(dev))
-    if rc:
-        _lib.check(rc, "gated_ffn_bwd")
+    _launch("gated_ffn_bwd", lib.sca2_gated_ffn_bwd, x.get_device(), a, pdh, _ptr(dx), _ptr(dwg), _ptr(dwu), work.data_ptr(), n)
     return dx, dwg, dwu
 
 
@@ -1437,11 +1435,12 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
         raise E(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
     if not x.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16:
         raise E("gated_ffn: x and the weights must be bfloat16")
-    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[-1]:
-        raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(w_gate.shape)} and "
+    shape = w_gate.shape
+    if x.dim() < 1 or len(shape) != 2 or shape != w_up.shape or shape[1] != x.shape[-1]:
+        raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(shape)} and "
                 f"{tuple(w_up.shape)}")
-    if not gated_ffn_supported(x.shape[-1], w_gate.shape[0]):
-        raise E(f"gated_ffn: d and f must be multiples of 8, got {x.shape[-1]} and {w_gate.shape[0]}")
+    if not gated_ffn_supported(shape[1], shape[0]):
+        raise E(f"gated_ffn: d and f must be multiples of 8, got {shape[1]} and {shape[0]}")
     if torch.compiler.is_compiling():
         return torch.ops.sca2b200.gated_ffn_fwd(x, w_gate, w_up, _ACT[act])
     if _wants_grad(x, w_gate, w_up):
@@ -1484,35 +1483,30 @@ def _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
 
 
 def _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, save: bool):
-    dev, dense = x.get_device(), torch.contiguous_format
+    dense = torch.contiguous_format
     y = torch.empty_like(x, memory_format=dense)
     z = torch.empty_like(x, dtype=zdt, memory_format=dense) if w is not None else x.new_empty(0, dtype=zdt)
     stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if save else None
     a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
-    with _on(dev):
-        rc = _lib.load().sca2_residual_norm_fwd(a, y.data_ptr(), z.data_ptr() if w is not None else None, _ptr(stats),
-                                                _stream_of(dev))
-    if rc:
-        _lib.check(rc, "residual_norm")
+    _launch("residual_norm", _lib.load().sca2_residual_norm_fwd, x.get_device(), a, y.data_ptr(),
+            z.data_ptr() if w is not None else None, _ptr(stats))
     return y, z, stats
 
 
 def _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, stats, dy, dz):
-    dev, dense = x.get_device(), torch.contiguous_format
+    dense = torch.contiguous_format
     dy = None if dy is None else dy.to(x.dtype).contiguous()
     dz = None if dz is None else dz.to(zdt).contiguous()
     dx, du = torch.empty_like(x, memory_format=dense), torch.empty_like(u, memory_format=dense)
     dgate = torch.empty_like(gate, memory_format=dense) if gate is not None else None
-    dw, db, dscale, dpw, dpb = (None if t is None else torch.empty_like(t) for t in (w, b, scale, pw, pb))
+    dw, db, dscale, dpw, dpb = [None if t is None else torch.empty_like(t) for t in (w, b, scale, pw, pb)]
     a, hold = _rnorm_args(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt)
     lib = _lib.load()
     n = lib.sca2_residual_norm_work_bytes(a.rows, a.d)
     work = x.new_empty(n, dtype=torch.uint8)
     g = _lib.RNormGrads(dx.data_ptr(), du.data_ptr(), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(dscale), _ptr(dpw), _ptr(dpb))
-    with _on(dev):
-        rc = lib.sca2_residual_norm_bwd(a, stats.data_ptr(), _ptr(dy), _ptr(dz), g, work.data_ptr(), n, _stream_of(dev))
-    if rc:
-        _lib.check(rc, "residual_norm_bwd")
+    _launch("residual_norm_bwd", lib.sca2_residual_norm_bwd, x.get_device(), a, stats.data_ptr(), _ptr(dy), _ptr(dz), g,
+            work.data_ptr(), n)
     return dx, du, dw, db, dgate, dscale, dpw, dpb
 
 
@@ -1651,12 +1645,14 @@ def _grad_list(what: str, grads, out=None):
         raise E(f"{what}: {len(grads)} gradients and {len(outs)} destinations")
     dev, types = None, []
     for ts in (grads,) if out is None else (grads, outs):
-        if not all([isinstance(t, _T) for t in ts]):
-            raise E(f"{what}: gradients must be tensors")
-        types.append(list(map(_dtype, ts)))
-        if not set(types[-1]) <= _DT.keys() or any([t.is_sparse for t in ts]):
+        try:
+            types.append(list(map(_dtype, ts)))
+            devs = set(map(_T.get_device, ts))
+            ok = set(types[-1]) <= _DT.keys() and {t.layout for t in ts} <= {torch.strided}
+        except (AttributeError, TypeError):  # not tensors
+            ok = False
+        if not ok:
             raise E(f"{what}: gradients must be dense float32 or bfloat16 tensors")
-        devs = set(map(_T.get_device, ts))
         if ts and (len(devs) != 1 or min(devs) < 0 or dev not in (None, *devs)):
             devs = {_need_cuda(*grads, *outs).index}
         dev = devs.pop() if devs else None
@@ -1691,14 +1687,10 @@ def _clip_run(grads, outs, types, max_norm: Optional[float], dev: int) -> torch.
     norm = src[0].new_empty((), dtype=torch.float32)
     nb = lib.sca2_clip_grads_work_bytes(n)
     work = src[0].new_empty(nb, dtype=torch.uint8)
-    with _on(dev):
-        if max_norm is None:
-            rc = lib.sca2_grad_norm(table, n, norm.data_ptr(), work.data_ptr(), nb, _stream_of(dev))
-        else:
-            rc = lib.sca2_clip_grads(table, n, max_norm, norm.data_ptr(), work.data_ptr(), nb, _stream_of(dev))
-    if rc:
-        _lib.check(rc, "grad_norm" if max_norm is None else "clip_grads")
-    if max_norm is not None:
+    if max_norm is None:
+        _launch("grad_norm", lib.sca2_grad_norm, dev, table, n, norm.data_ptr(), work.data_ptr(), nb)
+    else:
+        _launch("clip_grads", lib.sca2_clip_grads, dev, table, n, max_norm, norm.data_ptr(), work.data_ptr(), nb)
         for g, s in back:
             g.copy_(s)
     return norm
