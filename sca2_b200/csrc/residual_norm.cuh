@@ -291,11 +291,14 @@ __device__ __forceinline__ void copies_wait() {
 // Forward for rows of up to 1024 aligned values: a warp owns a row, each lane NG groups of four
 // values, so that every copy, load and store of the warp is one run of whole sectors in either type.
 // The slots hold one row: the next row's u is asked for once this row's is in registers, its x and
-// gate once the join has read this row's, and both travel under the rest of the row's work.
+// gate once the join has read this row's, and both travel under the rest of the row's work.  The
+// parameters lie in shared memory too: read from L1 their latency was the kernel's bound (65536 x
+// 768, everything on: 141 us, 116 us so; 705 MB are 109 us at the copy rate).
 template <int NG, int GATE, class TX, class TU>
 struct FwdRing {  // bytes of a thread's group in each array; the arrays' slots lie thread by thread
   static constexpr int BU = 4 * sizeof(TU), BX = 4 * sizeof(TX), BG = GATE == 2 ? BU : 0;
-  static constexpr int OX = NG * BU * FT, OG = OX + NG * BX * FT, BYTES = OG + NG * BG * FT;
+  static constexpr int OX = NG * BU * FT, OG = OX + NG * BX * FT, OP = OG + NG * BG * FT;
+  static constexpr int D = NG * 128, BYTES = OP + 5 * D * 4;  // w, b, pw, pb, scale
 };
 
 template <int NG, int GATE, bool POST, class TX, class TU>
@@ -358,6 +361,14 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
   };
 
   fetch_u(row), fetch_x(row);
+  float* par = reinterpret_cast<float*>(slots + L::OP);
+  const auto stage = [&](int i, const float* p) -> const float* {
+    if (!p) return nullptr;
+    for (int c = threadIdx.x; c < d; c += FT) par[i * L::D + c] = p[c];
+    return par + i * L::D;
+  };
+  const float *w = stage(0, a.w), *b = stage(1, a.b), *pw = stage(2, a.pw), *pb = stage(3, a.pb), *scale = stage(4, a.scale);
+  __syncthreads();
   for (; row < a.rows; row += step) {
     float gt = 1.f;
     if constexpr (GATE == 1) {
@@ -376,7 +387,7 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
       normalise(mu, rs);
 #pragma unroll
       for (int k = 0; k < NG; ++k)
-        if (col(k) < d) affine(k, rs, a.pw, a.pb);
+        if (col(k) < d) affine(k, rs, pw, pb);
     }
     if (a.stats && lane == 0) a.stats[4 * row] = mu, a.stats[4 * row + 1] = rs;
     copies_wait<1>();
@@ -384,8 +395,8 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
         F2 q[2];
-        if (a.scale) {
-          load2(a.scale + col(k), q);
+        if (scale) {
+          load2(scale + col(k), q);
           y[k][0] = y[k][0] * q[0], y[k][1] = y[k][1] * q[1];
         }
         if constexpr (GATE == 2) {
@@ -404,7 +415,7 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
 #pragma unroll
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
-        affine(k, rs, a.w, a.b);
+        affine(k, rs, w, b);
         if (a.zdt == SCA2_BF16) store2(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), y[k]);
         else store2(reinterpret_cast<float*>(a.z) + row * d + col(k), y[k]);
       }
@@ -844,14 +855,17 @@ cudaError_t fwd_ring_gate(const Args& a, cudaStream_t st) {
   return a.gate_mode == 0 ? fwd_ring_width<0, POST, TX, TU>(a, st)
          : a.gate_mode == 1 ? fwd_ring_width<1, POST, TX, TU>(a, st) : fwd_ring_width<2, POST, TX, TU>(a, st);
 }
-// vec: rows and pointers allow groups of four values
+// Up to FEW_ROWS rows a CTA owns a row (fwd_kernel): all rows at once, each by more threads.  vec:
+// rows and pointers allow groups of four values.
+constexpr int FEW_ROWS = 148 * 4;
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   const int d = a.d;
-  if (vec && d <= 1024) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
+  if (vec && d <= 1024 && a.rows > FEW_ROWS) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
   const int grid = (int)(a.rows < 148 * 8 ? a.rows : 148 * 8);
   if (vec) {
-    if (d <= 2048) fwd_kernel<2, 4, TX, TU><<<grid, FT, 0, st>>>(a);
+    if (d <= 1024) fwd_kernel<1, 4, TX, TU><<<grid, FT, 0, st>>>(a);
+    else if (d <= 2048) fwd_kernel<2, 4, TX, TU><<<grid, FT, 0, st>>>(a);
     else fwd_kernel<4, 4, TX, TU><<<grid, FT, 0, st>>>(a);
   } else {
     if (d <= 1024) fwd_kernel<4, 1, TX, TU><<<grid, FT, 0, st>>>(a);
