@@ -527,7 +527,13 @@ __global__ void __launch_bounds__(256) dw_reduce(const float4* __restrict__ part
 // 16 x 16 fragments come straight from memory: a lane reads 16 bytes (8 steps) of its two rows, and
 // takes them as the fragments of two products; the steps' order inside a group of 32 does not
 // matter as long as x, read the same way, agrees.  NG groups of 8 rows of x.
+//
+// Two CTAs to an SM hide each other's loads (768 -> 2048, one row 3.6 -> 2.6 us; 1024 -> 2736, 4.6 us:
+// 11.2 MB of weights, 1.7 us at the copy rate).  With more than 32 rows the accumulators take 64
+// registers: where the grid leaves no SM a second CTA, one with twice the loads in flight is faster
+// (64 rows, 768 -> 2048: 6.0 against 7.4 us), otherwise two with fewer (1024 -> 2736: 11.3 against 13.0).
 constexpr int FT = 256;
+constexpr int RED_ROW = 20;  // floats of a row of 16 sums: a fragment's 32 lanes on 32 banks
 
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -537,12 +543,13 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NG, int ACT>
-__global__ void __launch_bounds__(FT) ffn_few(const __nv_bfloat16* __restrict__ x, int64_t ldx,
+template <int NG, int ACT, int MINB>
+__global__ void __launch_bounds__(FT, MINB) ffn_few(const __nv_bfloat16* __restrict__ x, int64_t ldx,
                                               const __nv_bfloat16* __restrict__ wg, int64_t ldg,
                                               const __nv_bfloat16* __restrict__ wu, int64_t ldu,
                                               __nv_bfloat16* __restrict__ h, int rows, int d, int f) {
-  extern __shared__ float red[];  // (8 warps, 2, 8 NG, 16)
+  extern __shared__ float red[];  // (8 warps, gate | up, 8 NG rows, RED_ROW)
+  constexpr int PART = 8 * NG * RED_ROW;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
   const int f0 = blockIdx.x * 16;
   const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -557,7 +564,7 @@ __global__ void __launch_bounds__(FT) ffn_few(const __nv_bfloat16* __restrict__ 
   const auto ld = [&](const __nv_bfloat16* p, bool ok) {
     return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : zero;
   };
-  constexpr int UN = 4;  // groups of 32 steps whose weights are in flight at once
+  constexpr int UN = NG == 8 && MINB == 2 ? 2 : 4;  // groups of 32 steps whose weights are in flight at once
   for (int kb = 32 * warp; kb < d; kb += 32 * 8 * UN) {
     uint4 a[UN][4];
 #pragma unroll
@@ -582,14 +589,14 @@ __global__ void __launch_bounds__(FT) ffn_few(const __nv_bfloat16* __restrict__ 
     }
   }
   // fragment (row gr or gr + 8 of the weights, rows 2 tq and 2 tq + 1 of x) -> red[warp][gate|up][row][column]
-  float* mine = red + warp * (2 * 8 * NG * 16);
+  float* mine = red + warp * 2 * PART;
 #pragma unroll
   for (int j = 0; j < NG; ++j)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int at = (8 * j + 2 * tq + (k & 1)) * 16 + gr + 8 * (k >> 1);
+      const int at = (8 * j + 2 * tq + (k & 1)) * RED_ROW + gr + 8 * (k >> 1);
       mine[at] = cg[j][k];
-      mine[8 * NG * 16 + at] = cu[j][k];
+      mine[PART + at] = cu[j][k];
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 8 * NG * 16; i += FT) {
@@ -598,8 +605,8 @@ __global__ void __launch_bounds__(FT) ffn_few(const __nv_bfloat16* __restrict__ 
     float sg = 0.f, su = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      sg += red[w * (2 * 8 * NG * 16) + i];
-      su += red[w * (2 * 8 * NG * 16) + 8 * NG * 16 + i];
+      sg += red[w * 2 * PART + r * RED_ROW + c];
+      su += red[w * 2 * PART + PART + r * RED_ROW + c];
     }
     h[(int64_t)r * f + f0 + c] = __float2bfloat16_rn(act_of<ACT>(sg) * su);
   }
@@ -666,11 +673,11 @@ cudaError_t launch_act(int act, const Maps& maps, const Geo& g, cudaStream_t st)
   return act == SCA2_ACT_SILU ? launch<MODE, SILU>(maps, g, st) : launch<MODE, GELU>(maps, g, st);
 }
 
-template <int NG>
+template <int NG, int MINB = 2>
 cudaError_t launch_few(const sca2_ffn_args& a, void* h, cudaStream_t st) {
   const auto bf = [](const void* p) { return static_cast<const __nv_bfloat16*>(p); };
-  const int smem = 8 * 2 * 8 * NG * 16 * 4, grid = (a.f + 15) / 16;
-  const auto k = a.act == SCA2_ACT_SILU ? ffn_few<NG, SILU> : ffn_few<NG, GELU>;
+  const int smem = 8 * 2 * 8 * NG * RED_ROW * 4, grid = (a.f + 15) / 16;
+  const auto k = a.act == SCA2_ACT_SILU ? ffn_few<NG, SILU, MINB> : ffn_few<NG, GELU, MINB>;
   if (smem > 48 * 1024)
     if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
   k<<<grid, FT, smem, st>>>(bf(a.x), a.ldx, bf(a.w_gate), a.ldg, bf(a.w_up), a.ldu, static_cast<__nv_bfloat16*>(h),
@@ -754,7 +761,8 @@ int sca2_gated_ffn_fwd(const sca2_ffn_args* a, void* h, void* stream) {
   cudaError_t e;
   if (a->rows <= FEW_ROWS) {
     e = a->rows <= 8 ? launch_few<1>(*a, h, st) : a->rows <= 16 ? launch_few<2>(*a, h, st)
-        : a->rows <= 32 ? launch_few<4>(*a, h, st) : launch_few<8>(*a, h, st);
+        : a->rows <= 32 ? launch_few<4>(*a, h, st)
+        : a->f <= 16 * 148 ? launch_few<8, 1>(*a, h, st) : launch_few<8, 2>(*a, h, st);
   } else {
     if ((e = allow_act<FWD>(a->act)) != cudaSuccess) return cuda_fail(e, "sca2_gated_ffn_fwd");
     if (!sca2::tensor_map_encoder()) return fail(SCA2_ERR_CUDA, "gated_ffn: no tensor-map encoder in the driver");
