@@ -1676,13 +1676,25 @@ def _grad_table(src, dst, types):
     return struct.pack("=" + "QQqii" * n, *flat)
 
 
+def _apart(grads):
+    """Refuse tensors whose ranges of memory overlap (the library sees only the copies of those that
+    are not contiguous)."""
+    end = 0
+    for a, b in sorted((g.data_ptr(), g.element_size() * (1 + sum((n - 1) * abs(k) for n, k in zip(g.shape, g.stride()))))
+                       for g in grads if g.numel()):
+        if a < end:
+            raise _lib.Sca2Error("clip_grads: tensors that are not contiguous overlap another tensor of the list")
+        end = a + b
+
+
 def _clip_run(grads, outs, types, max_norm: Optional[float], dev: int) -> torch.Tensor:
     # a gradient that is not contiguous goes through a contiguous copy
     src, back = grads, ()
     if not all(map(_T.is_contiguous, grads)):
         src = [g.contiguous() for g in grads]
-        if outs is grads:
+        if outs is grads and max_norm is not None:
             back = [(g, s) for g, s in zip(grads, src) if g is not s]
+            _apart(grads)
     table, n, lib = _grad_table(src, src if outs is grads else outs, types), len(src), _lib.load()
     norm = src[0].new_empty((), dtype=torch.float32)
     nb = lib.sca2_clip_grads_work_bytes(n)
@@ -1724,12 +1736,12 @@ def grad_norm(grads) -> torch.Tensor:
     """2-norm of all values of the tensors together (fp32 scalar on their device; summed in 64 bits
     in a fixed order).  grads: a tensor or a list of float32 / bfloat16 tensors on one device; no
     tensor gives 0 (on the current CUDA device).  Not differentiable."""
+    if torch.compiler.is_compiling():
+        return torch.ops.sca2b200.grad_norm([grads] if isinstance(grads, _T) else list(grads))
     grads, outs, types, dev = _grad_list("grad_norm", grads)
     if not grads:
         return torch.zeros((), device="cuda")
     with torch.no_grad():
-        if torch.compiler.is_compiling():
-            return torch.ops.sca2b200.grad_norm(grads)
         return _clip_run(grads, outs, types, None, dev)
 
 
@@ -1737,19 +1749,21 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     """Scale the gradients so that their global 2-norm is at most max_norm, and return the norm
     before (fp32 scalar; nothing waits for the device): g * min(1, max_norm / (norm + 1e-6)), as
     torch.nn.utils.clip_grad_norm_.  In place, or into the contiguous tensors `out` (float32 or
-    bfloat16, one for each gradient, with as many values).  A tensor that is written may not share memory with another
-    of the call (refused).  Not differentiable."""
+    bfloat16, one for each gradient, with as many values).  A tensor that is written may not share
+    memory with another of the call (refused; of one that is not contiguous, its whole range counts).
+    Not differentiable."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise _lib.Sca2Error("clip_grads: max_norm must be >= 0")
+    if torch.compiler.is_compiling() and out is None:
+        return torch.ops.sca2b200.clip_grads_([grads] if isinstance(grads, _T) else list(grads), max_norm)
     grads, outs, types, dev = _grad_list("clip_grads", grads, out)
     if not grads:
         return torch.zeros((), device="cuda")
     with torch.no_grad():
-        if torch.compiler.is_compiling() and out is None:
-            return torch.ops.sca2b200.clip_grads_(grads, max_norm)
         norm = _clip_run(grads, outs, types, max_norm, dev)
-    torch.autograd.graph.increment_version(outs)
+    if not torch.is_inference_mode_enabled():  # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
     return norm
 
 

@@ -140,6 +140,33 @@ def test_shared_memory_is_refused():
     _check([keep], [t], torch.tensor(_norm64([keep])), 0.5)
 
 
+def test_not_contiguous_tensors_apart():
+    from sca2_b200 import _lib, ops
+    t = _tensors([(64, 64)])[0]
+    keep = t.clone()
+    for ts in ([t[:, ::2], t[:, ::2]], [t[:, :40], t[:, 30:]], [t[::2], t], [t.t(), t]):
+        with pytest.raises(_lib.Sca2Error, match="overlap"):
+            ops.clip_grads(ts, 0.5)
+    assert torch.equal(t, keep)
+    parts = [t[:20, ::2], t[20:40].t(), t[40:]]
+    ref = [p.clone() for p in parts]
+    _check(ref, parts, ops.clip_grads(parts, 0.5), 0.5)
+    with torch.inference_mode():
+        i = keep.clone()
+        _check([keep], [i], ops.clip_grads([i], 0.5), 0.5)
+
+
+def test_compiled():
+    from sca2_b200 import ops
+    a, b = _tensors([(40,), (3, 5)])
+    x, y = a.clone(), b.clone()
+    n = ops.clip_grads([a, b], 0.1)
+    f = torch.compile(lambda u, v: ops.clip_grads([u, v], 0.1), fullgraph=True, backend="aot_eager")
+    assert torch.equal(f(x, y), n) and torch.equal(x, a) and torch.equal(y, b)
+    g = torch.compile(lambda u, v: ops.grad_norm([u, v]), fullgraph=True, backend="aot_eager")
+    assert torch.equal(g(a, b), ops.grad_norm([a, b]))
+
+
 def test_versions():
     """An in-place clip counts as one for autograd's check of saved tensors."""
     from sca2_b200 import ops
