@@ -4,11 +4,11 @@
 //     dg = dh u act'(g),  du = dh act(g)
 //     dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
 //
-// Four products share one kernel, `ffn_gemm<MODE>`: a pair of CTAs (cta_group::2) computes a
+// Four kinds of product share one kernel, `ffn_gemm<KIND>`: a pair of CTAs (cta_group::2) computes a
 // 256 x 256 tile with tcgen05.mma, the operands staged by TMA in 128-byte swizzled tiles of 64
 // contraction steps, one mbarrier ring, the accumulator double-buffered in TMEM (2 x 256 columns)
 // so that the epilogue of a tile runs under the products of the next; tiles are dealt to the pairs
-// in a fixed order.
+// in a fixed order.  The launches: FWD; BACK; GRADS, which holds DW and DX.
 //   FWD   tile = 256 rows x (128 gate columns | the same 128 up columns): CTA 0 of the pair stages
 //         Wg's rows and CTA 1 Wu's, so one accumulator row holds g and u of a column and the
 //         epilogue forms h without a trip to memory.
@@ -19,7 +19,16 @@
 //         as they lie (MN-major operand), no transposed copy.
 //   DW    contraction over the rows, both operands MN-major; split over the rows where the tiles
 //         alone do not fill the machine, the fp32 parts added in a fixed order by `dw_reduce`.
+//   GRADS gives each pair its DW tiles (few and long) and then as many of the DX tiles (many and
+//         short) as even out the pairs' contraction blocks, so neither has a last round of its own:
+//         65536 x 768 -> 2048 555 us for both, 580 as two launches and a pass over split parts.
 // Ragged sizes: TMA fills what lies outside with zeros and clips what is stored there.
+//
+// Measured (one B200, device time in short bursts): 32768 x 1024 -> 4096 forward 360 us (1530 TFLOP/s,
+// 91% of the measured cuBLAS burst); 65536 x 768 -> 2048 forward 290 us, BACK 340, GRADS 555.  Bound by
+// the tensor cores under the power limit: a contraction block of a tile takes 0.37 us at any width,
+// which is cuBLAS's rate; at d = 768 the epilogue and the switch of tiles add 15%, in BACK 30% (half of
+// that its stores).  L2 prefetches of the operands by TMA slowed every product (360 -> 400 us).
 //
 // Up to FFN_FEW_ROWS rows (decode) the forward is bound by reading the weights and by latency:
 // `ffn_few` keeps no tiles, each warp streams weight rows straight into mma.sync fragments.
@@ -28,6 +37,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstring>
 #include <string>
 
@@ -44,7 +54,7 @@ using umma::smem_u32;
 
 __device__ unsigned int g_fault_ffn;
 
-enum Mode { FWD, BACK, DX, DW };
+enum Mode { FWD, BACK, DX, DW, GRADS };
 enum Act { SILU, GELU };
 
 constexpr int BK = 64;               // contraction steps of a stage: 128 bytes, one swizzle row
@@ -54,10 +64,10 @@ constexpr int NT = 128 + 32 * EPI_WARPS;
 constexpr int STG = 2048;            // one staged output block: 32 rows of 64 bytes
 constexpr uint64_t WAIT_NS = 4000000000ull;  // a wait gives up after this
 
-template <int MODE>
+template <int KIND>
 struct Layout {
-  static constexpr int STAGES = MODE == FWD ? 6 : 5;
-  static constexpr int NSTG = MODE == FWD ? 1 : 2;  // staged output blocks of a warp
+  static constexpr int STAGES = KIND == FWD ? 6 : 5;
+  static constexpr int NSTG = KIND == FWD ? 1 : 2;  // staged output blocks of a warp
   static constexpr int RING = STAGES * 2 * HALF;
   static constexpr int BARS = RING + EPI_WARPS * NSTG * STG;
   static constexpr int TOTAL = BARS + 320 + 1024;  // 1024: room to align the ring
@@ -66,14 +76,16 @@ struct Layout {
 struct Geo {
   int rows, d, f;
   int tiles_n, tiles_m, slices, splits;  // unit = ((split * slices + slice) * tiles_m + m) * tiles_n + n
-  int units;
+  int units;                             // of FWD or BACK, or those of DW
   int kb, kb_half;                       // contraction blocks of a whole tile; DX: those of one half
   int kb_split, kb_more;                 // those of a split, and how many splits have one more
   int sn, sm, ss, sp;                    // the grid's pairs as digits of a unit
+  int x_units, x_pairs, x_a, x_b;        // DX: units; a pair below x_pairs takes up to x_a of them, another x_b
 };
 
 struct Maps {
-  CUtensorMap a0, a1, b0, b1, o0, o1, dh;
+  CUtensorMap a0, a1, b0, b1, o0, o1, dh;  // GRADS: a0, a1, b0, o0, o1 of DW
+  CUtensorMap xa0, xa1, xb0, xb1, xo;      // and those of DX
 };
 
 // ---- cluster, barrier and TMA primitives ---------------------------------------------------
@@ -270,14 +282,49 @@ struct Unit {
     slice -= f ? g.slices : 0;
     split += g.sp + f;
   }
+  // DX: a unit, and the one `step` (as digits) on
+  __device__ __forceinline__ void first_x(const Geo& g, int u) { n = u % g.tiles_n, m = u / g.tiles_n, slice = split = 0; }
+  __device__ __forceinline__ void next_x(const Geo& g, int step_n, int step_m) {
+    n += step_n;
+    const int c = n >= g.tiles_n;
+    n -= c ? g.tiles_n : 0, m += step_m + c;
+  }
   // its contraction blocks: the first `kb_more` splits have one more
   __device__ __forceinline__ int k0(const Geo& g) const { return split * g.kb_split + (split < g.kb_more ? split : g.kb_more); }
   __device__ __forceinline__ int k1(const Geo& g) const { return k0(g) + g.kb_split + (split < g.kb_more ? 1 : 0); }
 };
 
-template <int MODE, int ACT>
+template <int M>
+struct ModeOf {
+  static constexpr int value = M;
+};
+
+// f(mode, unit) for the pair's units in order; false from f ends it
+template <int KIND, class F>
+__device__ __forceinline__ void for_units(const Geo& g, int pair, int pairs, F f) {
+  Unit t;
+  if (pair < g.units) {
+    t.first(g, pair);
+    for (int u = pair; u < g.units; u += pairs, t.next(g))
+      if (!f(ModeOf<KIND == GRADS ? DW : KIND>{}, t)) return;
+  }
+  if constexpr (KIND == GRADS) {
+    // pairs with equally many DW units come here together and take the DX units of their share in
+    // turn: neighbours have the same rows, which reach L2 once
+    const bool a = pair < g.x_pairs;
+    const int step = a ? g.x_pairs : pairs - g.x_pairs, count = a ? g.x_a : g.x_b;
+    int u = a ? pair : g.x_a * g.x_pairs + (pair - g.x_pairs);
+    if (count == 0 || u >= g.x_units) return;
+    t.first_x(g, u);
+    const int step_n = step % g.tiles_n, step_m = step / g.tiles_n;
+    for (int i = 0; i < count && u < g.x_units; ++i, u += step, t.next_x(g, step_n, step_m))
+      if (!f(ModeOf<DX>{}, t)) return;
+  }
+}
+
+template <int KIND, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(const __grid_constant__ Maps maps, const Geo g) {
-  using L = Layout<MODE>;
+  using L = Layout<KIND>;
   constexpr int ST = L::STAGES;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;  // the same offset in both CTAs
@@ -313,12 +360,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
       const uint32_t full0 = map_to(full, 0);
       int s = 0, ph = 1, issued = 0;
       bool ok = true;
-      Unit t;
-      t.first(g, pair);
-      for (int u = pair; u < g.units && ok; u += pairs, t.next(g)) {
-        const int k1 = t.k1(g);
-        for (int k = t.k0(g); k < k1; ++k) {
-          if (!(ok = wait_for(empty + 8 * s, ph))) break;
+      for_units<KIND>(g, pair, pairs, [&](auto mode, const Unit& t) {
+        constexpr int MODE = decltype(mode)::value;
+        const int k0 = MODE == DW ? t.k0(g) : 0, k1 = MODE == DX ? 2 * g.kb_half : MODE == DW ? t.k1(g) : g.kb;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = wait_for(empty + 8 * s, ph))) return false;
           if (rank == 0) expect(full + 8 * s, 4 * HALF);
           const uint32_t A = base + s * 2 * HALF, B = A + HALF, bar = full0 + 8 * s;
           if constexpr (MODE == FWD || MODE == BACK) {
@@ -327,8 +373,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           } else if constexpr (MODE == DX) {
             const bool up = k >= g.kb_half;
             const int kk = (up ? k - g.kb_half : k) * BK, n = t.n * 256 + 128 * rank;
-            const CUtensorMap* w = up ? &maps.b1 : &maps.b0;
-            load2(A, up ? &maps.a1 : &maps.a0, kk, t.m * 256 + 128 * rank, bar);
+            const CUtensorMap* w = up ? &maps.xb1 : &maps.xb0;
+            load2(A, up ? &maps.xa1 : &maps.xa0, kk, t.m * 256 + 128 * rank, bar);
             load2(B, w, n, kk, bar);
             load2(B + HALF / 2, w, n + 64, kk, bar);
           } else {
@@ -342,7 +388,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           if (++s == ST) s = 0, ph ^= 1;
           issued = issued < ST ? issued + 1 : ST;
         }
-      }
+        return true;
+      });
       if (!ok && rank == 0)  // leave no copy in flight: both CTAs' copies complete on these
         for (; issued > 0; --issued) {
           if (--s < 0) s = ST - 1, ph ^= 1;
@@ -351,19 +398,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // ---- products of both CTAs
-      constexpr bool a_mn = MODE == DW, b_mn = MODE == DX || MODE == DW;
-      const uint32_t id = umma::idesc_bf16_t(256, 256, a_mn, b_mn);
       int n = 0, s = 0, ph = 0;
-      bool ok = true;
-      Unit t;
-      t.first(g, pair);
-      for (int u = pair; u < g.units && ok; u += pairs, ++n) {
-        const int acc = n & 1, kn = t.k1(g) - t.k0(g);
-        t.next(g);
-        if (!(ok = wait_for(tempty + 8 * acc, ((n >> 1) & 1) ^ 1))) break;
+      for_units<KIND>(g, pair, pairs, [&](auto mode, const Unit& t) {
+        constexpr int MODE = decltype(mode)::value;
+        constexpr bool a_mn = MODE == DW, b_mn = MODE == DX || MODE == DW;
+        constexpr uint32_t id = umma::idesc_bf16_t(256, 256, a_mn, b_mn);
+        const int acc = n & 1, kn = MODE == DX ? 2 * g.kb_half : MODE == DW ? t.k1(g) - t.k0(g) : g.kb;
+        if (!wait_for(tempty + 8 * acc, ((n >> 1) & 1) ^ 1)) return false;
         umma::fence_after_sync();
         for (int k = 0; k < kn; ++k) {
-          if (!(ok = wait_for(full + 8 * s, ph))) break;
+          if (!wait_for(full + 8 * s, ph)) return false;
           umma::fence_after_sync();
           const uint32_t A = base + s * 2 * HALF, B = A + HALF;
           const uint64_t da = a_mn ? desc_mn(A) : desc_k(A), db = b_mn ? desc_mn(B) : desc_k(B);
@@ -373,16 +417,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           commit2(empty + 8 * s);
           if (++s == ST) s = 0, ph ^= 1;
         }
-        if (ok) commit2(tfull + 8 * acc);
-      }
+        commit2(tfull + 8 * acc);
+        ++n;
+        return true;
+      });
     }
   } else if (warp >= 4) {  // ---- epilogue: 32 rows (the warp's quarter of TMEM) x a quarter of the columns
     const int e = warp - 4, q = warp & 3, part = e >> 2;
     const uint32_t stg = stg0 + e * L::NSTG * STG, dhb = dhbar + 8 * e, tempty0 = map_to(tempty, 0);
     int n = 0;
-    Unit t;
-    t.first(g, pair);
-    for (int u = pair; u < g.units; u += pairs, ++n, t.next(g)) {
+    for_units<KIND>(g, pair, pairs, [&](auto mode, const Unit& t) {
+      constexpr int MODE = decltype(mode)::value;
       const int acc = n & 1;
       const int row = t.m * 256 + 128 * rank + 32 * q;
       const uint32_t tm = umma::taddr(tmem, 32 * q, 256 * acc);
@@ -394,7 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           load1(stg, &maps.dh, hc, row, dhb);
         }
       }
-      if (!__all_sync(0xffffffffu, wait_for(tfull + 8 * acc, (n >> 1) & 1))) break;
+      if (!__all_sync(0xffffffffu, wait_for(tfull + 8 * acc, (n >> 1) & 1))) return false;
       umma::fence_after_sync();
       if constexpr (MODE == FWD || MODE == BACK) {
         uint32_t rg[32], ru[32];
@@ -409,7 +454,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
         __syncwarp();
         if (lane == 0) arrive_cluster(tempty0 + 8 * acc);
         if constexpr (MODE == BACK) {
-          if (!__all_sync(0xffffffffu, wait_for(dhb, n & 1))) break;
+          if (!__all_sync(0xffffffffu, wait_for(dhb, n & 1))) return false;
         } else {
           if (lane == 0) stores_read<0>();
           __syncwarp();
@@ -494,13 +539,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
             umma::fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (row < limit && col < g.d) store2d(MODE == DW && t.slice ? &maps.o1 : &maps.o0, stg + c * STG, col, row);
+              if (row < limit && col < g.d)
+                store2d(MODE == DX ? &maps.xo : t.slice ? &maps.o1 : &maps.o0, stg + c * STG, col, row);
               stores_commit();
             }
           }
         }
       }
-    }
+      ++n;
+      return true;
+    });
     if (lane == 0) stores_done();
   }
   __syncthreads();
@@ -648,29 +696,30 @@ constexpr int PAIRS = 74;  // 148 SMs
 // The kernels' shared memory.  Before any tensor map is encoded: as a call of the runtime it also
 // makes the device's context current in this thread (autograd's threads come without one, and the
 // driver then refuses to encode).
-template <int MODE, int ACT>
+template <int KIND, int ACT>
 cudaError_t allow() {
-  return cudaFuncSetAttribute(ffn_gemm<MODE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<MODE>::TOTAL);
+  return cudaFuncSetAttribute(ffn_gemm<KIND, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<KIND>::TOTAL);
 }
-template <int MODE>
+template <int KIND>
 cudaError_t allow_act(int act) {
-  return act == SCA2_ACT_SILU ? allow<MODE, SILU>() : allow<MODE, GELU>();
+  return act == SCA2_ACT_SILU ? allow<KIND, SILU>() : allow<KIND, GELU>();
 }
-template <int MODE, int ACT>
+int pairs_of(const Geo& g) { return std::min(PAIRS, g.units + g.x_units); }
+template <int KIND, int ACT>
 cudaError_t launch(const Maps& maps, const Geo& g, cudaStream_t st) {
-  const int pairs = g.units < PAIRS ? g.units : PAIRS;
+  const int pairs = pairs_of(g);
   Geo k = g;
   k.kb_split = g.kb / g.splits, k.kb_more = g.kb % g.splits;
   int u = pairs;
   k.sn = u % g.tiles_n, u /= g.tiles_n;
   k.sm = u % g.tiles_m, u /= g.tiles_m;
   k.ss = u % g.slices, k.sp = u / g.slices;
-  ffn_gemm<MODE, ACT><<<2 * pairs, NT, Layout<MODE>::TOTAL, st>>>(maps, k);
+  ffn_gemm<KIND, ACT><<<2 * pairs, NT, Layout<KIND>::TOTAL, st>>>(maps, k);
   return cudaGetLastError();
 }
-template <int MODE>
+template <int KIND>
 cudaError_t launch_act(int act, const Maps& maps, const Geo& g, cudaStream_t st) {
-  return act == SCA2_ACT_SILU ? launch<MODE, SILU>(maps, g, st) : launch<MODE, GELU>(maps, g, st);
+  return act == SCA2_ACT_SILU ? launch<KIND, SILU>(maps, g, st) : launch<KIND, GELU>(maps, g, st);
 }
 
 template <int NG, int MINB = 2>
@@ -694,27 +743,43 @@ Geo geo_proj(const sca2_ffn_args& a) {
   g.units = g.tiles_n * g.tiles_m, g.kb = ceil_div(a.d, BK);
   return g;
 }
-Geo geo_dx(const sca2_ffn_args& a) {
-  Geo g = geo_proj(a);
-  g.tiles_n = ceil_div(a.d, 256);
-  g.units = g.tiles_n * g.tiles_m, g.kb_half = ceil_div(a.f, BK), g.kb = 2 * g.kb_half;
-  return g;
+// The pairs' share of the DX tiles beside their DW tiles (pair p has DW units p, p + pairs, ...): x_a
+// for those with one DW unit more than the others, x_b for the others.  Returns the longest pair's
+// contraction blocks, a tile's start and end counted as `LAP` blocks.
+constexpr int LAP = 4;
+double share(Geo& g) {
+  const int pairs = pairs_of(g);
+  const double cw = (double)g.kb / g.splits + LAP, cx = 2.0 * g.kb_half + LAP;
+  const int q = g.units / pairs;
+  g.x_pairs = g.units % pairs;
+  const int rest = pairs - g.x_pairs;
+  const double even = (g.units * cw + g.x_units * cx) / pairs;
+  double best = 1e30;
+  for (int i = 0; i < 2; ++i) {
+    const int xa = std::max(0, (int)((even - (q + 1) * cw) / cx) + i);
+    const int64_t left = std::max<int64_t>(0, g.x_units - (int64_t)xa * g.x_pairs);
+    const int xb = (int)((left + rest - 1) / rest);
+    const double longest = std::max(g.x_pairs ? (q + 1) * cw + xa * cx : 0.0, q * cw + xb * cx);
+    if (longest < best) best = longest, g.x_a = xa, g.x_b = xb;
+  }
+  return best;
 }
-// Splits of the rows: the fewest whose rounds of tiles waste least of the machine, each split
-// keeping at least 16 contraction blocks (its fp32 part costs a write and a read of the tile).
-Geo geo_dw(const sca2_ffn_args& a) {
+// DW and DX.  Splits of the rows: the fewest whose longest pair is shortest, each split keeping at
+// least 16 contraction blocks; from two on, the parts cost a launch and a pass over them.
+Geo geo_grads(const sca2_ffn_args& a, bool need_x, bool need_w) {
   Geo g = geo_proj(a);
   g.tiles_n = ceil_div(a.d, 256), g.tiles_m = ceil_div(a.f, 256), g.slices = 2;
-  g.kb = ceil_div(a.rows, BK);
-  const int tiles = g.tiles_n * g.tiles_m * 2;
-  double best = 1e30;
-  g.splits = 1;
-  for (int s = 1; s <= 32 && (s == 1 || g.kb / s >= 16); ++s) {
-    const double cost = ((double)ceil_div((int64_t)tiles * s, PAIRS) / s) * (g.kb + 6.0 * s);
-    if (cost < best * 0.97) best = cost, g.splits = s;
+  g.kb = ceil_div(a.rows, BK), g.kb_half = ceil_div(a.f, BK);
+  g.x_units = need_x ? g.tiles_n * ceil_div(a.rows, 256) : 0;
+  const int tiles = need_w ? g.tiles_n * g.tiles_m * 2 : 0;
+  Geo best = g;
+  double least = 1e30;
+  for (int s = 1; s <= (need_w ? 32 : 1) && (s == 1 || g.kb / s >= 16); ++s) {
+    g.splits = s, g.units = tiles * s;
+    const double cost = share(g) + (s > 1 ? 12 + 2 * s : 0);
+    if (cost < least * 0.97) least = cost, best = g;
   }
-  g.units = tiles * g.splits;
-  return g;
+  return best;
 }
 
 int check(const sca2_ffn_args* a) {
@@ -780,7 +845,7 @@ int64_t sca2_gated_ffn_work_bytes(int64_t rows, int32_t d, int32_t f) {
   if (rows < 1 || d < 1 || f < 1 || rows > (1LL << 30)) return 0;
   sca2_ffn_args a{};
   a.rows = rows, a.d = d, a.f = f;
-  const int s = geo_dw(a).splits;
+  const int s = std::max(geo_grads(a, true, true).splits, geo_grads(a, false, true).splits);
   return 2 * up256(rows * f * 2) + (s > 1 ? (int64_t)s * 2 * f * d * 4 : 0);
 }
 
@@ -802,44 +867,37 @@ int sca2_gated_ffn_bwd(const sca2_ffn_args* a, const void* dh, void* dx, void* d
     return fail(SCA2_ERR_ARG, "gated_ffn: workspace null, not 256-byte aligned or too small");
   if (!dx && !dw_gate) return SCA2_OK;
   e = allow_act<BACK>(a->act);
-  if (e == cudaSuccess) e = allow<DX, SILU>();
-  if (e == cudaSuccess) e = allow<DW, SILU>();
+  if (e == cudaSuccess) e = allow<GRADS, SILU>();
   if (e != cudaSuccess) return cuda_fail(e, "sca2_gated_ffn_bwd");
   if (!sca2::tensor_map_encoder()) return fail(SCA2_ERR_CUDA, "gated_ffn: no tensor-map encoder in the driver");
   uint8_t* w = static_cast<uint8_t*>(work);
   void *dg = w, *du = w + up256(a->rows * a->f * 2), *part = w + 2 * up256(a->rows * a->f * 2);
   const int64_t n = a->rows;
-  const char* refused = "gated_ffn: tensor map refused";
-  Maps m;
+  const Geo g = geo_grads(*a, dx != nullptr, dw_gate != nullptr);
+  Maps m, x;
   memset(&m, 0, sizeof(m));
-  if (!map2(&m.a0, a->x, n, a->d, a->ldx, 128) || !map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 128) ||
-      !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) || !map2(&m.o0, dg, n, a->f, a->f, 0) ||
-      !map2(&m.o1, du, n, a->f, a->f, 0) || !map2(&m.dh, dh, n, a->f, a->f, 0))
-    return fail(SCA2_ERR_CUDA, refused);
-  e = launch_act<BACK>(a->act, m, geo_proj(*a), st);
-  if (e == cudaSuccess && dx) {
-    memset(&m, 0, sizeof(m));
-    if (!map2(&m.a0, dg, n, a->f, a->f, 128) || !map2(&m.a1, du, n, a->f, a->f, 128) ||
-        !map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 64) || !map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 64) ||
-        !map2(&m.o0, dx, n, a->d, a->d, 0))
-      return fail(SCA2_ERR_CUDA, refused);
-    e = launch<DX, SILU>(m, geo_dx(*a), st);
+  bool ok = map2(&m.a0, a->x, n, a->d, a->ldx, 128) && map2(&m.b0, a->w_gate, a->f, a->d, a->ldg, 128) &&
+            map2(&m.b1, a->w_up, a->f, a->d, a->ldu, 128) && map2(&m.o0, dg, n, a->f, a->f, 0) &&
+            map2(&m.o1, du, n, a->f, a->f, 0) && map2(&m.dh, dh, n, a->f, a->f, 0);
+  memset(&x, 0, sizeof(x));
+  if (dx)
+    ok = ok && map2(&x.xa0, dg, n, a->f, a->f, 128) && map2(&x.xa1, du, n, a->f, a->f, 128) &&
+         map2(&x.xb0, a->w_gate, a->f, a->d, a->ldg, 64) && map2(&x.xb1, a->w_up, a->f, a->d, a->ldu, 64) &&
+         map2(&x.xo, dx, n, a->d, a->d, 0);
+  if (dw_gate) {
+    ok = ok && map2(&x.a0, dg, n, a->f, a->f, 64) && map2(&x.a1, du, n, a->f, a->f, 64) &&
+         map2(&x.b0, a->x, n, a->d, a->ldx, 64);
+    if (g.splits > 1) ok = ok && map3(&x.o0, part, 2 * g.splits, a->f, a->d);
+    else ok = ok && map2(&x.o0, dw_gate, a->f, a->d, a->d, 0) && map2(&x.o1, dw_up, a->f, a->d, a->d, 0);
   }
-  if (e == cudaSuccess && dw_gate) {
-    const Geo g = geo_dw(*a);
-    memset(&m, 0, sizeof(m));
-    bool ok = map2(&m.a0, dg, n, a->f, a->f, 64) && map2(&m.a1, du, n, a->f, a->f, 64) &&
-              map2(&m.b0, a->x, n, a->d, a->ldx, 64);
-    if (g.splits > 1) ok = ok && map3(&m.o0, part, 2 * g.splits, a->f, a->d);
-    else ok = ok && map2(&m.o0, dw_gate, a->f, a->d, a->d, 0) && map2(&m.o1, dw_up, a->f, a->d, a->d, 0);
-    if (!ok) return fail(SCA2_ERR_CUDA, refused);
-    e = launch<DW, SILU>(m, g, st);
-    if (e == cudaSuccess && g.splits > 1) {
-      const int64_t n4 = (int64_t)a->f * a->d / 4;
-      dw_reduce<<<(unsigned)((2 * n4 + 255) / 256), 256, 0, st>>>(static_cast<const float4*>(part), g.splits, n4,
-                                                                  static_cast<uint2*>(dw_gate), static_cast<uint2*>(dw_up));
-      e = cudaGetLastError();
-    }
+  if (!ok) return fail(SCA2_ERR_CUDA, "gated_ffn: tensor map refused");
+  e = launch_act<BACK>(a->act, m, geo_proj(*a), st);
+  if (e == cudaSuccess) e = launch<GRADS, SILU>(x, g, st);
+  if (e == cudaSuccess && dw_gate && g.splits > 1) {
+    const int64_t n4 = (int64_t)a->f * a->d / 4;
+    dw_reduce<<<(unsigned)((2 * n4 + 255) / 256), 256, 0, st>>>(static_cast<const float4*>(part), g.splits, n4,
+                                                                static_cast<uint2*>(dw_gate), static_cast<uint2*>(dw_up));
+    e = cudaGetLastError();
   }
   return e == cudaSuccess ? SCA2_OK : cuda_fail(e, "sca2_gated_ffn_bwd");
 }
