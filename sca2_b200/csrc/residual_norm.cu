@@ -13,20 +13,23 @@ struct Outs {
   float* p[NPART];
 };
 
-// column sums of the CTAs' partials, 32 columns to a CTA, the partial rows over its 8 warps
-__global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ part, int nparts, int d, const Outs o) {
-  __shared__ float s[8][32];
+// column sums of the CTAs' partials, 32 columns to a CTA, the partial rows over its 16 warps
+constexpr int RW = 16;
+__global__ void __launch_bounds__(32 * RW) reduce_kernel(const float* __restrict__ part, int nparts, int d, const Outs o) {
+  __shared__ float s[RW][32];
   float* out = o.p[blockIdx.y];
   if (!out) return;
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (c < d)
-    for (int i = w; i < nparts; i += 8) v += part[((int64_t)i * NPART + blockIdx.y) * d + c];
-  s[w][threadIdx.x & 31] = v;
+  if (c < d) {
+#pragma unroll 8
+    for (int i = w; i < nparts; i += RW) v += part[((int64_t)i * NPART + blockIdx.y) * d + c];
+  }
+  s[w][lane] = v;
   __syncthreads();
   if (w == 0 && c < d) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) v += s[k][threadIdx.x];
+    for (int k = 1; k < RW; ++k) v += s[k][lane];
     out[c] = v;
   }
 }
@@ -136,7 +139,7 @@ int sca2_residual_norm_bwd(const sca2_rnorm_args* a, const float* stats, const v
                                          : (a->u_dtype == SCA2_BF16 ? bwd_f32_bf16 : bwd_f32_f32);
   cudaError_t e = f(k, contig, st);
   if (e == cudaSuccess && (o.p[0] || o.p[1] || o.p[2] || o.p[3] || o.p[4])) {
-    reduce_kernel<<<dim3((a->d + 31) / 32, NPART), 256, 0, st>>>(k.part, bwd_grid(a->rows, a->d), a->d, o);
+    reduce_kernel<<<dim3((a->d + 31) / 32, NPART), 32 * RW, 0, st>>>(k.part, bwd_grid(a->rows, a->d), a->d, o);
     e = cudaGetLastError();
   }
   return e == cudaSuccess ? SCA2_OK : cuda_fail(e, "sca2_residual_norm_bwd");

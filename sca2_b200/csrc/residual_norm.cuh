@@ -626,11 +626,12 @@ __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
 }
 
 // Backward for rows of up to 1024 aligned values, many of them: as bwd_kernel with the options that
-// cost instructions as template parameters, and the rows to come on their way into shared memory
-// (STAGES - 1 steps ahead) while the present ones are reduced.
+// cost instructions as template parameters, and the next rows on their way into shared memory while
+// the present ones are reduced.  Two rows a step, one step ahead: three ahead need so much shared
+// memory that one CTA an SM is left (65536 x 768: 226 us, 340 so; one row a step 249, three 246).
 template <int GATE, bool HASZ, class TX, class TU>
 struct BwdRing {
-  static constexpr int R = 2, STAGES = 3, MAXT = 256;
+  static constexpr int R = 2, STAGES = 2, MAXT = 256;
   // offsets of a row's slots, in bytes of one thread; every array's slots lie thread by thread
   static constexpr int BX = 4 * sizeof(TX), BU = 4 * sizeof(TU), BZ = 16;
   static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0),
@@ -822,8 +823,10 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
 }
 
 // Rows in flight in a CTA, and the CTAs (each leaves one row of partials): two to an SM, three of the
-// few-row kernel.  `many`: rows enough that every CTA of bwd_ring (or its unaligned form) has several steps.
-inline bool many(int64_t rows, int d) { return d <= 1024 && rows >= 148 * 8; }
+// few-row kernel.  `many`: rows from which two at a time win (backward of 1184, 2368, 4736 rows, few-row kernel
+// against bwd_ring: d = 256 7.2 / 5.6, 12.1 / 7.7, 20.6 / 12.4 us; d = 768 8.5 / 12.4, 13.8 / 16.1, 30.8 / 24.1;
+// d = 1024 9.5 / 14.6, 16.4 / 21.1, 36.4 / 33.1).
+inline bool many(int64_t rows, int d) { return d <= 1024 && rows >= 4 * d; }
 inline int bwd_grid(int64_t rows, int d) {
   const bool m = many(rows, d);
   const int most = 148 * (d > 2048 ? 1 : d > 1024 || m ? 2 : 3);
@@ -855,9 +858,10 @@ cudaError_t fwd_ring_gate(const Args& a, cudaStream_t st) {
   return a.gate_mode == 0 ? fwd_ring_width<0, POST, TX, TU>(a, st)
          : a.gate_mode == 1 ? fwd_ring_width<1, POST, TX, TU>(a, st) : fwd_ring_width<2, POST, TX, TU>(a, st);
 }
-// Up to FEW_ROWS rows a CTA owns a row (fwd_kernel): all rows at once, each by more threads.  vec:
-// rows and pointers allow groups of four values.
-constexpr int FEW_ROWS = 148 * 4;
+// Up to FEW_ROWS rows a CTA owns a row (fwd_kernel), all rows at once, each by more threads (64, 592,
+// 1184, 2368 rows of 768 values, against fwd_ring: 3.3 / 7.4, 4.1 / 7.6, 6.9 / 7.7, 11.1 / 9.5 us; of 1024:
+// 3.3 / 6.5, 4.3 / 6.7, 7.2 / 6.9, 11.9 / 9.6).  vec: rows and pointers allow groups of four values.
+constexpr int FEW_ROWS = 148 * 8;
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   const int d = a.d;

@@ -1402,6 +1402,12 @@ def _gated_ffn_backward(ctx, dh):
 _gated_ffn_fwd.register_autograd(_gated_ffn_backward, setup_context=_gated_ffn_setup)
 
 
+def _tied(t: Optional[torch.Tensor]):
+    """An upstream gradient that requires one itself: what once_differentiable makes of it then raises
+    when it is differentiated, where it would otherwise count as constant."""
+    return t if t is None or t.requires_grad else t.detach().requires_grad_(True)
+
+
 class _GatedFFN(torch.autograd.Function):
     """The eager path of gated_ffn: the same two calls without the operator dispatch."""
 
@@ -1412,10 +1418,16 @@ class _GatedFFN(torch.autograd.Function):
         return _gated_ffn_run(x, wg, wu, act)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh):
+        return _GatedFFN.grads(ctx, dh) if not torch.is_grad_enabled() else _GatedFFN.once(ctx, _tied(dh))
+
+    @staticmethod
+    def grads(ctx, dh):
         need = ctx.needs_input_grad
-        return (*_gated_ffn_bwd_run(*ctx.saved_tensors, ctx.act, dh, need[0], need[1] or need[2]), None)
+        x, wg, wu = ctx.saved_tensors
+        return (*_gated_ffn_bwd_run(x, wg, wu, ctx.act, dh, need[0], need[1] or need[2]), None)
+
+    once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
 
 
 def gated_ffn_supported(d: int, f: int) -> bool:
@@ -1495,8 +1507,10 @@ def _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, z
 
 def _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: float, zdt: torch.dtype, stats, dy, dz):
     dense = torch.contiguous_format
-    dy = None if dy is None else dy.to(x.dtype).contiguous()
-    dz = None if dz is None else dz.to(zdt).contiguous()
+    if dy is not None and (dy.dtype != x.dtype or not dy.is_contiguous()):
+        dy = dy.to(x.dtype).contiguous()
+    if dz is not None and (dz.dtype != zdt or not dz.is_contiguous()):
+        dz = dz.to(zdt).contiguous()
     dx, du = torch.empty_like(x, memory_format=dense), torch.empty_like(u, memory_format=dense)
     dgate = torch.empty_like(gate, memory_format=dense) if gate is not None else None
     dw, db, dscale, dpw, dpb = [None if t is None else torch.empty_like(t) for t in (w, b, scale, pw, pb)]
@@ -1571,11 +1585,18 @@ class _ResidualNorm(torch.autograd.Function):
         return y, z
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dz):
+        if torch.is_grad_enabled():
+            return _ResidualNorm.once(ctx, _tied(dy), _tied(dz))
+        return _ResidualNorm.grads(ctx, dy, dz)
+
+    @staticmethod
+    def grads(ctx, dy, dz):
         *ins, stats = ctx.saved_tensors
         return (*_residual_norm_bwd_run(*ins, *ctx.opts, stats, dy, dz if ins[2] is not None else None),
                 None, None, None)
+
+    once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
 
 
 def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tensor] = None,

@@ -250,3 +250,14 @@ def test_custom_op():
     assert torch.equal(a, b)
     for p, q in zip(torch.autograd.grad(a, leaves, dh), torch.autograd.grad(b, leaves, dh)):
         assert torch.equal(p, q)
+
+
+def test_not_twice_differentiable():
+    from sca2_b200 import ops
+    x, wg, wu, dh = _inputs(70, 64, 72)
+    leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    ref = _run(x, wg, wu, dh, "silu")
+    (g,) = torch.autograd.grad(ops.gated_ffn(*leaves), leaves[:1], dh, create_graph=True)
+    assert torch.equal(g, ref["dx"])
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()

@@ -133,7 +133,7 @@ def test_widths(rows, d, kind):
     _check(*_inputs(rows, d, bias=kind == "layer"), kind=kind)
 
 
-@pytest.mark.parametrize("rows", [1183, 1184, 1189, 5000])
+@pytest.mark.parametrize("rows", [383, 384, 1184, 1185, 1331, 1332, 3071, 3073, 5000])
 @pytest.mark.parametrize("d", [96, 333, 768, 1536])
 def test_many_rows(rows, d):
     _check(*_inputs(rows, d, F, H), zt=H)
@@ -325,3 +325,13 @@ def test_custom_op():
     assert torch.equal(a, b)
     for p, q in zip(torch.autograd.grad(a, (x, u), dz), torch.autograd.grad(b, (x, u), dz)):
         assert torch.equal(p, q)
+
+
+def test_not_twice_differentiable():
+    from sca2_b200 import ops
+    i, dy, dz = _inputs(6, 40)
+    x = i["x"].requires_grad_(True)
+    y, z = ops.residual_norm(x, i["u"], i["weight"])
+    (g,) = torch.autograd.grad((y, z), x, (dy, dz), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
