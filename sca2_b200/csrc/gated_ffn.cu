@@ -30,7 +30,7 @@
 // which is cuBLAS's rate; at d = 768 the epilogue and the switch of tiles add 15%, in BACK 30% (half of
 // that its stores).  L2 prefetches of the operands by TMA slowed every product (360 -> 400 us).
 //
-// Up to FFN_FEW_ROWS rows (decode) the forward is bound by reading the weights and by latency:
+// Up to FEW_ROWS rows (decode) the forward is bound by reading the weights and by latency:
 // `ffn_few` keeps no tiles, each warp streams weight rows straight into mma.sync fragments.
 //
 // Every wait is bounded: a wait that runs out sets the fault word and the kernel leaves.
