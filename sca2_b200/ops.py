@@ -1316,9 +1316,6 @@ def linear16(x: torch.Tensor, w: torch.Tensor, sizes: Tuple[int, ...]) -> Tuple[
 
 
 # ======================================================================================
-#  preallocated plans (benchmarks, CUDA-graph capture)
-# ======================================================================================
-# ======================================================================================
 #  gated feed-forward projections
 # ======================================================================================
 _ACT = {"silu": 0, "gelu": 1}
@@ -1402,6 +1399,15 @@ def _gated_ffn_backward(ctx, dh):
 _gated_ffn_fwd.register_autograd(_gated_ffn_backward, setup_context=_gated_ffn_setup)
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _traced(x: torch.Tensor) -> bool:
+    """Whether a call goes through the registered operator (tracing, fake and other tensor subclasses)
+    rather than straight to the library."""
+    return torch.compiler.is_compiling() or type(x) not in _PLAIN
+
+
 def _tied(t: Optional[torch.Tensor]):
     """An upstream gradient that requires one itself: what once_differentiable makes of it then raises
     when it is differentiated, where it would otherwise count as constant."""
@@ -1453,7 +1459,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
                 f"{tuple(w_up.shape)}")
     if not gated_ffn_supported(shape[1], shape[0]):
         raise E(f"gated_ffn: d and f must be multiples of 8, got {shape[1]} and {shape[0]}")
-    if torch.compiler.is_compiling():
+    if _traced(x):
         return torch.ops.sca2b200.gated_ffn_fwd(x, w_gate, w_up, _ACT[act])
     if _wants_grad(x, w_gate, w_up):
         return _GatedFFN.apply(x, w_gate, w_up, _ACT[act])
@@ -1640,7 +1646,7 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
         gate = gate.to(u.dtype)
     w, b, sc, pw, pb = par
     kid, eps = _NORM_KIND[kind], float(eps)
-    if torch.compiler.is_compiling():
+    if _traced(x):
         y, z, _ = torch.ops.sca2b200.residual_norm_fwd(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt,
                                                        _wants_grad(x, u, w, b, gate, sc, pw, pb))
     elif _wants_grad(x, u, w, b, gate, sc, pw, pb):
@@ -1788,6 +1794,9 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     return norm
 
 
+# ======================================================================================
+#  preallocated plans (benchmarks, CUDA-graph capture)
+# ======================================================================================
 class PhaseScanPlan:
     """A phase-flavour scan with every output / saved / gradient buffer allocated once, so
     fwd() and bwd() are exactly one library call each and can be timed or captured in a CUDA

@@ -166,6 +166,10 @@ def test_gated_ffn_entry_refusals():
 def test_fake_shapes():
     with FakeTensorMode():
         b, w2 = torch.empty(2, 3, 16, device="cuda", dtype=torch.bfloat16), torch.empty(24, 16, device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(16, device="cuda", requires_grad=True)
+        y, z = ops.residual_norm(b, b, w, post_weight=w)  # the public calls trace too
+        assert y.shape == z.shape == b.shape and z.requires_grad
+        assert ops.gated_ffn(b, w2, w2).shape == (2, 3, 24)
         h = torch.ops.sca2b200.gated_ffn_fwd(b, w2, w2, 0)
         assert h.shape == (2, 3, 24) and h.dtype == torch.bfloat16
         out = torch.ops.sca2b200.gated_ffn_bwd(b, w2, w2, 0, h, True, False)
