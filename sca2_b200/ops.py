@@ -1675,7 +1675,7 @@ def _grad_list(what: str, grads, out=None):
         try:
             types.append(list(map(_dtype, ts)))
             devs = set(map(_T.get_device, ts))
-            ok = set(types[-1]) <= _DT.keys() and {t.layout for t in ts} <= {torch.strided}
+            ok = set(types[-1]) <= _DT.keys()
         except (AttributeError, TypeError):  # not tensors
             ok = False
         if not ok:
@@ -1717,7 +1717,9 @@ def _apart(grads):
 def _clip_run(grads, outs, types, max_norm: Optional[float], dev: int) -> torch.Tensor:
     # a gradient that is not contiguous goes through a contiguous copy
     src, back = grads, ()
-    if not all(map(_T.is_contiguous, grads)):
+    if not all(map(_T.is_contiguous, grads)):  # sparse tensors are not
+        if any(g.layout is not torch.strided for g in grads):
+            raise _lib.Sca2Error("clip_grads: gradients must be dense tensors")
         src = [g.contiguous() for g in grads]
         if outs is grads and max_norm is not None:
             back = [(g, s) for g, s in zip(grads, src) if g is not s]
@@ -1789,7 +1791,9 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
         return torch.zeros((), device="cuda")
     with torch.no_grad():
         norm = _clip_run(grads, outs, types, max_norm, dev)
-    if not torch.is_inference_mode_enabled():  # inference tensors have no version
+    try:
+        torch.autograd.graph.increment_version(outs)
+    except RuntimeError:  # inference tensors have no version
         torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
     return norm
 

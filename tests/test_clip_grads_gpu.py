@@ -156,6 +156,14 @@ def test_not_contiguous_tensors_apart():
         _check([keep], [i], ops.clip_grads([i], 0.5), 0.5)
 
 
+def test_sparse_is_refused():
+    from sca2_b200 import _lib, ops
+    t = torch.eye(4, device="cuda").to_sparse()
+    for call in (lambda: ops.grad_norm([t]), lambda: ops.clip_grads([t], 1.0)):
+        with pytest.raises(_lib.Sca2Error, match="dense"):
+            call()
+
+
 def test_compiled():
     from sca2_b200 import ops
     a, b = _tensors([(40,), (3, 5)])
