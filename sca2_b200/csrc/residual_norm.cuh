@@ -12,6 +12,8 @@
 // inputs and the saved means and deviations (16 bytes a row) instead of keeping them.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace sca2 {
@@ -423,6 +425,121 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
   copies_wait<0>();
 }
 
+// Forward for wider aligned rows: a CTA owns a row, each thread NG groups of four columns and their
+// parameters; the next row travels as in fwd_ring.
+template <int NG, int GATE, bool POST, class TX, class TU>
+__global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
+  using L = FwdRing<NG, GATE, TX, TU>;
+  extern __shared__ __align__(16) uint8_t slots[];
+  const int t = threadIdx.x, d = a.d;
+  const float inv = 1.f / (float)d;
+  const auto col = [&](int k) { return 4 * (t + FT * k); };
+  const auto slot = [&](int off, int k, int bytes) { return slots + off + (k * FT + t) * bytes; };
+  const auto fetch_u = [&](int64_t r) {
+    if (r < a.rows) {
+      const TU* p = reinterpret_cast<const TU*>(a.u) + r * a.su;
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        if (col(k) < d) copy_async<L::BU>(slot(0, k, L::BU), p + col(k));
+    }
+    copies_commit();
+  };
+  const auto fetch_x = [&](int64_t r) {
+    if (r < a.rows) {
+      const TX* p = reinterpret_cast<const TX*>(a.x) + r * a.sx;
+      const TU* q = reinterpret_cast<const TU*>(a.gate) + r * a.sg;
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        if (col(k) < d) {
+          copy_async<L::BX>(slot(L::OX, k, L::BX), p + col(k));
+          if constexpr (GATE == 2) copy_async<L::BU>(slot(L::OG, k, L::BU), q + col(k));
+        }
+    }
+    copies_commit();
+  };
+  int64_t row = blockIdx.x;
+  fetch_u(row), fetch_x(row);
+  F2 w[NG][2], b[NG][2], pw[NG][2], pb[NG][2], sc[NG][2], y[NG][2];
+  const auto param = [&](const float* p, float fill, F2 (&v)[NG][2]) {
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      v[k][0] = v[k][1] = both(fill);
+      if (p && col(k) < d) load2(p + col(k), v[k]);
+    }
+  };
+  param(a.w, 0.f, w), param(a.b, 0.f, b), param(a.scale, 1.f, sc);
+  if constexpr (POST) param(a.pw, 0.f, pw), param(a.pb, 0.f, pb);
+  int flip = 0;
+  const auto normalise = [&](float& mu, float& rs) {  // y <- y - mean
+    mu = 0.f;
+    if (!a.rms) {
+      F2 s = both(0.f);
+#pragma unroll
+      for (int k = 0; k < NG; ++k) s = s + (y[k][0] + y[k][1]);  // columns past d hold 0
+      mu = row_sum(sum(s), flip) * inv;
+    }
+    const F2 m = both(-mu);
+    F2 q0 = both(0.f), q1 = q0;
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+        y[k][0] = y[k][0] + m, y[k][1] = y[k][1] + m;
+        q0 = fma(y[k][0], y[k][0], q0), q1 = fma(y[k][1], y[k][1], q1);
+      }
+    rs = rsqrtf(row_sum(sum(q0 + q1), flip) * inv + a.eps);
+  };
+  for (; row < a.rows; row += gridDim.x) {
+    float gt = 1.f;
+    if constexpr (GATE == 1) {
+      loadv<1>(reinterpret_cast<const TU*>(a.gate) + row * a.sg, &gt);
+      gt = sigmoid(gt);
+    }
+    copies_wait<1>();
+    float mu = 0.f, rs = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      y[k][0] = y[k][1] = both(0.f);
+      if (col(k) < d) load2(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
+    }
+    fetch_u(row + gridDim.x);
+    if constexpr (POST) {
+      normalise(mu, rs);
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) y[k][j] = fma(y[k][j] * both(rs), pw[k][j], pb[k][j]);  // 0 past d
+    }
+    if (a.stats && t == 0) a.stats[4 * row] = mu, a.stats[4 * row + 1] = rs;
+    copies_wait<1>();
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+        F2 q[2];
+        if constexpr (GATE == 2) {
+          load2(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
+          y[k][0] = y[k][0] * sigmoid(q[0]), y[k][1] = y[k][1] * sigmoid(q[1]);
+        }
+        load2(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) y[k][j] = fma(GATE == 1 ? both(gt) * sc[k][j] : sc[k][j], y[k][j], q[j]);
+        store2(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
+      }
+    fetch_x(row + gridDim.x);
+    if (!a.z) continue;
+    normalise(mu, rs);
+    if (a.stats && t == 0) a.stats[4 * row + 2] = mu, a.stats[4 * row + 3] = rs;
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (col(k) < d) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) y[k][j] = fma(y[k][j] * both(rs), w[k][j], b[k][j]);
+        if (a.zdt == SCA2_BF16) store2(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), y[k]);
+        else store2(reinterpret_cast<float*>(a.z) + row * d + col(k), y[k]);
+      }
+  }
+  copies_wait<0>();
+}
+
 // ---- backward -------------------------------------------------------------------------------
 // A thread owns four columns of every row (4t ... 4t+3, or t + T k where rows are not aligned), so
 // the five column sums stay in its registers over all its rows; R rows are in flight at once,
@@ -625,59 +742,89 @@ __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
   if (post && a.pb) store(part + PART_PB * d, apb);
 }
 
-// Backward for rows of up to 1024 aligned values, many of them: as bwd_kernel with the options that
-// cost instructions as template parameters, and the next rows on their way into shared memory while
-// the present ones are reduced.  Two rows a step, one step ahead: three ahead need so much shared
-// memory that one CTA an SM is left (65536 x 768: 226 us, 340 so; one row a step 249, three 246).
-template <int GATE, bool HASZ, class TX, class TU>
+// Backward for aligned rows, many of them: as bwd_kernel with the options that cost instructions as
+// template parameters, and the next rows on their way into shared memory while the present ones are
+// reduced.  A thread owns C groups of four columns (4t and, C = 2, 4(t + T)) of R rows at a time, C R = 2:
+// two rows to 1024 values, one beyond.  One step ahead: three ahead need so much shared memory that one
+// CTA an SM is left (65536 x 768: 226 us, 340 so; one row a step 249, three 246).  With C = 2 the
+// parameters lie in the thread's slots too; their sums fill the registers.
+template <int C, int GATE, bool HASZ, class TX, class TU>
 struct BwdRing {
-  static constexpr int R = 2, STAGES = 2, MAXT = 256;
-  // offsets of a row's slots, in bytes of one thread; every array's slots lie thread by thread
-  static constexpr int BX = 4 * sizeof(TX), BU = 4 * sizeof(TU), BZ = 16;
-  static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0),
-                       OST = OZ + (HASZ ? BZ : 0), ROW = OST + 16;
+  static constexpr int R = 2 / C, STAGES = 2, MAXT = C == 1 ? 256 : 512, MINB = C == 1 ? 2 : 1;
+  // offsets of a group's slots, in bytes of one thread; every array's slots lie thread by thread
+  static constexpr int BX = 4 * sizeof(TX), BU = 4 * sizeof(TU);
+  static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0);
+  // bytes of a thread: a group with z of zb bytes a group; all of it
+  static __host__ __device__ int group(int zb) { return OZ + (HASZ ? zb : 0); }
+  static __host__ __device__ int thread(int zb) {
+    return STAGES * R * (C * group(zb) + 16) + (C == 2 ? C * 4 * 16 : 0);  // 16: the row's statistics
+  }
 };
-template <int GATE, bool POST, bool HASZ, class TX, class TU>
-__global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
-  using L = BwdRing<GATE, HASZ, TX, TU>;
-  constexpr int W = 8, R = L::R, ST = L::STAGES;
+template <int C, int GATE, bool POST, bool HASZ, class TX, class TU>
+__global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<C, GATE, HASZ, TX, TU>::MINB)
+    bwd_ring(const Args a) {
+  using L = BwdRing<C, GATE, HASZ, TX, TU>;
+  constexpr int W = L::MAXT / 32, R = L::R, ST = L::STAGES, N = 2 * C;  // N pairs of a row
   __shared__ __align__(16) float red[2][3 * R * W];
   extern __shared__ __align__(16) uint8_t slots[];
   const int t = threadIdx.x, T = blockDim.x, d = a.d;
   const float inv = 1.f / (float)d;
-  const bool mine = 4 * t < d;
+  const auto col = [&](int g) { return 4 * (t + T * g); };
   for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
   __syncthreads();
-  const auto param = [&](const float* p, float fill, F2 (&v)[2]) {
-    v[0] = v[1] = both(mine ? fill : 0.f);  // columns past d: kept out of the sums
-    if (p && mine) load2(p + 4 * t, v);
+  const bool zb16 = a.zdt == SCA2_BF16;
+  const int zb = zb16 ? 8 : 16, grp = L::group(zb);
+  const auto slot = [&](int stage, int i, int g, int off, int bytes) {
+    return slots + ((stage * R + i) * C + g) * grp * T + off * T + bytes * t;
   };
+  uint8_t* const stat0 = slots + ST * R * C * grp * T + 16 * t;  // statistics of (stage, row): + (stage R + row) 16 T
+  float* const par0 = reinterpret_cast<float*>(slots + ST * R * (C * grp + 16) * T) + 4 * t;  // parameter i of group g: + (4 g + i) 4 T
   const F2 zero = both(0.f), one = both(1.f), minus = both(-1.f);
-  F2 w[2], sc[2], pw[2], pb[2];
-  if constexpr (HASZ) param(a.w, 0.f, w);
-  param(a.scale, 1.f, sc);
-  if constexpr (POST) param(a.pw, 1.f, pw), param(a.pb, 0.f, pb);
-  F2 aw[2] = {zero, zero}, ab[2] = {zero, zero}, as[2] = {zero, zero}, apw[2] = {zero, zero}, apb[2] = {zero, zero};
+  // w, scale, pw, pb of the thread's columns; 0 past d, which keeps those out of the sums
+  F2 reg[4][2];
+  {
+    const float* src[4] = {HASZ ? a.w : nullptr, a.scale, POST ? a.pw : nullptr, POST ? a.pb : nullptr};
+#pragma unroll
+    for (int g = 0; g < C; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool mine = col(g) < d;
+        F2 v[2];
+        v[0] = v[1] = both(mine && (i == 1 || i == 2) ? 1.f : 0.f);
+        if (src[i] && mine) load2(src[i] + col(g), v);
+        if constexpr (C == 1) reg[i][0] = v[0], reg[i][1] = v[1];
+        else store2(par0 + (4 * g + i) * 4 * T, v);
+      }
+  }
+  const auto param = [&](int i, int g, F2 (&v)[2]) {
+    if constexpr (C == 1) v[0] = reg[i][0], v[1] = reg[i][1];
+    else load2(par0 + (4 * g + i) * 4 * T, v);
+  };
+  F2 aw[N], ab[N], as[N], apw[N], apb[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) aw[j] = ab[j] = as[j] = apw[j] = apb[j] = zero;
 
   const int64_t step = (int64_t)gridDim.x * R;
-  const auto slot = [&](int stage, int i, int off, int bytes) {
-    return slots + (int64_t)(stage * R + i) * L::ROW * T + off * T + bytes * t;
-  };
   const auto fetch = [&](int64_t r0, int stage) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int64_t r = r0 + i;
-      if (r < a.rows && mine) {
-        copy_async<L::BU>(slot(stage, i, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su + 4 * t);
-        copy_async<L::BX>(slot(stage, i, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx + 4 * t);
-        if (a.dy) copy_async<L::BX>(slot(stage, i, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d + 4 * t);
-        if constexpr (GATE == 2)
-          copy_async<L::BU>(slot(stage, i, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg + 4 * t);
-        if constexpr (HASZ) {
-          if (a.zdt == SCA2_BF16) copy_async<8>(slot(stage, i, L::OZ, L::BZ), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d + 4 * t);
-          else copy_async<16>(slot(stage, i, L::OZ, L::BZ), reinterpret_cast<const float*>(a.dz) + r * d + 4 * t);
+      if (r < a.rows) {
+#pragma unroll
+        for (int g = 0; g < C; ++g) {
+          const int c = col(g);
+          if (c >= d) continue;
+          copy_async<L::BU>(slot(stage, i, g, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su + c);
+          copy_async<L::BX>(slot(stage, i, g, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx + c);
+          if (a.dy) copy_async<L::BX>(slot(stage, i, g, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d + c);
+          if constexpr (GATE == 2)
+            copy_async<L::BU>(slot(stage, i, g, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg + c);
+          if constexpr (HASZ) {
+            if (zb16) copy_async<8>(slot(stage, i, g, L::OZ, 8), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d + c);
+            else copy_async<16>(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const float*>(a.dz) + r * d + c);
+          }
         }
-        copy_async<16>(slot(stage, i, L::OST, 16), a.stats + 4 * r);
+        copy_async<16>(stat0 + (stage * R + i) * 16 * T, a.stats + 4 * r);
       }
     }
     copies_commit();
@@ -697,41 +844,49 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
       }
     }
     copies_wait<ST - 1>();
-    F2 un[R][2], s[R][2], dy[R][2], yn[R][2], dn[R][2];
+    F2 un[R][N], s[R][N], dy[R][N], yn[R][N], dn[R][N];
     float v[2 * R], ru[R], ry[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float st[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) un[i][j] = dy[i][j] = yn[i][j] = dn[i][j] = zero, s[i][j] = one;
-      if (r0 + i < a.rows && mine) {
-        loadv<4>(reinterpret_cast<const float*>(slot(stage, i, L::OST, 16)), st);
-        load2(reinterpret_cast<const TU*>(slot(stage, i, L::OU, L::BU)), un[i]);
-        if constexpr (HASZ) load2(reinterpret_cast<const TX*>(slot(stage, i, L::OX, L::BX)), yn[i]);
-        if (a.dy) load2(reinterpret_cast<const TX*>(slot(stage, i, L::ODY, L::BX)), dy[i]);
-        if constexpr (GATE == 2) load2(reinterpret_cast<const TU*>(slot(stage, i, L::OG, L::BU)), s[i]);
-        if constexpr (HASZ) {
-          if (a.zdt == SCA2_BF16) load2(reinterpret_cast<const __nv_bfloat16*>(slot(stage, i, L::OZ, L::BZ)), dn[i]);
-          else load2(reinterpret_cast<const float*>(slot(stage, i, L::OZ, L::BZ)), dn[i]);
-        }
-      }
+      const bool in = r0 + i < a.rows;
+      if (in) loadv<4>(reinterpret_cast<const float*>(stat0 + (stage * R + i) * 16 * T), st);
       ru[i] = st[1], ry[i] = st[3];
       const F2 g1 = both(GATE == 1 ? sigmoid(tok[i]) : 1.f);
       F2 v0 = zero, v1 = zero;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if constexpr (POST) un[i][j] = (un[i][j] + both(-st[0])) * both(ru[i]);
-        if constexpr (GATE == 1) s[i][j] = g1;
-        if constexpr (GATE == 2) s[i][j] = sigmoid(s[i][j]);
-        if constexpr (HASZ) {
-          const F2 p = POST ? fma(un[i][j], pw[j], pb[j]) : un[i][j];
-          const F2 y = fma(GATE ? sc[j] * s[i][j] : sc[j], p, yn[i][j]);
-          yn[i][j] = (y + both(-st[2])) * both(ry[i]);
-          aw[j] = fma(dn[i][j], yn[i][j], aw[j]);
-          ab[j] = ab[j] + dn[i][j];
-          dn[i][j] = dn[i][j] * w[j];
-          v0 = v0 + dn[i][j];
-          v1 = fma(dn[i][j], yn[i][j], v1);
+      for (int g = 0; g < C; ++g) {
+        F2 lu[2] = {zero, zero}, lx[2] = {zero, zero}, ly[2] = {zero, zero}, lg[2] = {one, one}, lz[2] = {zero, zero};
+        if (in && col(g) < d) {
+          load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OU, L::BU)), lu);
+          if constexpr (HASZ) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::OX, L::BX)), lx);
+          if (a.dy) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::ODY, L::BX)), ly);
+          if constexpr (GATE == 2) load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OG, L::BU)), lg);
+          if constexpr (HASZ) {
+            if (zb16) load2(reinterpret_cast<const __nv_bfloat16*>(slot(stage, i, g, L::OZ, 8)), lz);
+            else load2(reinterpret_cast<const float*>(slot(stage, i, g, L::OZ, 16)), lz);
+          }
+        }
+        F2 w[2], sc[2], pw[2], pb[2];
+        if constexpr (HASZ) param(0, g, w), param(1, g, sc);
+        if constexpr (POST && HASZ) param(2, g, pw), param(3, g, pb);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = 2 * g + j;
+          un[i][k] = POST ? (lu[j] + both(-st[0])) * both(ru[i]) : lu[j];
+          s[i][k] = GATE == 1 ? g1 : GATE == 2 ? sigmoid(lg[j]) : one;
+          dy[i][k] = ly[j];
+          dn[i][k] = lz[j];
+          if constexpr (HASZ) {
+            const F2 p = POST ? fma(un[i][k], pw[j], pb[j]) : un[i][k];
+            const F2 y = fma(GATE ? sc[j] * s[i][k] : sc[j], p, lx[j]);
+            yn[i][k] = (y + both(-st[2])) * both(ry[i]);
+            aw[k] = fma(dn[i][k], yn[i][k], aw[k]);
+            ab[k] = ab[k] + dn[i][k];
+            dn[i][k] = dn[i][k] * w[j];
+            v0 = v0 + dn[i][k];
+            v1 = fma(dn[i][k], yn[i][k], v1);
+          }
         }
       }
       v[2 * i] = sum(v0), v[2 * i + 1] = sum(v1);
@@ -744,35 +899,42 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int64_t r = r0 + i;
-      if constexpr (HASZ) {
-        const F2 m1 = both(a.rms ? 0.f : -v[2 * i] * inv), m2 = both(-v[2 * i + 1] * inv), rr = both(ry[i]);
+      F2 m1 = zero, m2 = zero;
+      const F2 rr = both(ry[i]);
+      if constexpr (HASZ) m1 = both(a.rms ? 0.f : -v[2 * i] * inv), m2 = both(-v[2 * i + 1] * inv);
+      F2 q0 = zero, q1 = zero, q2 = zero;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) dy[i][j] = fma(rr, fma(yn[i][j], m2, dn[i][j] + m1), dy[i][j]);
-      }
-      const bool in = r < a.rows && mine;
-      if (in) store2(reinterpret_cast<TX*>(a.dx) + r * d + 4 * t, dy[i]);
-      F2 q0 = zero, q1 = zero, q2 = zero, dg[2];
+      for (int g = 0; g < C; ++g) {
+        F2 sc[2], pw[2], pb[2], ey[2], dg[2];
+        param(1, g, sc);
+        if constexpr (POST) param(2, g, pw), param(3, g, pb);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const F2 p = POST ? fma(un[i][j], pw[j], pb[j]) : un[i][j];
-        const F2 es = GATE ? dy[i][j] * s[i][j] : dy[i][j], dp = es * sc[j];
-        as[j] = fma(es, p, as[j]);
-        if constexpr (GATE != 0) {
-          dg[j] = dp * p * fma(s[i][j], minus, one);
-          if constexpr (GATE == 1) q2 = q2 + dg[j];
+        for (int j = 0; j < 2; ++j) {
+          const int k = 2 * g + j;
+          if constexpr (HASZ) dy[i][k] = fma(rr, fma(yn[i][k], m2, dn[i][k] + m1), dy[i][k]);
+          ey[j] = dy[i][k];
+          const F2 p = POST ? fma(un[i][k], pw[j], pb[j]) : un[i][k];
+          const F2 es = GATE ? ey[j] * s[i][k] : ey[j], dp = es * sc[j];
+          as[k] = fma(es, p, as[k]);
+          if constexpr (GATE != 0) {
+            dg[j] = dp * p * fma(s[i][k], minus, one);
+            if constexpr (GATE == 1) q2 = q2 + dg[j];
+          }
+          if constexpr (POST) {
+            apw[k] = fma(dp, un[i][k], apw[k]);
+            apb[k] = apb[k] + dp;
+            dn[i][k] = dp * pw[j];
+            q0 = q0 + dn[i][k];
+            q1 = fma(dn[i][k], un[i][k], q1);
+          } else {
+            dn[i][k] = dp;
+          }
         }
-        if constexpr (POST) {
-          apw[j] = fma(dp, un[i][j], apw[j]);
-          apb[j] = apb[j] + dp;
-          dn[i][j] = dp * pw[j];
-          q0 = q0 + dn[i][j];
-          q1 = fma(dn[i][j], un[i][j], q1);
-        } else {
-          dn[i][j] = dp;
+        if (r < a.rows && col(g) < d) {
+          store2(reinterpret_cast<TX*>(a.dx) + r * d + col(g), ey);
+          if constexpr (GATE == 2) store2(reinterpret_cast<TU*>(a.dgate) + r * d + col(g), dg);
         }
       }
-      if constexpr (GATE == 2)
-        if (in) store2(reinterpret_cast<TU*>(a.dgate) + r * d + 4 * t, dg);
       q[3 * i] = sum(q0), q[3 * i + 1] = sum(q1), q[3 * i + 2] = sum(q2);
     }
     if constexpr (POST && GATE == 1) {
@@ -780,13 +942,13 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
       flip ^= 1;
     } else if constexpr (POST || GATE == 1) {
       float h[2 * R];  // two sums a row, or one
-      constexpr int N = POST ? 2 * R : R;
+      constexpr int M = POST ? 2 * R : R;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         if constexpr (POST) h[2 * i] = q[3 * i], h[2 * i + 1] = q[3 * i + 1];
         else h[i] = q[3 * i + 2];
       }
-      cta_sums<N, W>(h, red[flip]);
+      cta_sums<M, W>(h, red[flip]);
       flip ^= 1;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
@@ -798,39 +960,54 @@ __global__ void __launch_bounds__(256, 2) bwd_ring(const Args a) {
     for (int i = 0; i < R; ++i) {
       const int64_t r = r0 + i;
       if (r >= a.rows) continue;
-      if constexpr (POST) {
-        const F2 m1 = both(a.rms ? 0.f : -q[3 * i] * inv), m2 = both(-q[3 * i + 1] * inv), rr = both(ru[i]);
+      const F2 m1 = both(POST && !a.rms ? -q[3 * i] * inv : 0.f), m2 = both(-q[3 * i + 1] * inv), rr = both(ru[i]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) dn[i][j] = rr * fma(un[i][j], m2, dn[i][j] + m1);
+      for (int g = 0; g < C; ++g) {
+        F2 o[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = 2 * g + j;
+          o[j] = POST ? rr * fma(un[i][k], m2, dn[i][k] + m1) : dn[i][k];
+        }
+        if (col(g) < d) store2(reinterpret_cast<TU*>(a.du) + r * d + col(g), o);
       }
-      if (mine) store2(reinterpret_cast<TU*>(a.du) + r * d + 4 * t, dn[i]);
       if constexpr (GATE == 1)
         if (t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &q[3 * i + 2]);
     }
   }
   copies_wait<0>();
-  if (!mine) return;
-  float* part = a.part + (int64_t)blockIdx.x * NPART * d + 4 * t;
-  if constexpr (HASZ) {
-    store2(part + PART_W * d, aw);
-    if (a.b) store2(part + PART_B * d, ab);
-  }
-  if (a.scale) store2(part + PART_SCALE * d, as);
-  if constexpr (POST) {
-    store2(part + PART_PW * d, apw);
-    if (a.pb) store2(part + PART_PB * d, apb);
+#pragma unroll
+  for (int g = 0; g < C; ++g) {
+    if (col(g) >= d) continue;
+    float* part = a.part + (int64_t)blockIdx.x * NPART * d + col(g);
+    const auto put = [&](int which, const F2* v) {
+      const F2 q[2] = {v[2 * g], v[2 * g + 1]};
+      store2(part + which * d, q);
+    };
+    if constexpr (HASZ) {
+      put(PART_W, aw);
+      if (a.b) put(PART_B, ab);
+    }
+    if (a.scale) put(PART_SCALE, as);
+    if constexpr (POST) {
+      put(PART_PW, apw);
+      if (a.pb) put(PART_PB, apb);
+    }
   }
 }
 
-// Rows in flight in a CTA, and the CTAs (each leaves one row of partials): two to an SM, three of the
-// few-row kernel.  `many`: rows from which two at a time win (backward of 1184, 2368, 4736 rows, few-row kernel
-// against bwd_ring: d = 256 7.2 / 5.6, 12.1 / 7.7, 20.6 / 12.4 us; d = 768 8.5 / 12.4, 13.8 / 16.1, 30.8 / 24.1;
-// d = 1024 9.5 / 14.6, 16.4 / 21.1, 36.4 / 33.1).
-inline bool many(int64_t rows, int d) { return d <= 1024 && rows >= 4 * d; }
+// Threads of a backward CTA: a row's groups of four columns, in warps; C = 2: half as many.
+inline int bwd_threads(int d, int c) { return ((d + 4 * c - 1) / (4 * c) + 31) / 32 * 32; }
+// `many`: rows from which bwd_ring, or two unaligned rows at a time, win (backward of 1184, 2368, 4736 rows,
+// few-row kernel against bwd_ring: d = 256 7.2 / 5.6, 12.1 / 7.7, 20.6 / 12.4 us; d = 768 8.5 / 12.4,
+// 13.8 / 16.1, 30.8 / 24.1; d = 1024 9.5 / 14.6, 16.4 / 21.1, 36.4 / 33.1).
+inline bool many(int64_t rows, int d) { return rows >= (d <= 1024 ? 4 * d : 2048); }
+// The CTAs, each of which leaves one row of partials: two to an SM, more of narrow rows.
 inline int bwd_grid(int64_t rows, int d) {
   const bool m = many(rows, d);
-  const int most = 148 * (d > 2048 ? 1 : d > 1024 || m ? 2 : 3);
-  const int64_t want = m ? (rows + 1) / 2 : rows;
+  const int T = bwd_threads(d, 1);
+  const int most = 148 * (d > 2048 ? 1 : d > 1024 ? 2 : m ? std::max(2, std::min(8, 512 / T)) : 3);
+  const int64_t want = m && d <= 1024 ? (rows + 1) / 2 : rows;
   return (int)(want < most ? want : most);
 }
 
@@ -844,8 +1021,19 @@ cudaError_t fwd_ring_launch(const Args& a, cudaStream_t st) {
   k<<<(int)(want < 148 * 3 ? want : 148 * 3), FT, smem, st>>>(a);
   return cudaGetLastError();
 }
+template <int NG, int GATE, bool POST, class TX, class TU>
+cudaError_t fwd_wide_launch(const Args& a, cudaStream_t st) {
+  constexpr int smem = FwdRing<NG, GATE, TX, TU>::OP;
+  const auto k = fwd_wide<NG, GATE, POST, TX, TU>;
+  if (smem > 47 * 1024)  // and the row sums beside it
+    if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  k<<<(int)(a.rows < 148 * 2 ? a.rows : 148 * 2), FT, smem, st>>>(a);
+  return cudaGetLastError();
+}
 template <int GATE, bool POST, class TX, class TU>
 cudaError_t fwd_ring_width(const Args& a, cudaStream_t st) {
+  if (a.d > 2048) return fwd_wide_launch<4, GATE, POST, TX, TU>(a, st);
+  if (a.d > 1024) return fwd_wide_launch<2, GATE, POST, TX, TU>(a, st);
   switch ((a.d + 255) / 256) {
     case 1: return fwd_ring_launch<2, GATE, POST, TX, TU>(a, st);
     case 2: return fwd_ring_launch<4, GATE, POST, TX, TU>(a, st);
@@ -865,7 +1053,7 @@ constexpr int FEW_ROWS = 148 * 8;
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   const int d = a.d;
-  if (vec && d <= 1024 && a.rows > FEW_ROWS) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
+  if (vec && a.rows > FEW_ROWS) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
   const int grid = (int)(a.rows < 148 * 8 ? a.rows : 148 * 8);
   if (vec) {
     if (d <= 1024) fwd_kernel<1, 4, TX, TU><<<grid, FT, 0, st>>>(a);
@@ -878,29 +1066,40 @@ cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-template <int GATE, bool POST, bool HASZ, class TX, class TU>
+constexpr int SMEM_MOST = 227 * 1024 - 2 * 3 * 16 * 4;  // a CTA's dynamic shared memory beside bwd_ring's sums
+
+template <int C, int GATE, bool POST, bool HASZ, class TX, class TU>
 cudaError_t bwd_ring_launch(const Args& a, cudaStream_t st) {
-  using L = BwdRing<GATE, HASZ, TX, TU>;
-  const int T = ((a.d + 3) / 4 + 31) / 32 * 32, smem = L::STAGES * L::R * L::ROW * T;
-  const auto k = bwd_ring<GATE, POST, HASZ, TX, TU>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, L::STAGES * L::R * L::ROW * L::MAXT)) return e;
+  using L = BwdRing<C, GATE, HASZ, TX, TU>;
+  const int T = bwd_threads(a.d, C), smem = L::thread(a.zdt == SCA2_BF16 ? 8 : 16) * T;
+  const auto k = bwd_ring<C, GATE, POST, HASZ, TX, TU>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
   k<<<bwd_grid(a.rows, a.d), T, smem, st>>>(a);
   return cudaGetLastError();
 }
-template <int GATE, class TX, class TU>
+template <int C, int GATE, class TX, class TU>
+cudaError_t bwd_ring_options(const Args& a, cudaStream_t st) {
+  if (a.pw)
+    return a.dz ? bwd_ring_launch<C, GATE, true, true, TX, TU>(a, st) : bwd_ring_launch<C, GATE, true, false, TX, TU>(a, st);
+  return a.dz ? bwd_ring_launch<C, GATE, false, true, TX, TU>(a, st) : bwd_ring_launch<C, GATE, false, false, TX, TU>(a, st);
+}
+template <int C, class TX, class TU>
 cudaError_t bwd_ring_gate(const Args& a, cudaStream_t st) {
-  if (a.pw) return a.dz ? bwd_ring_launch<GATE, true, true, TX, TU>(a, st) : bwd_ring_launch<GATE, true, false, TX, TU>(a, st);
-  return a.dz ? bwd_ring_launch<GATE, false, true, TX, TU>(a, st) : bwd_ring_launch<GATE, false, false, TX, TU>(a, st);
+  return a.gate_mode == 0 ? bwd_ring_options<C, 0, TX, TU>(a, st)
+         : a.gate_mode == 1 ? bwd_ring_options<C, 1, TX, TU>(a, st) : bwd_ring_options<C, 2, TX, TU>(a, st);
 }
 template <bool CONTIG, class TX, class TU>
 cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
-  const int d = a.d, grid = bwd_grid(a.rows, d);
-  const int T = ((d + 3) / 4 + 31) / 32 * 32;
+  const int d = a.d, grid = bwd_grid(a.rows, d), T = bwd_threads(d, 1);
+  if constexpr (CONTIG) {
+    // all-fp32 rows of 4096 values with everything on do not fit
+    const bool fits = d <= 1024 || BwdRing<2, 2, true, TX, TU>::thread(a.zdt == SCA2_BF16 ? 8 : 16) * bwd_threads(d, 2) <= SMEM_MOST;
+    if (many(a.rows, d) && fits) return d <= 1024 ? bwd_ring_gate<1, TX, TU>(a, st) : bwd_ring_gate<2, TX, TU>(a, st);
+  }
   if (d > 2048) bwd_kernel<1024, 1, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   else if (d > 1024) bwd_kernel<512, 1, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (!many(a.rows, d)) bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (CONTIG || !many(a.rows, d)) bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   else if constexpr (!CONTIG) bwd_kernel<256, 2, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else return a.gate_mode == 0 ? bwd_ring_gate<0, TX, TU>(a, st) : a.gate_mode == 1 ? bwd_ring_gate<1, TX, TU>(a, st) : bwd_ring_gate<2, TX, TU>(a, st);
   return cudaGetLastError();
 }
 template <class TX, class TU>

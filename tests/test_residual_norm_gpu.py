@@ -139,12 +139,29 @@ def test_many_rows(rows, d):
     _check(*_inputs(rows, d, F, H), zt=H)
 
 
+@pytest.mark.parametrize("rows,d", [(2047, 1028), (2048, 1028), (2100, 2048), (2101, 2052), (2050, 4096), (2049, 2501)])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_many_wide_rows(rows, d, kind):
+    _check(*_inputs(rows, d, F, H, bias=kind == "layer"), kind=kind, zt=H)
+    _check(*_inputs(rows, d, bias=kind == "layer"), kind=kind)
+
+
+@pytest.mark.parametrize("rows,d", [(1300, 136), (2050, 1100)])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", ["none", "token", "channel"])
+@pytest.mark.parametrize("scale", [False, True])
+@pytest.mark.parametrize("z", [False, True])
+def test_options_of_many_rows(rows, d, post, gate, scale, z):
+    i, dy, dz = _inputs(rows, d, H if scale else F, H, post, gate, scale, True, z)
+    _check(i, dy, dz, use=("z",) if z and not post else ("y", "z"))
+
+
 @pytest.mark.parametrize("xt", [F, H])
 @pytest.mark.parametrize("ut", [F, H])
 @pytest.mark.parametrize("zt", [F, H])
-@pytest.mark.parametrize("d", [64, 75])
-def test_types(xt, ut, zt, d):
-    _check(*_inputs(50, d, xt, ut), zt=zt)
+@pytest.mark.parametrize("rows,d", [(50, 64), (50, 75), (1250, 64), (1250, 300), (2060, 1056)])
+def test_types(xt, ut, zt, rows, d):
+    _check(*_inputs(rows, d, xt, ut), zt=zt)
 
 
 @pytest.mark.parametrize("post", [False, True])
