@@ -290,47 +290,132 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Forward for rows of up to 1024 aligned values: a warp owns a row, each lane NG groups of four
+// A group of four columns of a row, n of them inside it, in a thread's slot (GB bytes).  ANY: rows of
+// any alignment.  Values of 32 bits then travel one by one; of 16 bits, the two aligned 8-byte words
+// around the group, from which reading shifts it out (word by value at the tensor's two ends [lo, hi),
+// so that nothing outside is read).
+template <bool ANY, class T>
+constexpr int GB = ANY ? 16 : 4 * (int)sizeof(T);
+
+template <bool ANY, class T>
+__device__ __forceinline__ void group_copy(void* slot, const T* p, int n, const T* lo, const T* hi) {
+  if constexpr (!ANY) {
+    copy_async<4 * sizeof(T)>(slot, p);
+  } else if constexpr (sizeof(T) == 4) {
+    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 4 * k), "l"(p + k) : "memory");
+  } else {
+    const T* w = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)7);
+    const int m = (int)(p - w);  // the group's place in the words
+    if (w >= lo && w + 8 <= hi) {
+      copy_async<8>(slot, w);
+      if (m + n > 4) copy_async<8>(static_cast<uint8_t*>(slot) + 8, w + 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < n) static_cast<T*>(slot)[m + k] = p[k];
+    }
+  }
+}
+template <bool ANY, class T>
+__device__ __forceinline__ void group_read(const void* slot, const T* p, int n, F2 (&v)[2]) {
+  if constexpr (!ANY) {
+    load2(static_cast<const T*>(slot), v);
+  } else {
+    float q[4];
+    if constexpr (sizeof(T) == 4) {
+      loadv<4>(static_cast<const float*>(slot), q);
+    } else {
+      const ulonglong2 w = *static_cast<const ulonglong2*>(slot);
+      const int sh = 16 * (int)((reinterpret_cast<uintptr_t>(p) >> 1) & 3);
+      const unsigned long long u = sh ? (w.x >> sh) | (w.y << (64 - sh)) : w.x;
+      unpack2((uint32_t)u, q), unpack2((uint32_t)(u >> 32), q + 2);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k >= n) q[k] = 0.f;
+    v[0] = pair(q[0], q[1]), v[1] = pair(q[2], q[3]);
+  }
+}
+template <bool ANY, class T>
+__device__ __forceinline__ void group_store(T* p, int n, const F2 (&v)[2]) {
+  if constexpr (!ANY) {
+    store2(p, v);
+  } else {
+    const float q[4] = {first(v[0]), second(v[0]), first(v[1]), second(v[1])};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) storev<1>(p + k, q + k);
+  }
+}
+// n values of a parameter, `fill` beyond
+template <bool ANY>
+__device__ __forceinline__ void group_param(const float* p, int n, float fill, F2 (&v)[2]) {
+  if constexpr (!ANY) {
+    load2(p, v);
+  } else {
+    float q[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = k < n ? p[k] : fill;
+    v[0] = pair(q[0], q[1]), v[1] = pair(q[2], q[3]);
+  }
+}
+// zeros beyond the n values inside the row
+template <bool ANY>
+__device__ __forceinline__ void group_clean(int n, F2 (&v)[2]) {
+  if constexpr (ANY) {
+    if (n < 4) {
+      if (n < 1) v[0] = both(0.f);
+      else if (n < 2) v[0] = pair(first(v[0]), 0.f);
+      v[1] = n < 3 ? both(0.f) : pair(first(v[1]), 0.f);
+    }
+  }
+}
+
+// Forward for rows of up to 1024 values: a warp owns a row, each lane NG groups of four
 // values, so that every copy, load and store of the warp is one run of whole sectors in either type.
 // The slots hold one row: the next row's u is asked for once this row's is in registers, its x and
 // gate once the join has read this row's, and both travel under the rest of the row's work.  The
 // parameters lie in shared memory too: read from L1 their latency was the kernel's bound (65536 x
 // 768, everything on: 141 us, 116 us so; 705 MB are 109 us at the copy rate).
-template <int NG, int GATE, class TX, class TU>
+template <int NG, int GATE, bool ANY, class TX, class TU>
 struct FwdRing {  // bytes of a thread's group in each array; the arrays' slots lie thread by thread
-  static constexpr int BU = 4 * sizeof(TU), BX = 4 * sizeof(TX), BG = GATE == 2 ? BU : 0;
+  static constexpr int BU = GB<ANY, TU>, BX = GB<ANY, TX>, BG = GATE == 2 ? BU : 0;
   static constexpr int OX = NG * BU * FT, OG = OX + NG * BX * FT, OP = OG + NG * BG * FT;
   static constexpr int D = NG * 128, BYTES = OP + 5 * D * 4;  // w, b, pw, pb, scale
 };
 
-template <int NG, int GATE, bool POST, class TX, class TU>
+template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
 __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
-  using L = FwdRing<NG, GATE, TX, TU>;
+  using L = FwdRing<NG, GATE, ANY, TX, TU>;
   extern __shared__ __align__(16) uint8_t slots[];
   const int lane = threadIdx.x & 31, d = a.d;
   const float inv = 1.f / (float)d;
   const auto col = [&](int k) { return 4 * (lane + 32 * k); };
+  const auto in = [&](int k) { return ANY ? min(4, d - col(k)) : 4; };
   const auto slot = [&](int off, int k, int bytes) { return slots + off + (k * FT + threadIdx.x) * bytes; };
   const int64_t step = (int64_t)gridDim.x * (FT / 32);
   int64_t row = (int64_t)blockIdx.x * (FT / 32) + (threadIdx.x >> 5);
   const auto fetch_u = [&](int64_t r) {
     if (r < a.rows) {
-      const TU* p = reinterpret_cast<const TU*>(a.u) + r * a.su;
+      const TU *p = reinterpret_cast<const TU*>(a.u), *e = p + (a.rows - 1) * a.su + d;
 #pragma unroll
       for (int k = 0; k < NG; ++k)
-        if (col(k) < d) copy_async<L::BU>(slot(0, k, L::BU), p + col(k));
+        if (col(k) < d) group_copy<ANY>(slot(0, k, L::BU), p + r * a.su + col(k), in(k), p, e);
     }
     copies_commit();
   };
   const auto fetch_x = [&](int64_t r) {
     if (r < a.rows) {
-      const TX* p = reinterpret_cast<const TX*>(a.x) + r * a.sx;
-      const TU* q = reinterpret_cast<const TU*>(a.gate) + r * a.sg;
+      const TX *p = reinterpret_cast<const TX*>(a.x), *e = p + (a.rows - 1) * a.sx + d;
+      const TU *q = reinterpret_cast<const TU*>(a.gate), *f = q + (a.rows - 1) * a.sg + d;
 #pragma unroll
       for (int k = 0; k < NG; ++k)
         if (col(k) < d) {
-          copy_async<L::BX>(slot(L::OX, k, L::BX), p + col(k));
-          if constexpr (GATE == 2) copy_async<L::BU>(slot(L::OG, k, L::BU), q + col(k));
+          group_copy<ANY>(slot(L::OX, k, L::BX), p + r * a.sx + col(k), in(k), p, e);
+          if constexpr (GATE == 2) group_copy<ANY>(slot(L::OG, k, L::BU), q + r * a.sg + col(k), in(k), q, f);
         }
     }
     copies_commit();
@@ -350,6 +435,7 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
         y[k][0] = y[k][0] + m, y[k][1] = y[k][1] + m;
+        group_clean<ANY>(in(k), y[k]);
         q0 = fma(y[k][0], y[k][0], q0), q1 = fma(y[k][1], y[k][1], q1);
       }
     rs = rsqrtf(warp_sum(sum(q0 + q1)) * inv + a.eps);
@@ -366,7 +452,7 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
   float* par = reinterpret_cast<float*>(slots + L::OP);
   const auto stage = [&](int i, const float* p) -> const float* {
     if (!p) return nullptr;
-    for (int c = threadIdx.x; c < d; c += FT) par[i * L::D + c] = p[c];
+    for (int c = threadIdx.x; c < L::D; c += FT) par[i * L::D + c] = c < d ? p[c] : 0.f;
     return par + i * L::D;
   };
   const float *w = stage(0, a.w), *b = stage(1, a.b), *pw = stage(2, a.pw), *pb = stage(3, a.pb), *scale = stage(4, a.scale);
@@ -382,7 +468,7 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
       y[k][0] = y[k][1] = both(0.f);
-      if (col(k) < d) load2(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
+      if (col(k) < d) group_read<ANY>(slot(0, k, L::BU), reinterpret_cast<const TU*>(a.u) + row * a.su, in(k), y[k]);
     }
     fetch_u(row + step);
     if constexpr (POST) {
@@ -402,13 +488,14 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
           y[k][0] = y[k][0] * q[0], y[k][1] = y[k][1] * q[1];
         }
         if constexpr (GATE == 2) {
-          load2(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
+          group_read<ANY>(slot(L::OG, k, L::BU), reinterpret_cast<const TU*>(a.gate) + row * a.sg, in(k), q);
           y[k][0] = y[k][0] * sigmoid(q[0]), y[k][1] = y[k][1] * sigmoid(q[1]);
         }
-        load2(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
+        group_read<ANY>(slot(L::OX, k, L::BX), reinterpret_cast<const TX*>(a.x) + row * a.sx, in(k), q);
 #pragma unroll
         for (int j = 0; j < 2; ++j) y[k][j] = GATE == 1 ? fma(both(gt), y[k][j], q[j]) : y[k][j] + q[j];
-        store2(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
+        group_clean<ANY>(in(k), y[k]);
+        group_store<ANY>(reinterpret_cast<TX*>(a.y) + row * d + col(k), in(k), y[k]);
       }
     fetch_x(row + step);
     if (!a.z) continue;
@@ -418,41 +505,43 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
         affine(k, rs, w, b);
-        if (a.zdt == SCA2_BF16) store2(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), y[k]);
-        else store2(reinterpret_cast<float*>(a.z) + row * d + col(k), y[k]);
+        if (a.zdt == SCA2_BF16) group_store<ANY>(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), in(k), y[k]);
+        else group_store<ANY>(reinterpret_cast<float*>(a.z) + row * d + col(k), in(k), y[k]);
       }
   }
   copies_wait<0>();
 }
 
-// Forward for wider aligned rows: a CTA owns a row, each thread NG groups of four columns and their
-// parameters; the next row travels as in fwd_ring.
-template <int NG, int GATE, bool POST, class TX, class TU>
-__global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
-  using L = FwdRing<NG, GATE, TX, TU>;
+// Forward for wider rows, and from 513 values for those of any alignment (whose slots are larger: 32768 x
+// 1001 in bf16 317 us with fwd_ring, 184 so): a CTA owns a row, each thread NG groups of four columns and
+// their parameters; the next row travels as in fwd_ring.
+template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
+__global__ void __launch_bounds__(FT, NG == 1 ? 4 : 2) fwd_wide(const Args a) {
+  using L = FwdRing<NG, GATE, ANY, TX, TU>;
   extern __shared__ __align__(16) uint8_t slots[];
   const int t = threadIdx.x, d = a.d;
   const float inv = 1.f / (float)d;
   const auto col = [&](int k) { return 4 * (t + FT * k); };
+  const auto in = [&](int k) { return ANY ? min(4, d - col(k)) : 4; };
   const auto slot = [&](int off, int k, int bytes) { return slots + off + (k * FT + t) * bytes; };
   const auto fetch_u = [&](int64_t r) {
     if (r < a.rows) {
-      const TU* p = reinterpret_cast<const TU*>(a.u) + r * a.su;
+      const TU *p = reinterpret_cast<const TU*>(a.u), *e = p + (a.rows - 1) * a.su + d;
 #pragma unroll
       for (int k = 0; k < NG; ++k)
-        if (col(k) < d) copy_async<L::BU>(slot(0, k, L::BU), p + col(k));
+        if (col(k) < d) group_copy<ANY>(slot(0, k, L::BU), p + r * a.su + col(k), in(k), p, e);
     }
     copies_commit();
   };
   const auto fetch_x = [&](int64_t r) {
     if (r < a.rows) {
-      const TX* p = reinterpret_cast<const TX*>(a.x) + r * a.sx;
-      const TU* q = reinterpret_cast<const TU*>(a.gate) + r * a.sg;
+      const TX *p = reinterpret_cast<const TX*>(a.x), *e = p + (a.rows - 1) * a.sx + d;
+      const TU *q = reinterpret_cast<const TU*>(a.gate), *f = q + (a.rows - 1) * a.sg + d;
 #pragma unroll
       for (int k = 0; k < NG; ++k)
         if (col(k) < d) {
-          copy_async<L::BX>(slot(L::OX, k, L::BX), p + col(k));
-          if constexpr (GATE == 2) copy_async<L::BU>(slot(L::OG, k, L::BU), q + col(k));
+          group_copy<ANY>(slot(L::OX, k, L::BX), p + r * a.sx + col(k), in(k), p, e);
+          if constexpr (GATE == 2) group_copy<ANY>(slot(L::OG, k, L::BU), q + r * a.sg + col(k), in(k), q, f);
         }
     }
     copies_commit();
@@ -464,7 +553,7 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
       v[k][0] = v[k][1] = both(fill);
-      if (p && col(k) < d) load2(p + col(k), v[k]);
+      if (p && col(k) < d) group_param<ANY>(p + col(k), in(k), fill, v[k]);
     }
   };
   param(a.w, 0.f, w), param(a.b, 0.f, b), param(a.scale, 1.f, sc);
@@ -484,6 +573,7 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
     for (int k = 0; k < NG; ++k)
       if (col(k) < d) {
         y[k][0] = y[k][0] + m, y[k][1] = y[k][1] + m;
+        group_clean<ANY>(in(k), y[k]);
         q0 = fma(y[k][0], y[k][0], q0), q1 = fma(y[k][1], y[k][1], q1);
       }
     rs = rsqrtf(row_sum(sum(q0 + q1), flip) * inv + a.eps);
@@ -499,7 +589,7 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
       y[k][0] = y[k][1] = both(0.f);
-      if (col(k) < d) load2(reinterpret_cast<const TU*>(slot(0, k, L::BU)), y[k]);
+      if (col(k) < d) group_read<ANY>(slot(0, k, L::BU), reinterpret_cast<const TU*>(a.u) + row * a.su, in(k), y[k]);
     }
     fetch_u(row + gridDim.x);
     if constexpr (POST) {
@@ -516,13 +606,14 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
       if (col(k) < d) {
         F2 q[2];
         if constexpr (GATE == 2) {
-          load2(reinterpret_cast<const TU*>(slot(L::OG, k, L::BU)), q);
+          group_read<ANY>(slot(L::OG, k, L::BU), reinterpret_cast<const TU*>(a.gate) + row * a.sg, in(k), q);
           y[k][0] = y[k][0] * sigmoid(q[0]), y[k][1] = y[k][1] * sigmoid(q[1]);
         }
-        load2(reinterpret_cast<const TX*>(slot(L::OX, k, L::BX)), q);
+        group_read<ANY>(slot(L::OX, k, L::BX), reinterpret_cast<const TX*>(a.x) + row * a.sx, in(k), q);
 #pragma unroll
         for (int j = 0; j < 2; ++j) y[k][j] = fma(GATE == 1 ? both(gt) * sc[k][j] : sc[k][j], y[k][j], q[j]);
-        store2(reinterpret_cast<TX*>(a.y) + row * d + col(k), y[k]);
+        group_clean<ANY>(in(k), y[k]);
+        group_store<ANY>(reinterpret_cast<TX*>(a.y) + row * d + col(k), in(k), y[k]);
       }
     fetch_x(row + gridDim.x);
     if (!a.z) continue;
@@ -533,8 +624,8 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
       if (col(k) < d) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) y[k][j] = fma(y[k][j] * both(rs), w[k][j], b[k][j]);
-        if (a.zdt == SCA2_BF16) store2(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), y[k]);
-        else store2(reinterpret_cast<float*>(a.z) + row * d + col(k), y[k]);
+        if (a.zdt == SCA2_BF16) group_store<ANY>(reinterpret_cast<__nv_bfloat16*>(a.z) + row * d + col(k), in(k), y[k]);
+        else group_store<ANY>(reinterpret_cast<float*>(a.z) + row * d + col(k), in(k), y[k]);
       }
   }
   copies_wait<0>();
@@ -542,8 +633,8 @@ __global__ void __launch_bounds__(FT, 2) fwd_wide(const Args a) {
 
 // ---- backward -------------------------------------------------------------------------------
 // A thread owns four columns of every row (4t ... 4t+3, or t + T k where rows are not aligned), so
-// the five column sums stay in its registers over all its rows; R rows are in flight at once,
-// which hides their loads and shares the two barriers of their row sums.
+// the five column sums stay in its registers over all its rows.  bwd_kernel takes few rows (and the few
+// widest forms that bwd_ring's shared memory does not hold): a row at a time, by as many CTAs as the rows feed.
 template <int N, int O>
 __device__ __forceinline__ void warp_sums(float* v, int lane) {
   // after the halving steps a lane holds N / 2^s of the values, chosen by its upper lane bits
@@ -595,13 +686,13 @@ __device__ __forceinline__ void cta_sums(float* v, float* s) {
   for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, q[i / P], (i % P) * W);
 }
 
-template <int MAXT, int R, int MINB, bool CONTIG, class TX, class TU>
+template <int MAXT, int MINB, bool CONTIG, class TX, class TU>
 __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
   constexpr int W = MAXT <= 256 ? 8 : MAXT / 32;
-  __shared__ __align__(16) float red[2][3 * R * W];
+  __shared__ __align__(16) float red[2][3 * W];
   const int t = threadIdx.x, T = blockDim.x, d = a.d;
   const float inv = 1.f / (float)d;
-  for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
+  for (int i = t; i < 2 * 3 * W; i += T) (&red[0][0])[i] = 0.f;
   __syncthreads();
   const auto col = [&](int k) { return CONTIG ? 4 * t : t + T * k; };  // CONTIG: d % 4 == 0, all four or none
   const auto load = [&](const auto* p, float* v) {
@@ -638,101 +729,71 @@ __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
   float aw[4] = {}, ab[4] = {}, as[4] = {}, apw[4] = {}, apb[4] = {};
   int flip = 0;
 
-  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.rows; r0 += (int64_t)gridDim.x * R) {
-    // per row: un (normalised u, or u), s (the gate), dy, then yn and dn of z
-    float un[R][4], s[R][4], dy[R][4], yn[R][4], dn[R][4], st[R][4];
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    // un (normalised u, or u), s (the gate), dy, then yn and dn of z
+    float un[4] = {}, s[4] = {}, dy[4] = {}, yn[4] = {}, dn[4] = {}, st[4];
+    load(reinterpret_cast<const TU*>(a.u) + r * a.su, un);
+    load(reinterpret_cast<const TX*>(a.x) + r * a.sx, yn);
+    if (chan) load(reinterpret_cast<const TU*>(a.gate) + r * a.sg, s);
+    if (token) {
+      float g;
+      loadv<1>(reinterpret_cast<const TU*>(a.gate) + r * a.sg, &g);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) un[i][k] = s[i][k] = dy[i][k] = yn[i][k] = dn[i][k] = st[i][k] = 0.f;
-      const int64_t r = r0 + i;
-      if (r < a.rows) {
-        load(reinterpret_cast<const TU*>(a.u) + r * a.su, un[i]);
-        load(reinterpret_cast<const TX*>(a.x) + r * a.sx, yn[i]);
-        if (chan) load(reinterpret_cast<const TU*>(a.gate) + r * a.sg, s[i]);
-        if (token) {
-          float g;
-          loadv<1>(reinterpret_cast<const TU*>(a.gate) + r * a.sg, &g);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[i][k] = g;
-        }
-        if (a.dy) load(reinterpret_cast<const TX*>(a.dy) + r * d, dy[i]);
-        if (has_z) {
-          if (a.zdt == SCA2_BF16) load(reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d, dn[i]);
-          else load(reinterpret_cast<const float*>(a.dz) + r * d, dn[i]);
-        }
-        loadv<4>(a.stats + 4 * r, st[i]);
-      }
+      for (int k = 0; k < 4; ++k) s[k] = g;
     }
-    float v[3 * R];
+    if (a.dy) load(reinterpret_cast<const TX*>(a.dy) + r * d, dy);
+    if (has_z) {
+      if (a.zdt == SCA2_BF16) load(reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d, dn);
+      else load(reinterpret_cast<const float*>(a.dz) + r * d, dn);
+    }
+    loadv<4>(a.stats + 4 * r, st);
+    float v[2] = {}, q[3] = {}, dg[4];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      v[2 * i] = v[2 * i + 1] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (post) un[i][k] = (un[i][k] - st[i][0]) * st[i][1];
-        s[i][k] = a.gate_mode ? sigmoid(s[i][k]) : 1.f;
-        if (has_z) {
-          const float y = fmaf(sc[k] * s[i][k], fmaf(un[i][k], pw[k], pb[k]), yn[i][k]);
-          yn[i][k] = (y - st[i][2]) * st[i][3];
-          aw[k] = fmaf(dn[i][k], yn[i][k], aw[k]);
-          ab[k] += dn[i][k];
-          dn[i][k] *= w[k];
-          v[2 * i] += dn[i][k];
-          v[2 * i + 1] = fmaf(dn[i][k], yn[i][k], v[2 * i + 1]);
-        }
+    for (int k = 0; k < 4; ++k) {
+      if (post) un[k] = (un[k] - st[0]) * st[1];
+      s[k] = a.gate_mode ? sigmoid(s[k]) : 1.f;
+      if (has_z) {
+        const float y = fmaf(sc[k] * s[k], fmaf(un[k], pw[k], pb[k]), yn[k]);
+        yn[k] = (y - st[2]) * st[3];
+        aw[k] = fmaf(dn[k], yn[k], aw[k]);
+        ab[k] += dn[k];
+        dn[k] *= w[k];
+        v[0] += dn[k];
+        v[1] = fmaf(dn[k], yn[k], v[1]);
       }
     }
     if (has_z) {
-      cta_sums<2 * R, W>(v, red[flip]);
+      cta_sums<2, W>(v, red[flip]);
       flip ^= 1;
+      const float m1 = a.rms ? 0.f : v[0] * inv, m2 = v[1] * inv;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dy[k] += st[3] * (dn[k] - m1 - yn[k] * m2);
     }
+    store(reinterpret_cast<TX*>(a.dx) + r * d, dy);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int64_t r = r0 + i;
-      float dg[4];
-      if (has_z) {
-        const float m1 = a.rms ? 0.f : v[2 * i] * inv, m2 = v[2 * i + 1] * inv;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) dy[i][k] += st[i][3] * (dn[i][k] - m1 - yn[i][k] * m2);
-      }
-      if (r < a.rows) store(reinterpret_cast<TX*>(a.dx) + r * d, dy[i]);
-      float q0 = 0.f, q1 = 0.f, q2 = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float e = dy[i][k];
-        const float p = fmaf(un[i][k], pw[k], pb[k]);
-        as[k] = fmaf(e * s[i][k], p, as[k]);
-        dg[k] = e * sc[k] * p * s[i][k] * (1.f - s[i][k]);
-        q2 += dg[k];
-        const float dp = e * sc[k] * s[i][k];
-        apw[k] = fmaf(dp, un[i][k], apw[k]);
-        apb[k] += dp;
-        dn[i][k] = dp * pw[k];
-        q0 += dn[i][k];
-        q1 = fmaf(dn[i][k], un[i][k], q1);
-      }
-      if (chan && r < a.rows) store(reinterpret_cast<TU*>(a.dgate) + r * d, dg);
-      s[i][0] = q0, s[i][1] = q1, s[i][2] = q2;  // the gate's values are done with
+    for (int k = 0; k < 4; ++k) {
+      const float e = dy[k], p = fmaf(un[k], pw[k], pb[k]), dp = e * sc[k] * s[k];
+      as[k] = fmaf(e * s[k], p, as[k]);
+      dg[k] = e * sc[k] * p * s[k] * (1.f - s[k]);
+      q[2] += dg[k];
+      apw[k] = fmaf(dp, un[k], apw[k]);
+      apb[k] += dp;
+      dn[k] = dp * pw[k];
+      q[0] += dn[k];
+      q[1] = fmaf(dn[k], un[k], q[1]);
     }
+    if (chan) store(reinterpret_cast<TU*>(a.dgate) + r * d, dg);
     if (post || token) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) v[3 * i] = s[i][0], v[3 * i + 1] = s[i][1], v[3 * i + 2] = s[i][2];
-      cta_sums<3 * R, W>(v, red[flip]);
+      cta_sums<3, W>(q, red[flip]);
       flip ^= 1;
     }
+    if (post) {
+      const float m1 = a.rms ? 0.f : q[0] * inv, m2 = q[1] * inv;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int64_t r = r0 + i;
-      if (r >= a.rows) continue;
-      if (post) {
-        const float m1 = a.rms ? 0.f : v[3 * i] * inv, m2 = v[3 * i + 1] * inv;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) dn[i][k] = st[i][1] * (dn[i][k] - m1 - un[i][k] * m2);
-      }
-      store(reinterpret_cast<TU*>(a.du) + r * d, dn[i]);
-      if (token && t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &v[3 * i + 2]);
+      for (int k = 0; k < 4; ++k) dn[k] = st[1] * (dn[k] - m1 - un[k] * m2);
     }
+    store(reinterpret_cast<TU*>(a.du) + r * d, dn);
+    if (token && t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &q[2]);
   }
   float* part = a.part + (int64_t)blockIdx.x * NPART * d;
   if (has_z) store(part + PART_W * d, aw);
@@ -742,38 +803,43 @@ __global__ void __launch_bounds__(MAXT, MINB) bwd_kernel(const Args a) {
   if (post && a.pb) store(part + PART_PB * d, apb);
 }
 
-// Backward for aligned rows, many of them: as bwd_kernel with the options that cost instructions as
+// Backward for many rows: as bwd_kernel with the options that cost instructions as
 // template parameters, and the next rows on their way into shared memory while the present ones are
 // reduced.  A thread owns C groups of four columns (4t and, C = 2, 4(t + T)) of R rows at a time, C R = 2:
 // two rows to 1024 values, one beyond.  One step ahead: three ahead need so much shared memory that one
 // CTA an SM is left (65536 x 768: 226 us, 340 so; one row a step 249, three 246).  With C = 2 the
-// parameters lie in the thread's slots too; their sums fill the registers.
-template <int C, int GATE, bool HASZ, class TX, class TU>
+// parameters lie in the thread's slots too; their sums fill the registers.  Aligned rows have their copies,
+// reads and stores written out: through the group functions the compiler orders them so that C = 2 loses
+// 4 to 8 % (24576 x 1536: 176 us, 191 so).  Rows of any alignment on bwd_kernel instead: 49152 x 333
+// 200 us, 135 here; 32768 x 1001 in bf16 417, 267; 12288 x 3001 in fp32 522, 412.
+template <int C, int GATE, bool HASZ, bool ANY, class TX, class TU>
 struct BwdRing {
   static constexpr int R = 2 / C, STAGES = 2, MAXT = C == 1 ? 256 : 512, MINB = C == 1 ? 2 : 1;
   // offsets of a group's slots, in bytes of one thread; every array's slots lie thread by thread
-  static constexpr int BX = 4 * sizeof(TX), BU = 4 * sizeof(TU);
+  static constexpr int BX = GB<ANY, TX>, BU = GB<ANY, TU>;
   static constexpr int OU = 0, OX = OU + BU, ODY = OX + BX, OG = ODY + BX, OZ = OG + (GATE == 2 ? BU : 0);
+  static __host__ __device__ int z_bytes(bool bf16) { return bf16 && !ANY ? 8 : 16; }
   // bytes of a thread: a group with z of zb bytes a group; all of it
   static __host__ __device__ int group(int zb) { return OZ + (HASZ ? zb : 0); }
   static __host__ __device__ int thread(int zb) {
     return STAGES * R * (C * group(zb) + 16) + (C == 2 ? C * 4 * 16 : 0);  // 16: the row's statistics
   }
 };
-template <int C, int GATE, bool POST, bool HASZ, class TX, class TU>
-__global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<C, GATE, HASZ, TX, TU>::MINB)
+template <int C, int GATE, bool POST, bool HASZ, bool ANY, class TX, class TU>
+__global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, ANY, TX, TU>::MAXT, BwdRing<C, GATE, HASZ, ANY, TX, TU>::MINB)
     bwd_ring(const Args a) {
-  using L = BwdRing<C, GATE, HASZ, TX, TU>;
+  using L = BwdRing<C, GATE, HASZ, ANY, TX, TU>;
   constexpr int W = L::MAXT / 32, R = L::R, ST = L::STAGES, N = 2 * C;  // N pairs of a row
   __shared__ __align__(16) float red[2][3 * R * W];
   extern __shared__ __align__(16) uint8_t slots[];
   const int t = threadIdx.x, T = blockDim.x, d = a.d;
   const float inv = 1.f / (float)d;
   const auto col = [&](int g) { return 4 * (t + T * g); };
+  const auto inside = [&](int g) { return ANY ? min(4, d - col(g)) : 4; };
   for (int i = t; i < 2 * 3 * R * W; i += T) (&red[0][0])[i] = 0.f;
   __syncthreads();
   const bool zb16 = a.zdt == SCA2_BF16;
-  const int zb = zb16 ? 8 : 16, grp = L::group(zb);
+  const int zb = L::z_bytes(zb16), grp = L::group(zb);
   const auto slot = [&](int stage, int i, int g, int off, int bytes) {
     return slots + ((stage * R + i) * C + g) * grp * T + off * T + bytes * t;
   };
@@ -791,7 +857,12 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
         const bool mine = col(g) < d;
         F2 v[2];
         v[0] = v[1] = both(mine && (i == 1 || i == 2) ? 1.f : 0.f);
-        if (src[i] && mine) load2(src[i] + col(g), v);
+        if constexpr (!ANY) {
+          if (src[i] && mine) load2(src[i] + col(g), v);
+        } else if (mine) {
+          if (src[i]) group_param<ANY>(src[i] + col(g), inside(g), 0.f, v);
+          else group_clean<ANY>(inside(g), v);
+        }
         if constexpr (C == 1) reg[i][0] = v[0], reg[i][1] = v[1];
         else store2(par0 + (4 * g + i) * 4 * T, v);
       }
@@ -814,14 +885,28 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
         for (int g = 0; g < C; ++g) {
           const int c = col(g);
           if (c >= d) continue;
-          copy_async<L::BU>(slot(stage, i, g, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su + c);
-          copy_async<L::BX>(slot(stage, i, g, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx + c);
-          if (a.dy) copy_async<L::BX>(slot(stage, i, g, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d + c);
-          if constexpr (GATE == 2)
-            copy_async<L::BU>(slot(stage, i, g, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg + c);
-          if constexpr (HASZ) {
-            if (zb16) copy_async<8>(slot(stage, i, g, L::OZ, 8), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d + c);
-            else copy_async<16>(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const float*>(a.dz) + r * d + c);
+          if constexpr (!ANY) {
+            copy_async<L::BU>(slot(stage, i, g, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su + c);
+            copy_async<L::BX>(slot(stage, i, g, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx + c);
+            if (a.dy) copy_async<L::BX>(slot(stage, i, g, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d + c);
+            if constexpr (GATE == 2)
+              copy_async<L::BU>(slot(stage, i, g, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg + c);
+            if constexpr (HASZ) {
+              if (zb16) copy_async<8>(slot(stage, i, g, L::OZ, 8), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d + c);
+              else copy_async<16>(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const float*>(a.dz) + r * d + c);
+            }
+          } else {
+            const auto copy = [&](uint8_t* s, const auto* p, int64_t stride) {
+              group_copy<ANY>(s, p + r * stride + c, inside(g), p, p + (a.rows - 1) * stride + d);
+            };
+            copy(slot(stage, i, g, L::OU, L::BU), reinterpret_cast<const TU*>(a.u), a.su);
+            copy(slot(stage, i, g, L::OX, L::BX), reinterpret_cast<const TX*>(a.x), a.sx);
+            if (a.dy) copy(slot(stage, i, g, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy), d);
+            if constexpr (GATE == 2) copy(slot(stage, i, g, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate), a.sg);
+            if constexpr (HASZ) {
+              if (zb16) copy(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const __nv_bfloat16*>(a.dz), d);
+              else copy(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const float*>(a.dz), d);
+            }
           }
         }
         copy_async<16>(stat0 + (stage * R + i) * 16 * T, a.stats + 4 * r);
@@ -858,13 +943,27 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
       for (int g = 0; g < C; ++g) {
         F2 lu[2] = {zero, zero}, lx[2] = {zero, zero}, ly[2] = {zero, zero}, lg[2] = {one, one}, lz[2] = {zero, zero};
         if (in && col(g) < d) {
-          load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OU, L::BU)), lu);
-          if constexpr (HASZ) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::OX, L::BX)), lx);
-          if (a.dy) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::ODY, L::BX)), ly);
-          if constexpr (GATE == 2) load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OG, L::BU)), lg);
-          if constexpr (HASZ) {
-            if (zb16) load2(reinterpret_cast<const __nv_bfloat16*>(slot(stage, i, g, L::OZ, 8)), lz);
-            else load2(reinterpret_cast<const float*>(slot(stage, i, g, L::OZ, 16)), lz);
+          if constexpr (!ANY) {
+            load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OU, L::BU)), lu);
+            if constexpr (HASZ) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::OX, L::BX)), lx);
+            if (a.dy) load2(reinterpret_cast<const TX*>(slot(stage, i, g, L::ODY, L::BX)), ly);
+            if constexpr (GATE == 2) load2(reinterpret_cast<const TU*>(slot(stage, i, g, L::OG, L::BU)), lg);
+            if constexpr (HASZ) {
+              if (zb16) load2(reinterpret_cast<const __nv_bfloat16*>(slot(stage, i, g, L::OZ, 8)), lz);
+              else load2(reinterpret_cast<const float*>(slot(stage, i, g, L::OZ, 16)), lz);
+            }
+          } else {
+            const int64_t r = r0 + i;
+            const int n = inside(g);
+            group_read<ANY>(slot(stage, i, g, L::OU, L::BU), reinterpret_cast<const TU*>(a.u) + r * a.su, n, lu);
+            if constexpr (HASZ) group_read<ANY>(slot(stage, i, g, L::OX, L::BX), reinterpret_cast<const TX*>(a.x) + r * a.sx, n, lx);
+            if (a.dy) group_read<ANY>(slot(stage, i, g, L::ODY, L::BX), reinterpret_cast<const TX*>(a.dy) + r * d, n, ly);
+            if constexpr (GATE == 2)
+              group_read<ANY>(slot(stage, i, g, L::OG, L::BU), reinterpret_cast<const TU*>(a.gate) + r * a.sg, n, lg);
+            if constexpr (HASZ) {
+              if (zb16) group_read<ANY>(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const __nv_bfloat16*>(a.dz) + r * d, n, lz);
+              else group_read<ANY>(slot(stage, i, g, L::OZ, 16), reinterpret_cast<const float*>(a.dz) + r * d, n, lz);
+            }
           }
         }
         F2 w[2], sc[2], pw[2], pb[2];
@@ -931,8 +1030,10 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
           }
         }
         if (r < a.rows && col(g) < d) {
-          store2(reinterpret_cast<TX*>(a.dx) + r * d + col(g), ey);
-          if constexpr (GATE == 2) store2(reinterpret_cast<TU*>(a.dgate) + r * d + col(g), dg);
+          if constexpr (ANY) group_store<ANY>(reinterpret_cast<TX*>(a.dx) + r * d + col(g), inside(g), ey);
+          else store2(reinterpret_cast<TX*>(a.dx) + r * d + col(g), ey);
+          if constexpr (GATE == 2) if constexpr (ANY) group_store<ANY>(reinterpret_cast<TU*>(a.dgate) + r * d + col(g), inside(g), dg);
+          else store2(reinterpret_cast<TU*>(a.dgate) + r * d + col(g), dg);
         }
       }
       q[3 * i] = sum(q0), q[3 * i + 1] = sum(q1), q[3 * i + 2] = sum(q2);
@@ -969,7 +1070,8 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
           const int k = 2 * g + j;
           o[j] = POST ? rr * fma(un[i][k], m2, dn[i][k] + m1) : dn[i][k];
         }
-        if (col(g) < d) store2(reinterpret_cast<TU*>(a.du) + r * d + col(g), o);
+        if (col(g) < d) if constexpr (ANY) group_store<ANY>(reinterpret_cast<TU*>(a.du) + r * d + col(g), inside(g), o);
+        else store2(reinterpret_cast<TU*>(a.du) + r * d + col(g), o);
       }
       if constexpr (GATE == 1)
         if (t == 0) storev<1>(reinterpret_cast<TU*>(a.dgate) + r, &q[3 * i + 2]);
@@ -982,7 +1084,8 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, TX, TU>::MAXT, BwdRing<
     float* part = a.part + (int64_t)blockIdx.x * NPART * d + col(g);
     const auto put = [&](int which, const F2* v) {
       const F2 q[2] = {v[2 * g], v[2 * g + 1]};
-      store2(part + which * d, q);
+      if constexpr (ANY) group_store<ANY>(part + which * d, inside(g), q);
+      else store2(part + which * d, q);
     };
     if constexpr (HASZ) {
       put(PART_W, aw);
@@ -1011,40 +1114,47 @@ inline int bwd_grid(int64_t rows, int d) {
   return (int)(want < most ? want : most);
 }
 
-template <int NG, int GATE, bool POST, class TX, class TU>
+template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
 cudaError_t fwd_ring_launch(const Args& a, cudaStream_t st) {
-  constexpr int smem = FwdRing<NG, GATE, TX, TU>::BYTES;
-  const auto k = fwd_ring<NG, GATE, POST, TX, TU>;
+  constexpr int smem = FwdRing<NG, GATE, ANY, TX, TU>::BYTES;
+  const auto k = fwd_ring<NG, GATE, POST, ANY, TX, TU>;
   if (smem > 48 * 1024)
     if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
   const int64_t want = (a.rows + 7) / 8;
   k<<<(int)(want < 148 * 3 ? want : 148 * 3), FT, smem, st>>>(a);
   return cudaGetLastError();
 }
-template <int NG, int GATE, bool POST, class TX, class TU>
+template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
 cudaError_t fwd_wide_launch(const Args& a, cudaStream_t st) {
-  constexpr int smem = FwdRing<NG, GATE, TX, TU>::OP;
-  const auto k = fwd_wide<NG, GATE, POST, TX, TU>;
+  constexpr int smem = FwdRing<NG, GATE, ANY, TX, TU>::OP;
+  const auto k = fwd_wide<NG, GATE, POST, ANY, TX, TU>;
   if (smem > 47 * 1024)  // and the row sums beside it
     if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
-  k<<<(int)(a.rows < 148 * 2 ? a.rows : 148 * 2), FT, smem, st>>>(a);
+  constexpr int most = 148 * (NG == 1 ? 4 : 2);
+  k<<<(int)(a.rows < most ? a.rows : most), FT, smem, st>>>(a);
   return cudaGetLastError();
 }
-template <int GATE, bool POST, class TX, class TU>
+template <int GATE, bool POST, bool ANY, class TX, class TU>
 cudaError_t fwd_ring_width(const Args& a, cudaStream_t st) {
-  if (a.d > 2048) return fwd_wide_launch<4, GATE, POST, TX, TU>(a, st);
-  if (a.d > 1024) return fwd_wide_launch<2, GATE, POST, TX, TU>(a, st);
+  if (a.d > 2048) return fwd_wide_launch<4, GATE, POST, ANY, TX, TU>(a, st);
+  if (a.d > 1024) return fwd_wide_launch<2, GATE, POST, ANY, TX, TU>(a, st);
+  if constexpr (ANY)
+    if (a.d > 512) return fwd_wide_launch<1, GATE, POST, ANY, TX, TU>(a, st);
   switch ((a.d + 255) / 256) {
-    case 1: return fwd_ring_launch<2, GATE, POST, TX, TU>(a, st);
-    case 2: return fwd_ring_launch<4, GATE, POST, TX, TU>(a, st);
-    case 3: return fwd_ring_launch<6, GATE, POST, TX, TU>(a, st);
-    default: return fwd_ring_launch<8, GATE, POST, TX, TU>(a, st);
+    case 1: return fwd_ring_launch<2, GATE, POST, ANY, TX, TU>(a, st);
+    case 2: return fwd_ring_launch<4, GATE, POST, ANY, TX, TU>(a, st);
+    default: break;
   }
+  if constexpr (ANY) return cudaErrorInvalidValue;  // not reached
+  else return a.d <= 768 ? fwd_ring_launch<6, GATE, POST, ANY, TX, TU>(a, st) : fwd_ring_launch<8, GATE, POST, ANY, TX, TU>(a, st);
 }
-template <bool POST, class TX, class TU>
-cudaError_t fwd_ring_gate(const Args& a, cudaStream_t st) {
-  return a.gate_mode == 0 ? fwd_ring_width<0, POST, TX, TU>(a, st)
-         : a.gate_mode == 1 ? fwd_ring_width<1, POST, TX, TU>(a, st) : fwd_ring_width<2, POST, TX, TU>(a, st);
+template <bool ANY, class TX, class TU>
+cudaError_t fwd_ring_options(const Args& a, cudaStream_t st) {
+  if (a.pw)
+    return a.gate_mode == 0 ? fwd_ring_width<0, true, ANY, TX, TU>(a, st)
+           : a.gate_mode == 1 ? fwd_ring_width<1, true, ANY, TX, TU>(a, st) : fwd_ring_width<2, true, ANY, TX, TU>(a, st);
+  return a.gate_mode == 0 ? fwd_ring_width<0, false, ANY, TX, TU>(a, st)
+         : a.gate_mode == 1 ? fwd_ring_width<1, false, ANY, TX, TU>(a, st) : fwd_ring_width<2, false, ANY, TX, TU>(a, st);
 }
 // Up to FEW_ROWS rows a CTA owns a row (fwd_kernel), all rows at once, each by more threads (64, 592,
 // 1184, 2368 rows of 768 values, against fwd_ring: 3.3 / 7.4, 4.1 / 7.6, 6.9 / 7.7, 11.1 / 9.5 us; of 1024:
@@ -1053,8 +1163,8 @@ constexpr int FEW_ROWS = 148 * 8;
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
   const int d = a.d;
-  if (vec && a.rows > FEW_ROWS) return a.pw ? fwd_ring_gate<true, TX, TU>(a, st) : fwd_ring_gate<false, TX, TU>(a, st);
-  const int grid = (int)(a.rows < 148 * 8 ? a.rows : 148 * 8);
+  if (a.rows > FEW_ROWS) return vec ? fwd_ring_options<false, TX, TU>(a, st) : fwd_ring_options<true, TX, TU>(a, st);
+  const int grid = (int)a.rows;
   if (vec) {
     if (d <= 1024) fwd_kernel<1, 4, TX, TU><<<grid, FT, 0, st>>>(a);
     else if (d <= 2048) fwd_kernel<2, 4, TX, TU><<<grid, FT, 0, st>>>(a);
@@ -1068,38 +1178,37 @@ cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
 
 constexpr int SMEM_MOST = 227 * 1024 - 2 * 3 * 16 * 4;  // a CTA's dynamic shared memory beside bwd_ring's sums
 
-template <int C, int GATE, bool POST, bool HASZ, class TX, class TU>
+template <int C, int GATE, bool POST, bool HASZ, bool ANY, class TX, class TU>
 cudaError_t bwd_ring_launch(const Args& a, cudaStream_t st) {
-  using L = BwdRing<C, GATE, HASZ, TX, TU>;
-  const int T = bwd_threads(a.d, C), smem = L::thread(a.zdt == SCA2_BF16 ? 8 : 16) * T;
-  const auto k = bwd_ring<C, GATE, POST, HASZ, TX, TU>;
+  using L = BwdRing<C, GATE, HASZ, ANY, TX, TU>;
+  const int T = bwd_threads(a.d, C), smem = L::thread(L::z_bytes(a.zdt == SCA2_BF16)) * T;
+  const auto k = bwd_ring<C, GATE, POST, HASZ, ANY, TX, TU>;
   if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
   k<<<bwd_grid(a.rows, a.d), T, smem, st>>>(a);
   return cudaGetLastError();
 }
-template <int C, int GATE, class TX, class TU>
+template <int C, int GATE, bool ANY, class TX, class TU>
 cudaError_t bwd_ring_options(const Args& a, cudaStream_t st) {
   if (a.pw)
-    return a.dz ? bwd_ring_launch<C, GATE, true, true, TX, TU>(a, st) : bwd_ring_launch<C, GATE, true, false, TX, TU>(a, st);
-  return a.dz ? bwd_ring_launch<C, GATE, false, true, TX, TU>(a, st) : bwd_ring_launch<C, GATE, false, false, TX, TU>(a, st);
+    return a.dz ? bwd_ring_launch<C, GATE, true, true, ANY, TX, TU>(a, st) : bwd_ring_launch<C, GATE, true, false, ANY, TX, TU>(a, st);
+  return a.dz ? bwd_ring_launch<C, GATE, false, true, ANY, TX, TU>(a, st) : bwd_ring_launch<C, GATE, false, false, ANY, TX, TU>(a, st);
 }
-template <int C, class TX, class TU>
+template <int C, bool ANY, class TX, class TU>
 cudaError_t bwd_ring_gate(const Args& a, cudaStream_t st) {
-  return a.gate_mode == 0 ? bwd_ring_options<C, 0, TX, TU>(a, st)
-         : a.gate_mode == 1 ? bwd_ring_options<C, 1, TX, TU>(a, st) : bwd_ring_options<C, 2, TX, TU>(a, st);
+  return a.gate_mode == 0 ? bwd_ring_options<C, 0, ANY, TX, TU>(a, st)
+         : a.gate_mode == 1 ? bwd_ring_options<C, 1, ANY, TX, TU>(a, st) : bwd_ring_options<C, 2, ANY, TX, TU>(a, st);
 }
 template <bool CONTIG, class TX, class TU>
 cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
   const int d = a.d, grid = bwd_grid(a.rows, d), T = bwd_threads(d, 1);
-  if constexpr (CONTIG) {
-    // all-fp32 rows of 4096 values with everything on do not fit
-    const bool fits = d <= 1024 || BwdRing<2, 2, true, TX, TU>::thread(a.zdt == SCA2_BF16 ? 8 : 16) * bwd_threads(d, 2) <= SMEM_MOST;
-    if (many(a.rows, d) && fits) return d <= 1024 ? bwd_ring_gate<1, TX, TU>(a, st) : bwd_ring_gate<2, TX, TU>(a, st);
-  }
-  if (d > 2048) bwd_kernel<1024, 1, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (d > 1024) bwd_kernel<512, 1, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if (CONTIG || !many(a.rows, d)) bwd_kernel<256, 1, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
-  else if constexpr (!CONTIG) bwd_kernel<256, 2, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  // rows near 4096 values with everything on and no type of 16 bits, or of any alignment, do not fit
+  using L = BwdRing<2, 2, true, !CONTIG, TX, TU>;
+  const bool fits = d <= 1024 || L::thread(L::z_bytes(a.zdt == SCA2_BF16)) * bwd_threads(d, 2) <= SMEM_MOST;
+  if (many(a.rows, d) && fits)
+    return d <= 1024 ? bwd_ring_gate<1, !CONTIG, TX, TU>(a, st) : bwd_ring_gate<2, !CONTIG, TX, TU>(a, st);
+  if (d > 2048) bwd_kernel<1024, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else if (d > 1024) bwd_kernel<512, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
+  else bwd_kernel<256, 3, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   return cudaGetLastError();
 }
 template <class TX, class TU>

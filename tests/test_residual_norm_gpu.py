@@ -146,7 +146,21 @@ def test_many_wide_rows(rows, d, kind):
     _check(*_inputs(rows, d, bias=kind == "layer"), kind=kind)
 
 
-@pytest.mark.parametrize("rows,d", [(1300, 136), (2050, 1100)])
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 33, 130, 515, 770, 1023, 1025, 2049, 3001, 4093])
+@pytest.mark.parametrize("xt,ut", [(F, H), (H, F), (H, H)])
+def test_many_rows_of_any_alignment(d, xt, ut):
+    """Rows that begin anywhere: odd widths, and (tensors shifted by a value, odd row strides) odd places."""
+    rows = 1300 if d <= 515 else max(2050, min(4 * d, 4100))
+    i, dy, dz = _inputs(rows, d, xt, ut)
+    _check(i, dy, dz, zt=ut)
+    if d in (5, 130, 770, 1025):
+        off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+        _check({n: off(t.detach()) for n, t in i.items()}, dy, dz, kind="layer", zt=xt)
+        i, dy, dz = _inputs(rows, d, xt, ut, pad=3)
+        _check(i, dy, dz)
+
+
+@pytest.mark.parametrize("rows,d", [(1300, 136), (1300, 135), (2050, 1100), (2050, 1101)])
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("gate", ["none", "token", "channel"])
 @pytest.mark.parametrize("scale", [False, True])
