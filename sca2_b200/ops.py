@@ -1403,9 +1403,9 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _traced(x: torch.Tensor) -> bool:
-    """Whether a call goes through the registered operator (tracing, fake and other tensor subclasses)
-    rather than straight to the library."""
-    return torch.compiler.is_compiling() or type(x) not in _PLAIN
+    """Whether a call goes through the registered operator (tracing, fake and other tensor subclasses,
+    vmap's batched tensors) rather than straight to the library."""
+    return torch.compiler.is_compiling() or type(x) not in _PLAIN or torch._C._are_functorch_transforms_active()
 
 
 def _tied(t: Optional[torch.Tensor]):

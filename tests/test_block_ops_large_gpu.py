@@ -45,6 +45,29 @@ def test_residual_norm():
         assert float((got.float() - ref.float()).abs().max()) <= 2 ** -7 * float(ref.float().abs().max())
 
 
+def test_residual_norm_of_any_alignment():
+    """As above with odd rows of a wider tensor: the copies of words around each group."""
+    from sca2_b200 import ops
+    _room(60)
+    n, d = 2 ** 31 // 1001 + 5000, 1001
+    x = torch.empty(n, d + 6, device="cuda", dtype=H).normal_()[:, 3:3 + d]
+    u = torch.empty(n, d, device="cuda", dtype=H).normal_()
+    w, s, dz = (torch.randn(d, device="cuda") for _ in range(3))
+    rows = _far((n, d))
+    xs, us = x.detach().requires_grad_(True), u.requires_grad_(True)
+    y, z = ops.residual_norm(xs, us, w, scale=s, kind="rms")
+    xr, ur = x[rows].requires_grad_(True), u.detach()[rows].requires_grad_(True)
+    yr, zr = ops.residual_norm(xr, ur, w, scale=s, kind="rms")
+    # two roundings to bf16 apart, and the sums' order: as above
+    near = lambda a, b: bool(((a.float() - b.float()).abs() <= 2 ** -7 * b.float().abs() + 2 * 64 * 2 ** -24 * 32).all())
+    assert near(y[rows], yr) and near(z[rows], zr)
+    g = dz.to(H).expand(n, d)
+    dx, du = torch.autograd.grad(z, (xs, us), g)
+    rx, ru = torch.autograd.grad(zr, (xr, ur), g[:len(rows)])
+    for got, ref in ((dx[rows], rx), (du[rows], ru)):
+        assert float((got.float() - ref.float()).abs().max()) <= 2 ** -7 * float(ref.float().abs().max())
+
+
 def test_gated_ffn():
     from sca2_b200 import ops
     _room(60)

@@ -183,3 +183,15 @@ def test_training_step_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(ref, out):
         assert torch.equal(a, b)
+
+
+def test_vmap():
+    """Batched by torch.func.vmap: the registered operators, one call for each."""
+    from sca2_b200 import ops
+    torch.manual_seed(8)
+    x, u, w = torch.randn(3, 5, 64, device="cuda"), torch.randn(3, 5, 64, device="cuda"), torch.randn(64, device="cuda")
+    y, z = torch.func.vmap(lambda x, u: ops.residual_norm(x, u, w))(x, u)
+    ry, rz = ops.residual_norm(x, u, w)
+    assert torch.equal(y, ry) and torch.equal(z, rz)
+    xh, wh = x.bfloat16(), torch.randn(2, 32, 64, device="cuda").bfloat16()
+    assert torch.equal(torch.func.vmap(lambda x: ops.gated_ffn(x, wh[0], wh[1]))(xh), ops.gated_ffn(xh, wh[0], wh[1]))
