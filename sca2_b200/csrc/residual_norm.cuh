@@ -94,29 +94,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&p);
 }
 
-// ---- VEC values at consecutive columns (VEC = 8, 4: aligned) or one value -----------------------
+// ---- four values at consecutive columns (VEC = 4: aligned) or one ------------------------------
 template <int VEC>
 __device__ __forceinline__ void loadv(const float* p, float* v) {
   if constexpr (VEC == 1) {
     v[0] = *p;
   } else {
-#pragma unroll
-    for (int k = 0; k < VEC / 4; ++k) {
-      const float4 q = reinterpret_cast<const float4*>(p)[k];
-      v[4 * k] = q.x, v[4 * k + 1] = q.y, v[4 * k + 2] = q.z, v[4 * k + 3] = q.w;
-    }
+    const float4 q = *reinterpret_cast<const float4*>(p);
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
   }
 }
 template <int VEC>
 __device__ __forceinline__ void loadv(const __nv_bfloat16* p, float* v) {
   if constexpr (VEC == 1) {
     v[0] = __bfloat162float(*p);
-  } else if constexpr (VEC == 4) {
+  } else {
     const uint2 q = *reinterpret_cast<const uint2*>(p);
     unpack2(q.x, v), unpack2(q.y, v + 2);
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    unpack2(q.x, v), unpack2(q.y, v + 2), unpack2(q.z, v + 4), unpack2(q.w, v + 6);
   }
 }
 template <int VEC>
@@ -124,36 +118,19 @@ __device__ __forceinline__ void storev(float* p, const float* v) {
   if constexpr (VEC == 1) {
     *p = v[0];
   } else {
-#pragma unroll
-    for (int k = 0; k < VEC / 4; ++k)
-      reinterpret_cast<float4*>(p)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
 template <int VEC>
 __device__ __forceinline__ void storev(__nv_bfloat16* p, const float* v) {
   if constexpr (VEC == 1) {
     *p = __float2bfloat16_rn(v[0]);
-  } else if constexpr (VEC == 4) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
   } else {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
   }
-}
-template <int VEC>
-__device__ __forceinline__ void load_dt(const void* p, int64_t i, int dt, float* v) {
-  if (dt == SCA2_BF16) loadv<VEC>(reinterpret_cast<const __nv_bfloat16*>(p) + i, v);
-  else loadv<VEC>(reinterpret_cast<const float*>(p) + i, v);
-}
-template <int VEC>
-__device__ __forceinline__ void store_dt(void* p, int64_t i, int dt, const float* v) {
-  if (dt == SCA2_BF16) storev<VEC>(reinterpret_cast<__nv_bfloat16*>(p) + i, v);
-  else storev<VEC>(reinterpret_cast<float*>(p) + i, v);
 }
 
 // ---- forward --------------------------------------------------------------------------------
-// Wide or unaligned rows: the CTA owns a row, each thread NV groups of VEC values: group k of thread t
-// starts at column VEC (t + FT k).  Few registers, so that many CTAs hide each other's barriers.
 constexpr int FT = 256;
 
 __device__ __forceinline__ float row_sum(float v, int& flip) {
@@ -166,101 +143,6 @@ __device__ __forceinline__ float row_sum(float v, int& flip) {
   for (int w = 0; w < FT / 32; ++w) v += s[flip][w];
   flip ^= 1;  // the next sum's writes pass this one's reads only after its own barrier
   return v;
-}
-
-template <int NV, int VEC, class TX, class TU>
-__global__ void __launch_bounds__(FT, NV * VEC <= 4 ? 6 : NV * VEC <= 8 ? 4 : 3) fwd_kernel(const Args a) {
-  const int t = threadIdx.x;
-  const int d = a.d;
-  const float inv = 1.f / (float)d;
-  int flip = 0;
-  const auto col = [&](int k) { return VEC * (t + FT * k); };
-  // mean and 1 / deviation of v, then v <- (v - mean) / deviation
-  const auto normalise = [&](float (&v)[NV][VEC], float& mu, float& rs) {
-    mu = 0.f;
-    if (!a.rms) {
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += v[k][j];  // columns past d hold 0
-      mu = row_sum(s, flip) * inv;
-    }
-    float q = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (col(k) < d) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k][j] -= mu, q = fmaf(v[k][j], v[k][j], q);
-      }
-    rs = rsqrtf(row_sum(q, flip) * inv + a.eps);
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] *= rs;
-  };
-  const auto affine = [&](float (&v)[VEC], const float* w, const float* b, int c) {
-    float q[VEC];
-    loadv<VEC>(w + c, q);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] *= q[j];
-    if (b) {
-      loadv<VEC>(b + c, q);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] += q[j];
-    }
-  };
-
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const TX* xr = reinterpret_cast<const TX*>(a.x) + row * a.sx;
-    const TU* ur = reinterpret_cast<const TU*>(a.u) + row * a.su;
-    const TU* gr = reinterpret_cast<const TU*>(a.gate) + row * a.sg;
-    float x[NV][VEC], p[NV][VEC], g[NV][VEC];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[k][j] = p[k][j] = g[k][j] = 0.f;
-      if (col(k) < d) {
-        loadv<VEC>(ur + col(k), p[k]);
-        loadv<VEC>(xr + col(k), x[k]);
-        if (a.gate_mode == 2) loadv<VEC>(gr + col(k), g[k]);
-      }
-    }
-    float gt = 1.f;
-    if (a.gate_mode == 1) loadv<1>(gr, &gt), gt = sigmoid(gt);
-    float mu = 0.f, rs = 0.f;
-    if (a.pw) {
-      normalise(p, mu, rs);
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-        if (col(k) < d) affine(p[k], a.pw, a.pb, col(k));
-    }
-    if (a.stats && t == 0) a.stats[4 * row] = mu, a.stats[4 * row + 1] = rs;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (col(k) < d) {
-        float s[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[j] = 1.f;
-        if (a.scale) loadv<VEC>(a.scale + col(k), s);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if (a.gate_mode == 2) s[j] *= sigmoid(g[k][j]);
-          else s[j] *= gt;
-          x[k][j] = fmaf(s[j], p[k][j], x[k][j]);
-        }
-        storev<VEC>(reinterpret_cast<TX*>(a.y) + row * d + col(k), x[k]);
-      }
-    if (!a.z) continue;
-    normalise(x, mu, rs);
-    if (a.stats && t == 0) a.stats[4 * row + 2] = mu, a.stats[4 * row + 3] = rs;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (col(k) < d) {
-        affine(x[k], a.w, a.b, col(k));
-        store_dt<VEC>(a.z, row * d + col(k), a.zdt, x[k]);
-      }
-  }
 }
 
 // four consecutive values as two pairs
@@ -1101,16 +983,20 @@ __global__ void __launch_bounds__(BwdRing<C, GATE, HASZ, ANY, TX, TU>::MAXT, Bwd
 
 // Threads of a backward CTA: a row's groups of four columns, in warps; C = 2: half as many.
 inline int bwd_threads(int d, int c) { return ((d + 4 * c - 1) / (4 * c) + 31) / 32 * 32; }
-// `many`: rows from which bwd_ring, or two unaligned rows at a time, win (backward of 1184, 2368, 4736 rows,
-// few-row kernel against bwd_ring: d = 256 7.2 / 5.6, 12.1 / 7.7, 20.6 / 12.4 us; d = 768 8.5 / 12.4,
-// 13.8 / 16.1, 30.8 / 24.1; d = 1024 9.5 / 14.6, 16.4 / 21.1, 36.4 / 33.1).
-inline bool many(int64_t rows, int d) { return rows >= (d <= 1024 ? 4 * d : 2048); }
+// `many`: rows from which bwd_ring wins to 1024 values (backward of 1184, 2368, 4736 rows, bwd_kernel against
+// bwd_ring: d = 256 7.2 / 5.6, 12.1 / 7.7, 20.6 / 12.4 us; d = 768 8.5 / 12.4, 13.8 / 16.1, 30.8 / 24.1;
+// d = 1024 9.5 / 14.6, 16.4 / 21.1, 36.4 / 33.1; odd rows: d = 333 9.4 / 7.9, 16.1 / 12.6, 27.6 / 18.2;
+// d = 1001 13.3 / 19.8, 22.0 / 29.9, 49.8 / 49.0).
+inline bool many(int64_t rows, int d) { return d <= 1024 && rows >= 4 * d; }
+// The same for wider rows (592, 1184, 2368 rows of 1536 values 8.0 / 10.4, 13.0 / 14.8, 28.4 / 23.5 us; of 4096
+// 18.3 / 25.5, 40.0 / 37.5, 80.2 / 63.4; odd: 2368 and 4736 of 2001 55.2 / 61.9 and 113 / 111).
+inline bool many_wide(int64_t rows, int d, bool any) { return d > 1024 && rows >= (any ? 4096 : d > 2048 ? 1184 : 2048); }
 // The CTAs, each of which leaves one row of partials: two to an SM, more of narrow rows.
 inline int bwd_grid(int64_t rows, int d) {
   const bool m = many(rows, d);
   const int T = bwd_threads(d, 1);
   const int most = 148 * (d > 2048 ? 1 : d > 1024 ? 2 : m ? std::max(2, std::min(8, 512 / T)) : 3);
-  const int64_t want = m && d <= 1024 ? (rows + 1) / 2 : rows;
+  const int64_t want = m ? (rows + 1) / 2 : rows;
   return (int)(want < most ? want : most);
 }
 
@@ -1120,8 +1006,10 @@ cudaError_t fwd_ring_launch(const Args& a, cudaStream_t st) {
   const auto k = fwd_ring<NG, GATE, POST, ANY, TX, TU>;
   if (smem > 48 * 1024)
     if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  // the CTAs that run at once (444 where 296 fit, 49152 x 1024: 133 us, 121 so)
+  constexpr int most = 148 * std::min(3, 228 * 1024 / (smem + 1024));
   const int64_t want = (a.rows + 7) / 8;
-  k<<<(int)(want < 148 * 3 ? want : 148 * 3), FT, smem, st>>>(a);
+  k<<<(int)(want < most ? want : most), FT, smem, st>>>(a);
   return cudaGetLastError();
 }
 template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
@@ -1134,46 +1022,34 @@ cudaError_t fwd_wide_launch(const Args& a, cudaStream_t st) {
   k<<<(int)(a.rows < most ? a.rows : most), FT, smem, st>>>(a);
   return cudaGetLastError();
 }
+// A CTA a row (fwd_wide) for rows wider than fwd_ring takes, for odd rows from 513 values, and for few rows,
+// each by more threads (against fwd_ring, everything on: 1184 and 1776 rows of 256 values 5.5 / 4.7 and 7.2 /
+// 4.7 us, of 768 6.2 / 8.8 and 8.1 / 9.0; 64 rows 2.7 / 7.1).  Beyond 768 values fwd_ring's slots leave two
+// CTAs an SM, and few means more rows (3552, 7104, 10656 rows of 1024 values 15.0 / 21.0, 27.0 / 28.2,
+// 38.9 / 38.1 us; of 896 14.3 / 19.1, 26.1 / 26.1, 37.4 / 35.2).
+inline int few_rows(int d) { return 148 * (d > 768 ? 48 : 8); }
 template <int GATE, bool POST, bool ANY, class TX, class TU>
-cudaError_t fwd_ring_width(const Args& a, cudaStream_t st) {
-  if (a.d > 2048) return fwd_wide_launch<4, GATE, POST, ANY, TX, TU>(a, st);
-  if (a.d > 1024) return fwd_wide_launch<2, GATE, POST, ANY, TX, TU>(a, st);
-  if constexpr (ANY)
-    if (a.d > 512) return fwd_wide_launch<1, GATE, POST, ANY, TX, TU>(a, st);
-  switch ((a.d + 255) / 256) {
-    case 1: return fwd_ring_launch<2, GATE, POST, ANY, TX, TU>(a, st);
-    case 2: return fwd_ring_launch<4, GATE, POST, ANY, TX, TU>(a, st);
-    default: break;
-  }
-  if constexpr (ANY) return cudaErrorInvalidValue;  // not reached
-  else return a.d <= 768 ? fwd_ring_launch<6, GATE, POST, ANY, TX, TU>(a, st) : fwd_ring_launch<8, GATE, POST, ANY, TX, TU>(a, st);
+cudaError_t fwd_width(const Args& a, cudaStream_t st) {
+  const int d = a.d;
+  if (d > 2048) return fwd_wide_launch<4, GATE, POST, ANY, TX, TU>(a, st);
+  if (d > 1024) return fwd_wide_launch<2, GATE, POST, ANY, TX, TU>(a, st);
+  if (a.rows <= few_rows(d) || (ANY && d > 512)) return fwd_wide_launch<1, GATE, POST, ANY, TX, TU>(a, st);
+  if (d <= 256) return fwd_ring_launch<2, GATE, POST, ANY, TX, TU>(a, st);
+  if constexpr (!ANY)
+    if (d > 512) return d <= 768 ? fwd_ring_launch<6, GATE, POST, ANY, TX, TU>(a, st) : fwd_ring_launch<8, GATE, POST, ANY, TX, TU>(a, st);
+  return fwd_ring_launch<4, GATE, POST, ANY, TX, TU>(a, st);
 }
 template <bool ANY, class TX, class TU>
-cudaError_t fwd_ring_options(const Args& a, cudaStream_t st) {
+cudaError_t fwd_options(const Args& a, cudaStream_t st) {
   if (a.pw)
-    return a.gate_mode == 0 ? fwd_ring_width<0, true, ANY, TX, TU>(a, st)
-           : a.gate_mode == 1 ? fwd_ring_width<1, true, ANY, TX, TU>(a, st) : fwd_ring_width<2, true, ANY, TX, TU>(a, st);
-  return a.gate_mode == 0 ? fwd_ring_width<0, false, ANY, TX, TU>(a, st)
-         : a.gate_mode == 1 ? fwd_ring_width<1, false, ANY, TX, TU>(a, st) : fwd_ring_width<2, false, ANY, TX, TU>(a, st);
+    return a.gate_mode == 0 ? fwd_width<0, true, ANY, TX, TU>(a, st)
+           : a.gate_mode == 1 ? fwd_width<1, true, ANY, TX, TU>(a, st) : fwd_width<2, true, ANY, TX, TU>(a, st);
+  return a.gate_mode == 0 ? fwd_width<0, false, ANY, TX, TU>(a, st)
+         : a.gate_mode == 1 ? fwd_width<1, false, ANY, TX, TU>(a, st) : fwd_width<2, false, ANY, TX, TU>(a, st);
 }
-// Up to FEW_ROWS rows a CTA owns a row (fwd_kernel), all rows at once, each by more threads (64, 592,
-// 1184, 2368 rows of 768 values, against fwd_ring: 3.3 / 7.4, 4.1 / 7.6, 6.9 / 7.7, 11.1 / 9.5 us; of 1024:
-// 3.3 / 6.5, 4.3 / 6.7, 7.2 / 6.9, 11.9 / 9.6).  vec: rows and pointers allow groups of four values.
-constexpr int FEW_ROWS = 148 * 8;
 template <class TX, class TU>
 cudaError_t fwd_types(const Args& a, bool vec, cudaStream_t st) {
-  const int d = a.d;
-  if (a.rows > FEW_ROWS) return vec ? fwd_ring_options<false, TX, TU>(a, st) : fwd_ring_options<true, TX, TU>(a, st);
-  const int grid = (int)a.rows;
-  if (vec) {
-    if (d <= 1024) fwd_kernel<1, 4, TX, TU><<<grid, FT, 0, st>>>(a);
-    else if (d <= 2048) fwd_kernel<2, 4, TX, TU><<<grid, FT, 0, st>>>(a);
-    else fwd_kernel<4, 4, TX, TU><<<grid, FT, 0, st>>>(a);
-  } else {
-    if (d <= 1024) fwd_kernel<4, 1, TX, TU><<<grid, FT, 0, st>>>(a);
-    else fwd_kernel<16, 1, TX, TU><<<grid, FT, 0, st>>>(a);
-  }
-  return cudaGetLastError();
+  return vec ? fwd_options<false, TX, TU>(a, st) : fwd_options<true, TX, TU>(a, st);
 }
 
 constexpr int SMEM_MOST = 227 * 1024 - 2 * 3 * 16 * 4;  // a CTA's dynamic shared memory beside bwd_ring's sums
@@ -1204,7 +1080,7 @@ cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
   // rows near 4096 values with everything on and no type of 16 bits, or of any alignment, do not fit
   using L = BwdRing<2, 2, true, !CONTIG, TX, TU>;
   const bool fits = d <= 1024 || L::thread(L::z_bytes(a.zdt == SCA2_BF16)) * bwd_threads(d, 2) <= SMEM_MOST;
-  if (many(a.rows, d) && fits)
+  if ((many(a.rows, d) || many_wide(a.rows, d, !CONTIG)) && fits)
     return d <= 1024 ? bwd_ring_gate<1, !CONTIG, TX, TU>(a, st) : bwd_ring_gate<2, !CONTIG, TX, TU>(a, st);
   if (d > 2048) bwd_kernel<1024, 1, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
   else if (d > 1024) bwd_kernel<512, 2, CONTIG, TX, TU><<<grid, T, 0, st>>>(a);
