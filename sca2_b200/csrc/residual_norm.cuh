@@ -266,7 +266,7 @@ template <int NG, int GATE, bool ANY, class TX, class TU>
 struct FwdRing {  // bytes of a thread's group in each array; the arrays' slots lie thread by thread
   static constexpr int BU = GB<ANY, TU>, BX = GB<ANY, TX>, BG = GATE == 2 ? BU : 0;
   static constexpr int OX = NG * BU * FT, OG = OX + NG * BX * FT, OP = OG + NG * BG * FT;
-  static constexpr int D = NG * 128, BYTES = OP + 5 * D * 4;  // w, b, pw, pb, scale
+  static constexpr int D = NG * 128;  // floats of a parameter, from OP
 };
 
 template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
@@ -332,12 +332,14 @@ __global__ void __launch_bounds__(FT, 3) fwd_ring(const Args a) {
 
   fetch_u(row), fetch_x(row);
   float* par = reinterpret_cast<float*>(slots + L::OP);
-  const auto stage = [&](int i, const float* p) -> const float* {
+  const auto stage = [&](const float* p) -> const float* {
     if (!p) return nullptr;
-    for (int c = threadIdx.x; c < L::D; c += FT) par[i * L::D + c] = c < d ? p[c] : 0.f;
-    return par + i * L::D;
+    float* q = par;
+    for (int c = threadIdx.x; c < L::D; c += FT) q[c] = c < d ? p[c] : 0.f;
+    par += L::D;
+    return q;
   };
-  const float *w = stage(0, a.w), *b = stage(1, a.b), *pw = stage(2, a.pw), *pb = stage(3, a.pb), *scale = stage(4, a.scale);
+  const float *w = stage(a.w), *b = stage(a.b), *pw = stage(a.pw), *pb = stage(a.pb), *scale = stage(a.scale);
   __syncthreads();
   for (; row < a.rows; row += step) {
     float gt = 1.f;
@@ -1002,12 +1004,15 @@ inline int bwd_grid(int64_t rows, int d) {
 
 template <int NG, int GATE, bool POST, bool ANY, class TX, class TU>
 cudaError_t fwd_ring_launch(const Args& a, cudaStream_t st) {
-  constexpr int smem = FwdRing<NG, GATE, ANY, TX, TU>::BYTES;
+  using L = FwdRing<NG, GATE, ANY, TX, TU>;
+  int params = 0;
+  for (const float* p : {a.w, a.b, a.pw, a.pb, a.scale}) params += p != nullptr;
+  const int smem = L::OP + params * L::D * 4;
   const auto k = fwd_ring<NG, GATE, POST, ANY, TX, TU>;
   if (smem > 48 * 1024)
     if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
   // the CTAs that run at once (444 where 296 fit, 49152 x 1024: 133 us, 121 so)
-  constexpr int most = 148 * std::min(3, 228 * 1024 / (smem + 1024));
+  const int most = 148 * std::min(3, 228 * 1024 / (smem + 1024));
   const int64_t want = (a.rows + 7) / 8;
   k<<<(int)(want < most ? want : most), FT, smem, st>>>(a);
   return cudaGetLastError();
