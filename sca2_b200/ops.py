@@ -1403,9 +1403,12 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _traced(x: torch.Tensor) -> bool:
-    """Whether a call goes through the registered operator (tracing, fake and other tensor subclasses,
-    vmap's batched tensors) rather than straight to the library."""
-    return torch.compiler.is_compiling() or type(x) not in _PLAIN or torch._C._are_functorch_transforms_active()
+    """Whether a call goes through the registered operator (compilation, traces and other dispatch modes,
+    function transforms, fake and other tensor subclasses) rather than straight to the library, where
+    none of them would see it."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._are_functorch_transforms_active() or torch._C._get_tracing_state() is not None
+            or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0 or type(x) not in _PLAIN)
 
 
 def _tied(t: Optional[torch.Tensor]):
@@ -1429,6 +1432,8 @@ class _GatedFFN(torch.autograd.Function):
 
     @staticmethod
     def grads(ctx, dh):
+        if _traced(dh):
+            return _gated_ffn_backward(ctx, dh)
         need = ctx.needs_input_grad
         x, wg, wu = ctx.saved_tensors
         return (*_gated_ffn_bwd_run(x, wg, wu, ctx.act, dh, need[0], need[1] or need[2]), None)
@@ -1570,10 +1575,10 @@ def _residual_norm_setup(ctx, inputs, output):
 
 
 def _residual_norm_backward(ctx, dy, dz, _dstats):
-    x, u, w, b, gate, scale, pw, pb, stats = ctx.saved_tensors
-    out = torch.ops.sca2b200.residual_norm_bwd(x, u, w, b, gate, scale, pw, pb, ctx.kind, ctx.eps, ctx.zdt, stats, dy,
-                                               dz if w is not None else None)
-    return (*[None if t is None else g for t, g in zip((x, u, w, b, gate, scale, pw, pb), out)], None, None, None, None)
+    *ins, stats = ctx.saved_tensors
+    out = torch.ops.sca2b200.residual_norm_bwd(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy,
+                                               dz if ins[2] is not None else None)
+    return (*[None if t is None else g for t, g in zip(ins, out)], None, None, None, None)
 
 
 _residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
@@ -1586,7 +1591,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
         y, z, stats = _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, True)
         ctx.save_for_backward(x, u, w, b, gate, scale, pw, pb, stats)
-        ctx.opts = kind, eps, zdt
+        ctx.kind, ctx.eps, ctx.zdt = kind, eps, zdt
         ctx.set_materialize_grads(False)
         return y, z
 
@@ -1598,8 +1603,10 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def grads(ctx, dy, dz):
+        if _traced(dz if dy is None else dy):
+            return _residual_norm_backward(ctx, dy, dz, None)[:11]
         *ins, stats = ctx.saved_tensors
-        return (*_residual_norm_bwd_run(*ins, *ctx.opts, stats, dy, dz if ins[2] is not None else None),
+        return (*_residual_norm_bwd_run(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy, dz if ins[2] is not None else None),
                 None, None, None)
 
     once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
@@ -1665,9 +1672,7 @@ _T = torch.Tensor
 
 def _grad_list(what: str, grads, out=None):
     """The call's tensors, the types of the gradients and of the destinations, and the device."""
-    grads = [grads] if isinstance(grads, _T) else list(grads)
-    outs = grads if out is None else ([out] if isinstance(out, _T) else list(out))
-    E = _lib.Sca2Error
+    outs, E = grads if out is None else out, _lib.Sca2Error
     if len(outs) != len(grads):
         raise E(f"{what}: {len(grads)} gradients and {len(outs)} destinations")
     dev, types = None, []
@@ -1688,12 +1693,17 @@ def _grad_list(what: str, grads, out=None):
     return grads, outs, types, dev
 
 
+def _same_sizes(numel, dst):
+    if list(map(_T.numel, dst)) != numel:
+        raise _lib.Sca2Error("clip_grads: a destination must have as many values as its gradient")
+
+
 def _grad_table(src, dst, types):
     """The sca2_grad_tensor list as bytes (host memory; the library copies it into the launch).  A
     destination has its gradient's number of values."""
     n, numel = len(src), list(map(_T.numel, src))
-    if dst is not src and list(map(_T.numel, dst)) != numel:
-        raise _lib.Sca2Error("clip_grads: a destination must have its gradient's shape")
+    if dst is not src:
+        _same_sizes(numel, dst)
     codes = [[_DT[t[0]]] * n if len(set(t)) == 1 else [_DT[x] for x in t] for t in types]
     flat = [0] * (5 * n)
     flat[0::5] = ptrs = list(map(_T.data_ptr, src))
@@ -1761,15 +1771,30 @@ def _(grads, max_norm):
     return grads[0].new_empty((), dtype=torch.float32)
 
 
+@torch.library.custom_op("sca2b200::clip_grads_out", mutates_args=("out",))
+def _clip_grads_out_op(grads: Sequence[torch.Tensor], out: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """sca2_clip_grads of a list of tensors into another; returns the norm before."""
+    grads, outs, types, dev = _grad_list("clip_grads", grads, out)
+    return _clip_run(grads, outs, types, max_norm, dev)
+
+
+@_clip_grads_out_op.register_fake
+def _(grads, out, max_norm):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
 def grad_norm(grads) -> torch.Tensor:
     """2-norm of all values of the tensors together (fp32 scalar on their device; summed in 64 bits
     in a fixed order).  grads: a tensor or a list of float32 / bfloat16 tensors on one device; no
     tensor gives 0 (on the current CUDA device).  Not differentiable."""
-    if torch.compiler.is_compiling():
-        return torch.ops.sca2b200.grad_norm([grads] if isinstance(grads, _T) else list(grads))
-    grads, outs, types, dev = _grad_list("grad_norm", grads)
+    grads = [grads] if isinstance(grads, _T) else list(grads)
     if not grads:
         return torch.zeros((), device="cuda")
+    if torch.compiler.is_compiling():
+        return torch.ops.sca2b200.grad_norm(grads)
+    grads, outs, types, dev = _grad_list("grad_norm", grads)
+    if _traced(grads[0]):
+        return torch.ops.sca2b200.grad_norm(grads)
     with torch.no_grad():
         return _clip_run(grads, outs, types, None, dev)
 
@@ -1784,11 +1809,19 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise _lib.Sca2Error("clip_grads: max_norm must be >= 0")
-    if torch.compiler.is_compiling() and out is None:
-        return torch.ops.sca2b200.clip_grads_([grads] if isinstance(grads, _T) else list(grads), max_norm)
-    grads, outs, types, dev = _grad_list("clip_grads", grads, out)
-    if not grads:
+    grads = [grads] if isinstance(grads, _T) else list(grads)
+    out = out if out is None else [out] if isinstance(out, _T) else list(out)
+    if not grads and not out:
         return torch.zeros((), device="cuda")
+    compiling = torch.compiler.is_compiling()
+    if not compiling:
+        grads, outs, types, dev = _grad_list("clip_grads", grads, out)
+    if compiling or _traced(grads[0]):
+        if out is None:
+            return torch.ops.sca2b200.clip_grads_(grads, max_norm)
+        if not compiling:  # else found out by the operator
+            _same_sizes([g.numel() for g in grads], out)
+        return torch.ops.sca2b200.clip_grads_out(grads, out, max_norm)
     with torch.no_grad():
         norm = _clip_run(grads, outs, types, max_norm, dev)
     try:

@@ -1,0 +1,99 @@
+"""The block operators and the clip as torch's transformations meet them, without a GPU: what a trace
+records, what batching keeps for the backward, what is refused.  The launches are stubbed (they write
+nothing), so only structure is compared, never values."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from sca2_b200 import ops
+
+H = torch.bfloat16
+
+
+@pytest.fixture
+def stub(monkeypatch):
+    """CPU tensors pass for CUDA ones and every launch is recorded instead of made."""
+    calls = []
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: torch.device("cuda", 0))
+    monkeypatch.setattr(ops, "_launch", lambda what, fn, dev, *args: calls.append((what, args)))
+    return calls
+
+
+def _ffn(grad=False):
+    return [torch.zeros(s, dtype=H).requires_grad_(grad) for s in ((4, 16), (24, 16), (24, 16))]
+
+
+def _norm(grad=False):
+    return [torch.zeros(s).requires_grad_(grad) for s in ((4, 16), (4, 16), (16,))]
+
+
+def _targets(gm):
+    return [str(n.target) for n in gm.graph.nodes if n.op == "call_function"]
+
+
+def _grads(f, outs):
+    def g(*args):
+        o = f(*args)
+        return torch.autograd.grad(o, args, torch.ones_like(o))
+    return g
+
+
+# (function, its tensors, the operators that its trace has to hold)
+CASES = {
+    "ffn": (lambda x, g, u: ops.gated_ffn(x, g, u), _ffn, ["gated_ffn_fwd"]),
+    "norm": (lambda x, u, w: ops.residual_norm(x, u, w)[1], _norm, ["residual_norm_fwd"]),
+    "grad_norm": (lambda x, u, w: ops.grad_norm([x, u, w]), _norm, ["grad_norm"]),
+    "clip": (lambda x, u, w: ops.clip_grads([x, u, w], 1.0), _norm, ["clip_grads_"]),
+    "clip_out": (lambda x, u, w: ops.clip_grads([x], 1.0, out=[u]), _norm, ["clip_grads_out"]),
+}
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(pre_dispatch=True), dict(tracing_mode="fake"), dict(tracing_mode="symbolic")],
+                         ids=lambda k: "-".join(map(str, k.values())) or "real")
+@pytest.mark.parametrize("case", CASES)
+def test_make_fx_records_the_operators(stub, case, kw):
+    f, ins, want = CASES[case]
+    got = _targets(make_fx(f, **kw)(*ins()))
+    assert all(any(f"sca2b200.{w}.default" in t for t in got) for w in want), got
+
+
+@pytest.mark.parametrize("case", ["ffn", "norm"])
+def test_make_fx_records_the_gradients(stub, case):
+    f, ins, want = CASES[case]
+    got = _targets(make_fx(_grads(f, 1))(*ins(True)))
+    for w in (want[0], want[0].replace("fwd", "bwd")):
+        assert any(f"sca2b200.{w}.default" in t for t in got), got
+    leaves = ins(True)  # a graph made outside of the trace
+    out = f(*leaves)
+    got = _targets(make_fx(lambda d: torch.autograd.grad(out, leaves, d, retain_graph=True))(torch.ones_like(out)))
+    assert any(f"sca2b200.{want[0].replace('fwd', 'bwd')}.default" in t for t in got), got
+
+
+@pytest.mark.parametrize("case", CASES)
+@pytest.mark.filterwarnings("ignore")
+def test_jit_trace_records_the_operators(stub, case):
+    f, ins, want = CASES[case]
+    assert f"sca2b200::{want[0]}" in str(torch.jit.trace(f, ins(), check_trace=False).graph)
+
+
+def test_dispatch_modes_see_the_operators(stub):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.ops.append(str(func))
+            return func(*args, **(kwargs or {}))
+    for f, ins, want in CASES.values():
+        with Seen() as seen:
+            f(*ins())
+        assert all(f"sca2b200.{w}.default" in seen.ops for w in want), seen.ops
+
+
+def test_plain_calls_go_straight_to_the_library(stub):
+    for f, ins, _ in CASES.values():
+        f(*ins())
+    assert [w for w, _ in stub] == ["gated_ffn", "residual_norm", "grad_norm", "clip_grads", "clip_grads"]

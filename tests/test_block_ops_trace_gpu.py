@@ -1,0 +1,74 @@
+"""The block operators and the clip in traces, run: graphs recorded by make_fx, torch.jit.trace and
+torch.compile give what the eager calls give, bit for bit (the same kernels on the same values)."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+pytestmark = pytest.mark.gpu
+H = torch.bfloat16
+
+
+def _randn(*s, seed=0, grad=False, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(s))
+    return torch.randn(*s, device="cuda", generator=g).to(dtype).requires_grad_(grad)
+
+
+def _ffn():
+    return [_randn(*s, seed=k, grad=True, dtype=H) for k, s in enumerate([(70, 64), (72, 64), (72, 64)])]
+
+
+def _norm():
+    return [_randn(*s, seed=k, grad=True) for k, s in enumerate([(70, 64), (70, 64), (64,), (70, 1)])]
+
+
+def _both(f, ins):
+    o = f(*ins)
+    return (o.detach(), *torch.autograd.grad(o, ins, torch.ones_like(o)))
+
+
+def _block(kind):
+    from sca2_b200 import ops
+    if kind == "ffn":
+        return (lambda x, g, u: ops.gated_ffn(x, g, u)), _ffn()
+    return (lambda x, u, w, g: ops.residual_norm(x, u, w, gate=g, post_weight=w)[1]), _norm()
+
+
+@pytest.mark.parametrize("mode", ["real", "fake"])
+@pytest.mark.parametrize("kind", ["ffn", "norm"])
+def test_make_fx(kind, mode):
+    f, ins = _block(kind)
+    ref = _both(f, ins)
+    gm = make_fx(lambda *t: _both(f, t), tracing_mode=mode)(*ins)
+    assert all(torch.equal(a, b) for a, b in zip(ref, gm(*ins)))
+    new = [t.detach() * 0.5 for t in ins]  # other values than those of the trace
+    ref = _both(f, [t.clone().requires_grad_(True) for t in new])
+    assert all(torch.equal(a, b) for a, b in zip(ref, gm(*new)))
+
+
+@pytest.mark.parametrize("kind", ["ffn", "norm"])
+@pytest.mark.filterwarnings("ignore")
+def test_jit_trace(kind):
+    f, ins = _block(kind)
+    t = torch.jit.trace(f, [i.detach() for i in ins], check_trace=False)
+    new = [i.detach() * 0.5 for i in ins]
+    assert torch.equal(t(*new), f(*new))
+
+
+def test_clip_in_a_trace():
+    from sca2_b200 import ops
+    src = lambda: [_randn(40), _randn(3, 5, dtype=H)]
+    a, b = src()
+    n = ops.clip_grads([a, b], 0.1)
+    norm = ops.grad_norm(src())
+    gm = make_fx(lambda x, y: ops.clip_grads([x, y], 0.1))(*src())
+    x, y = src()
+    assert torch.equal(gm(x, y), n) and torch.equal(x, a) and torch.equal(y, b)
+    assert torch.equal(make_fx(lambda x, y: ops.grad_norm([x, y]))(*src())(*src()), norm)
+    into = lambda x, y, p, q: ops.clip_grads([x, y], 0.1, out=[p, q])
+    for g in (make_fx(into)(*src(), torch.empty(40, device="cuda"), torch.empty(3, 5, device="cuda")),
+              torch.compile(into, fullgraph=True, backend="aot_eager")):
+        p, q = torch.zeros(40, device="cuda"), torch.zeros(3, 5, device="cuda", dtype=H)
+        assert torch.equal(g(*src(), p, q), n) and torch.equal(p, a) and torch.equal(q, b)
+    empty = torch.compile(lambda x: x + ops.clip_grads([], 1.0) + ops.grad_norm([]), fullgraph=True, backend="aot_eager")
+    assert torch.equal(empty(norm), norm)
+    torch.library.opcheck(torch.ops.sca2b200.clip_grads_out, (src(), [torch.zeros(40, device="cuda"), torch.zeros(3, 5, device="cuda")], 0.1))
