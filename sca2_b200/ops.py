@@ -1399,16 +1399,16 @@ def _gated_ffn_backward(ctx, dh):
 _gated_ffn_fwd.register_autograd(_gated_ffn_backward, setup_context=_gated_ffn_setup)
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
-def _traced(x: torch.Tensor) -> bool:
+def _traced(*ts) -> bool:
     """Whether a call goes through the registered operator (compilation, traces and other dispatch modes,
     function transforms, fake and other tensor subclasses) rather than straight to the library, where
     none of them would see it."""
     return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
             or torch._C._are_functorch_transforms_active() or torch._C._get_tracing_state() is not None
-            or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0 or type(x) not in _PLAIN)
+            or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0 or not _PLAIN.issuperset(map(type, ts)))
 
 
 def _tied(t: Optional[torch.Tensor]):
@@ -1432,10 +1432,10 @@ class _GatedFFN(torch.autograd.Function):
 
     @staticmethod
     def grads(ctx, dh):
-        if _traced(dh):
+        x, wg, wu = ctx.saved_tensors
+        if _traced(x, wg, wu, dh):
             return _gated_ffn_backward(ctx, dh)
         need = ctx.needs_input_grad
-        x, wg, wu = ctx.saved_tensors
         return (*_gated_ffn_bwd_run(x, wg, wu, ctx.act, dh, need[0], need[1] or need[2]), None)
 
     once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
@@ -1464,7 +1464,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
                 f"{tuple(w_up.shape)}")
     if not gated_ffn_supported(shape[1], shape[0]):
         raise E(f"gated_ffn: d and f must be multiples of 8, got {shape[1]} and {shape[0]}")
-    if _traced(x):
+    if _traced(x, w_gate, w_up):
         return torch.ops.sca2b200.gated_ffn_fwd(x, w_gate, w_up, _ACT[act])
     if _wants_grad(x, w_gate, w_up):
         return _GatedFFN.apply(x, w_gate, w_up, _ACT[act])
@@ -1603,9 +1603,9 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def grads(ctx, dy, dz):
-        if _traced(dz if dy is None else dy):
-            return _residual_norm_backward(ctx, dy, dz, None)[:11]
         *ins, stats = ctx.saved_tensors
+        if _traced(*ins, stats, dy, dz):
+            return _residual_norm_backward(ctx, dy, dz, None)[:11]
         return (*_residual_norm_bwd_run(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy, dz if ins[2] is not None else None),
                 None, None, None)
 
@@ -1653,7 +1653,7 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
         gate = gate.to(u.dtype)
     w, b, sc, pw, pb = par
     kid, eps = _NORM_KIND[kind], float(eps)
-    if _traced(x):
+    if _traced(x, u, w, b, gate, sc, pw, pb):
         y, z, _ = torch.ops.sca2b200.residual_norm_fwd(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt,
                                                        _wants_grad(x, u, w, b, gate, sc, pw, pb))
     elif _wants_grad(x, u, w, b, gate, sc, pw, pb):
@@ -1793,7 +1793,7 @@ def grad_norm(grads) -> torch.Tensor:
     if torch.compiler.is_compiling():
         return torch.ops.sca2b200.grad_norm(grads)
     grads, outs, types, dev = _grad_list("grad_norm", grads)
-    if _traced(grads[0]):
+    if _traced(*grads):
         return torch.ops.sca2b200.grad_norm(grads)
     with torch.no_grad():
         return _clip_run(grads, outs, types, None, dev)
@@ -1816,7 +1816,7 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     compiling = torch.compiler.is_compiling()
     if not compiling:
         grads, outs, types, dev = _grad_list("clip_grads", grads, out)
-    if compiling or _traced(grads[0]):
+    if compiling or _traced(*grads, *outs):
         if out is None:
             return torch.ops.sca2b200.clip_grads_(grads, max_norm)
         if not compiling:  # else found out by the operator

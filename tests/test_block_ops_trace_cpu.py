@@ -97,3 +97,47 @@ def test_plain_calls_go_straight_to_the_library(stub):
     for f, ins, _ in CASES.values():
         f(*ins())
     assert [w for w, _ in stub] == ["gated_ffn", "residual_norm", "grad_norm", "clip_grads", "clip_grads"]
+
+
+class Seen(torch.Tensor):
+    """A tensor that notes the operators it meets."""
+    ops = []
+
+    @staticmethod
+    def __new__(cls, t):
+        r = torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device, requires_grad=t.requires_grad)
+        r.inner = t.detach()
+        return r
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        cls.ops.append(str(func))
+        un = lambda t: t.inner if isinstance(t, cls) else [un(i) for i in t] if isinstance(t, (list, tuple)) else t
+        return func(*[un(a) for a in args], **{k: un(v) for k, v in (kwargs or {}).items()})
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_any_tensor_of_a_subclass_brings_the_operators(stub, case):
+    f, ins, want = CASES[case]
+    for k in range({"clip_out": 2}.get(case, 3)):
+        Seen.ops = []
+        f(*[Seen(t) if j == k else t for j, t in enumerate(ins())])
+        assert f"sca2b200.{want[0]}.default" in Seen.ops, k
+    if case in ("ffn", "norm"):  # a gradient of a subclass that reaches a plain graph
+        leaves = ins(True)
+        out = f(*leaves)
+        Seen.ops = []
+        torch.autograd.grad(out, leaves, Seen(torch.ones_like(out)))
+        assert f"sca2b200.{want[0].replace('fwd', 'bwd')}.default" in Seen.ops
+
+
+def test_fake_weights_beside_plain_inputs(stub):
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    mode = FakeTensorMode(allow_non_fake_inputs=True)
+    x, w, _ = _ffn()
+    assert isinstance(ops.gated_ffn(x, mode.from_tensor(w), w), FakeTensor)
+    x, u, w = _norm()
+    y, z = ops.residual_norm(x, u, mode.from_tensor(w))
+    assert isinstance(y, FakeTensor) and isinstance(z, FakeTensor)
+    assert isinstance(ops.clip_grads([x, mode.from_tensor(u)], 1.0), FakeTensor)
+    assert not stub
