@@ -1479,7 +1479,9 @@ _NORM_KIND = {"layer": 0, "rms": 1}
 
 def _row_view(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
     """t (..., d) as rows of contiguous values with one row stride (a copy only where its strides
-    do not allow that), and the stride."""
+    do not allow that, or torch keeps it lazily negated), and the stride."""
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t, d
     if t.stride(-1) == 1 or d == 1:
@@ -1648,6 +1650,8 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
                 raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
             if t.dtype != torch.float32 or not t.is_contiguous():
                 t = t.float().contiguous()
+            if d == 1 and not torch.compiler.is_compiling():  # one value needs no copy for its strides
+                t = t.resolve_neg()
         par.append(t)
     if gate is not None and gate.dtype != u.dtype:
         gate = gate.to(u.dtype)
@@ -1688,8 +1692,11 @@ def _grad_list(what: str, grads, out=None):
         if ts and (len(devs) != 1 or min(devs) < 0 or dev not in (None, *devs)):
             devs = {_need_cuda(*grads, *outs).index}
         dev = devs.pop() if devs else None
-    if out is not None and not all(map(_T.is_contiguous, outs)):
-        raise E(f"{what}: a destination must be contiguous")
+    if out is not None:
+        if not all(map(_T.is_contiguous, outs)) or any(map(_T.is_neg, outs)):
+            raise E(f"{what}: a destination must be contiguous")
+        if any(map(_T.is_neg, grads)):
+            grads = list(map(_T.resolve_neg, grads))
     return grads, outs, types, dev
 
 
