@@ -26,6 +26,7 @@ import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
+import torch.autograd.forward_ad as _fw
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -1411,6 +1412,12 @@ def _traced(*ts) -> bool:
             or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0 or not _PLAIN.issuperset(map(type, ts)))
 
 
+def _no_tangents(what: str, *ts):
+    """Refuse forward-mode derivatives: neither the library nor a registered operator carries them."""
+    if _fw._current_level >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None for t in ts):
+        raise _lib.Sca2Error(f"{what}: forward-mode differentiation is not supported")
+
+
 def _tied(t: Optional[torch.Tensor]):
     """An upstream gradient that requires one itself: what once_differentiable makes of it then raises
     when it is differentiated, where it would otherwise count as constant."""
@@ -1433,6 +1440,7 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def grads(ctx, dh):
         x, wg, wu = ctx.saved_tensors
+        _no_tangents("gated_ffn", x, wg, wu, dh)
         if _traced(x, wg, wu, dh):
             return _gated_ffn_backward(ctx, dh)
         need = ctx.needs_input_grad
@@ -1453,6 +1461,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
     Differentiable once in all three; the backward recomputes the projections, so nothing but the
     inputs is kept.  The weights may be the halves of one (2 f, d) tensor."""
     _device_of(x, w_gate, w_up)
+    _no_tangents("gated_ffn", x, w_gate, w_up)
     E = _lib.Sca2Error
     if act not in _ACT:
         raise E(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
@@ -1606,6 +1615,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def grads(ctx, dy, dz):
         *ins, stats = ctx.saved_tensors
+        _no_tangents("residual_norm", *ins, dy, dz)
         if _traced(*ins, stats, dy, dz):
             return _residual_norm_backward(ctx, dy, dz, None)[:11]
         return (*_residual_norm_bwd_run(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy, dz if ins[2] is not None else None),
@@ -1630,6 +1640,7 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
     (LayerNorm) or "rms" (no bias), for both norms.  y has x's type, z out_dtype (default: x's);
     arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
     _device_of(x, u, weight, bias, gate, scale, post_weight, post_bias)
+    _no_tangents("residual_norm", x, u, weight, bias, gate, scale, post_weight, post_bias)
     E, shape = _lib.Sca2Error, x.shape
     d = shape[-1] if shape else 0
     if kind not in _NORM_KIND:

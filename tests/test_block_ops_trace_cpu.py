@@ -141,3 +141,29 @@ def test_fake_weights_beside_plain_inputs(stub):
     assert isinstance(y, FakeTensor) and isinstance(z, FakeTensor)
     assert isinstance(ops.clip_grads([x, mode.from_tensor(u)], 1.0), FakeTensor)
     assert not stub
+
+
+@pytest.mark.parametrize("case", ["ffn", "norm"])
+def test_forward_mode_is_refused(stub, case):
+    """A tangent would be lost without a word, in either pass."""
+    import torch.autograd.forward_ad as fw
+    f, ins, _ = CASES[case]
+    refused = lambda: pytest.raises(ops._lib.Sca2Error, match="forward")
+    for k in range(3):
+        with fw.dual_level(), refused():
+            f(*[fw.make_dual(t, torch.ones_like(t)) if j == k else t for j, t in enumerate(ins())])
+        plain = ins()
+        one = lambda t, k=k: f(*[t if j == k else o for j, o in enumerate(plain)])
+        x = plain[k]
+        for call in (lambda: torch.func.jvp(one, (x,), (x,)), lambda: torch.func.jacfwd(one)(x),
+                     lambda: torch.func.jvp(lambda t: torch.func.vmap(lambda s: one(t))(torch.zeros(2)), (x,), (x,))):
+            with refused():
+                call()
+        with pytest.raises(RuntimeError):  # torch.func.grad itself does not take registered operators
+            torch.func.jvp(torch.func.grad(lambda t: one(t).float().sum()), (x,), (x,))
+    leaves = ins(True)
+    out = f(*leaves)
+    with fw.dual_level(), refused():
+        torch.autograd.grad(out, leaves, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    with fw.dual_level():  # without a tangent a level costs nothing
+        f(*ins())
