@@ -1401,15 +1401,16 @@ _gated_ffn_fwd.register_autograd(_gated_ffn_backward, setup_context=_gated_ffn_s
 
 
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+_is_compiling, _transforms, _jit_trace = torch.compiler.is_compiling, torch._C._are_functorch_transforms_active, torch._C._get_tracing_state
+_modes, _modes_before = torch._C._len_torch_dispatch_stack, torch._ops._len_torch_dispatch_stack_pre_dispatch
 
 
 def _traced(*ts) -> bool:
     """Whether a call goes through the registered operator (compilation, traces and other dispatch modes,
     function transforms, fake and other tensor subclasses) rather than straight to the library, where
     none of them would see it."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._are_functorch_transforms_active() or torch._C._get_tracing_state() is not None
-            or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0 or not _PLAIN.issuperset(map(type, ts)))
+    return (_is_compiling() or _modes() > 0 or _transforms() or _jit_trace() is not None or _modes_before() > 0
+            or not _PLAIN.issuperset(map(type, ts)))
 
 
 def _no_tangents(what: str, *ts):
@@ -1441,7 +1442,7 @@ class _GatedFFN(torch.autograd.Function):
     def grads(ctx, dh):
         x, wg, wu = ctx.saved_tensors
         _no_tangents("gated_ffn", x, wg, wu, dh)
-        if _traced(x, wg, wu, dh):
+        if _traced(dh):  # what was saved is plain
             return _gated_ffn_backward(ctx, dh)
         need = ctx.needs_input_grad
         return (*_gated_ffn_bwd_run(x, wg, wu, ctx.act, dh, need[0], need[1] or need[2]), None)
@@ -1489,7 +1490,7 @@ _NORM_KIND = {"layer": 0, "rms": 1}
 def _row_view(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
     """t (..., d) as rows of contiguous values with one row stride (a copy only where its strides
     do not allow that, or torch keeps it lazily negated), and the stride."""
-    if t.is_neg():
+    if d == 1 and t.is_neg():  # wider views of that kind are not contiguous
         t = t.resolve_neg()
     if t.is_contiguous():
         return t, d
@@ -1585,11 +1586,14 @@ def _residual_norm_setup(ctx, inputs, output):
     ctx.save_for_backward(x, u, w, b, gate, scale, pw, pb, output[2])
 
 
+def _residual_norm_op_grads(ins, kind, eps, zdt, stats, dy, dz):
+    out = torch.ops.sca2b200.residual_norm_bwd(*ins, kind, eps, zdt, stats, dy, dz if ins[2] is not None else None)
+    return [None if t is None else g for t, g in zip(ins, out)]
+
+
 def _residual_norm_backward(ctx, dy, dz, _dstats):
     *ins, stats = ctx.saved_tensors
-    out = torch.ops.sca2b200.residual_norm_bwd(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy,
-                                               dz if ins[2] is not None else None)
-    return (*[None if t is None else g for t, g in zip(ins, out)], None, None, None, None)
+    return (*_residual_norm_op_grads(ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy, dz), None, None, None, None)
 
 
 _residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
@@ -1602,7 +1606,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, u, w, b, gate, scale, pw, pb, kind, eps, zdt):
         y, z, stats = _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, True)
         ctx.save_for_backward(x, u, w, b, gate, scale, pw, pb, stats)
-        ctx.kind, ctx.eps, ctx.zdt = kind, eps, zdt
+        ctx.opts = kind, eps, zdt
         ctx.set_materialize_grads(False)
         return y, z
 
@@ -1616,9 +1620,9 @@ class _ResidualNorm(torch.autograd.Function):
     def grads(ctx, dy, dz):
         *ins, stats = ctx.saved_tensors
         _no_tangents("residual_norm", *ins, dy, dz)
-        if _traced(*ins, stats, dy, dz):
-            return _residual_norm_backward(ctx, dy, dz, None)[:11]
-        return (*_residual_norm_bwd_run(*ins, ctx.kind, ctx.eps, ctx.zdt, stats, dy, dz if ins[2] is not None else None),
+        if _traced(dy, dz):  # what was saved is plain
+            return (*_residual_norm_op_grads(ins, *ctx.opts, stats, dy, dz), None, None, None)
+        return (*_residual_norm_bwd_run(*ins, *ctx.opts, stats, dy, dz if ins[2] is not None else None),
                 None, None, None)
 
     once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
@@ -1704,10 +1708,8 @@ def _grad_list(what: str, grads, out=None):
             devs = {_need_cuda(*grads, *outs).index}
         dev = devs.pop() if devs else None
     if out is not None:
-        if not all(map(_T.is_contiguous, outs)) or any(map(_T.is_neg, outs)):
+        if not all(map(_T.is_contiguous, outs)):
             raise E(f"{what}: a destination must be contiguous")
-        if any(map(_T.is_neg, grads)):
-            grads = list(map(_T.resolve_neg, grads))
     return grads, outs, types, dev
 
 
@@ -1722,6 +1724,10 @@ def _grad_table(src, dst, types):
     n, numel = len(src), list(map(_T.numel, src))
     if dst is not src:
         _same_sizes(numel, dst)
+        if 1 in numel:  # lazily negated tensors that count as contiguous
+            if any(t.is_neg() for t, k in zip(dst, numel) if k == 1):
+                raise _lib.Sca2Error("clip_grads: a destination must be contiguous")
+            src[:] = [t.resolve_neg() if k == 1 else t for t, k in zip(src, numel)]
     codes = [[_DT[t[0]]] * n if len(set(t)) == 1 else [_DT[x] for x in t] for t in types]
     flat = [0] * (5 * n)
     flat[0::5] = ptrs = list(map(_T.data_ptr, src))
@@ -1834,7 +1840,7 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     compiling = torch.compiler.is_compiling()
     if not compiling:
         grads, outs, types, dev = _grad_list("clip_grads", grads, out)
-    if compiling or _traced(*grads, *outs):
+    if compiling or _traced(*grads, *(out or ())):
         if out is None:
             return torch.ops.sca2b200.clip_grads_(grads, max_norm)
         if not compiling:  # else found out by the operator
