@@ -1673,8 +1673,9 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
     w, b, sc, pw, pb = par
     kid, eps = _NORM_KIND[kind], float(eps)
     if _traced(x, u, w, b, gate, sc, pw, pb):
-        y, z, _ = torch.ops.sca2b200.residual_norm_fwd(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt,
-                                                       _wants_grad(x, u, w, b, gate, sc, pw, pb))
+        # a tensor that vmap batches does not say whether it requires gradients
+        save = _wants_grad(x, u, w, b, gate, sc, pw, pb) or (torch.is_grad_enabled() and _transforms())
+        y, z, _ = torch.ops.sca2b200.residual_norm_fwd(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt, save)
     elif _wants_grad(x, u, w, b, gate, sc, pw, pb):
         y, z = _ResidualNorm.apply(x, u, w, b, gate, sc, pw, pb, kid, eps, zdt)
     else:

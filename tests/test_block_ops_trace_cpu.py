@@ -167,3 +167,22 @@ def test_forward_mode_is_refused(stub, case):
         torch.autograd.grad(out, leaves, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
     with fw.dual_level():  # without a tangent a level costs nothing
         f(*ins())
+
+
+def test_a_batched_join_keeps_its_statistics(stub):
+    """A leaf outside of vmap: the batched tensor does not say that it requires gradients, its output does."""
+    x, u, w = (torch.zeros(s) for s in ((3, 4, 16), (3, 4, 16), (16,)))
+    for leaf in (x, w):
+        leaf.requires_grad_(True)
+        stub.clear()
+        y, z = torch.func.vmap(lambda a, b: ops.residual_norm(a, b, w))(x, u)
+        assert z.requires_grad
+        forward = [args for what, args in stub if what == "residual_norm"]
+        assert len(forward) == 3 and all(args[3] for args in forward)  # the statistics' address
+        torch.autograd.grad(z.sum() + y.sum(), leaf)
+        assert [args[1] for what, args in stub if what == "residual_norm_bwd"] == [args[3] for args in forward][::-1]
+        leaf.requires_grad_(False)
+    stub.clear()
+    with torch.no_grad():
+        torch.func.vmap(lambda a, b: ops.residual_norm(a, b, w))(x, u)
+    assert not any(args[3] for what, args in stub)

@@ -72,3 +72,21 @@ def test_clip_in_a_trace():
     empty = torch.compile(lambda x: x + ops.clip_grads([], 1.0) + ops.grad_norm([]), fullgraph=True, backend="aot_eager")
     assert torch.equal(empty(norm), norm)
     torch.library.opcheck(torch.ops.sca2b200.clip_grads_out, (src(), [torch.zeros(40, device="cuda"), torch.zeros(3, 5, device="cuda")], 0.1))
+
+
+@pytest.mark.parametrize("kind", ["ffn", "norm"])
+def test_vmap_backward(kind):
+    """Gradients of leaves outside of vmap: the calls one by one give the same."""
+    f, ins = _block(kind)
+    x = torch.stack([ins[0].detach() * k for k in (0.5, 1.0, 2.0)]).requires_grad_(True)
+    rest = [t.detach().clone().requires_grad_(True) for t in ins[1:]]
+    g = _randn(3, *f(*ins).shape, seed=9, dtype=ins[0].dtype)
+    out = torch.func.vmap(lambda a: f(a, *rest))(x)
+    got = torch.autograd.grad(out, (x, *rest), g)
+    one = [torch.autograd.grad(f(a, *rest), (a, *rest), d) for a, d in
+           zip([t.detach().requires_grad_(True) for t in x], g)]
+    assert torch.equal(got[0], torch.stack([o[0] for o in one]))
+    for k, t in enumerate(got[1:], 1):  # three gradients added, in an order that is autograd's: 2 roundings each way
+        ref = sum(o[k].double() for o in one)
+        size = sum(o[k].double().abs() for o in one)
+        assert bool(((t.double() - ref).abs() <= 2.02 * torch.finfo(t.dtype).eps / 2 * size + 1e-30).all())
