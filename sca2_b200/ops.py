@@ -1739,8 +1739,14 @@ def _grad_table(src, dst, types):
 
 
 def _apart(grads):
-    """Refuse tensors whose ranges of memory overlap (the library sees only the copies of those that
-    are not contiguous)."""
+    """Refuse tensors whose ranges of memory overlap, and those that may hold one value in two places
+    (the library sees only the copies of tensors that are not contiguous)."""
+    for g in grads:
+        end = 1  # past the values that the dimensions of smaller strides reach
+        for k, n in sorted((k, n) for n, k in zip(g.shape, g.stride()) if n > 1) if g.numel() else ():
+            if k < end:
+                raise _lib.Sca2Error("clip_grads: a tensor that is scaled in place overlaps itself")
+            end += (n - 1) * k
     end = 0
     for a, b in sorted((g.data_ptr(), g.element_size() * (1 + sum((n - 1) * abs(k) for n, k in zip(g.shape, g.stride()))))
                        for g in grads if g.numel()):
@@ -1829,7 +1835,8 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     before (fp32 scalar; nothing waits for the device): g * min(1, max_norm / (norm + 1e-6)), as
     torch.nn.utils.clip_grad_norm_.  In place, or into the contiguous tensors `out` (float32 or
     bfloat16, one for each gradient, with as many values).  A tensor that is written may not share
-    memory with another of the call (refused; of one that is not contiguous, its whole range counts).
+    memory with another of the call (refused; of one that is not contiguous, its whole range counts), nor
+    hold a value in two places, as an expanded one does (refused, as are strides that interleave).
     Not differentiable."""
     max_norm = float(max_norm)
     if not max_norm >= 0:

@@ -186,3 +186,17 @@ def test_a_batched_join_keeps_its_statistics(stub):
     with torch.no_grad():
         torch.func.vmap(lambda a, b: ops.residual_norm(a, b, w))(x, u)
     assert not any(args[3] for what, args in stub)
+
+
+def test_a_tensor_that_overlaps_itself_is_not_clipped_in_place(stub):
+    x = torch.zeros(8, 16)
+    for bad in (x[:1, :1].expand(8, 16), x.view(-1).unfold(0, 8, 4), x[:, :3].as_strided((4, 3), (2, 1))):
+        with pytest.raises(ops._lib.Sca2Error, match="overlap"):
+            ops.clip_grads([torch.zeros(5), bad], 1.0)
+        assert not stub
+        ops.grad_norm([bad])
+        ops.clip_grads([bad], 1.0, out=[torch.zeros(bad.shape)])
+        stub.clear()
+    for good in (x.t(), x[::2, 3:9], x.view(2, 4, 16).permute(2, 0, 1), x[:1, 2:3].expand(1, 1, 1), x[:0].expand(3, 0, 16)):
+        ops.clip_grads([good], 1.0)
+    assert len(stub) == 5

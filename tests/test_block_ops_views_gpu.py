@@ -34,3 +34,26 @@ def test_a_negated_destination_is_refused():
     from sca2_b200 import _lib, ops
     with pytest.raises(_lib.Sca2Error, match="contiguous"):
         ops.clip_grads([torch.ones(1, device="cuda")], 0.5, out=[_negated(torch.ones(1, device="cuda"))])
+
+
+def test_a_tensor_that_overlaps_itself_is_not_clipped_in_place():
+    """Refused before anything is written: the gradient of a sum is one value, expanded."""
+    from sca2_b200 import _lib, ops
+    plain = torch.randn(100, device="cuda")
+    x = torch.zeros(8, 16, device="cuda", requires_grad=True)
+    (expanded,) = torch.autograd.grad(x.sum(), x)
+    assert expanded.stride() == (0, 0)
+    windows = torch.randn(40, device="cuda").unfold(0, 8, 4)
+    for bad in (expanded, windows, windows.t(), torch.zeros(6, device="cuda").as_strided((3, 2), (2, 1))[:, :1].expand(3, 5)):
+        keep, was, version = plain.clone(), bad.clone(), plain._version
+        with pytest.raises(_lib.Sca2Error, match="overlap"):
+            ops.clip_grads([plain, bad], 0.5)
+        assert torch.equal(plain, keep) and torch.equal(bad, was) and plain._version == version
+        # read, it counts with the values that it shows
+        n = ops.grad_norm([plain, bad])
+        ref = float((plain.double().square().sum() + bad.double().square().sum()).sqrt())
+        assert abs(float(n) - ref) <= (2.0 ** -24 + 1e-11) * ref
+        out = [torch.zeros(100, device="cuda"), torch.zeros(bad.shape, device="cuda")]
+        assert torch.equal(ops.clip_grads([plain, bad], 0.5, out=out), n)
+    one = torch.randn(5, 1, device="cuda").expand(5, 1)[:, :, None]  # strides of single values do not matter
+    ops.clip_grads([plain, one.as_strided((5, 1, 1), (1, 0, 7))], 0.5)
