@@ -1362,9 +1362,22 @@ def _gated_ffn_bwd_run(x, wg, wu, act: int, dh, need_x: bool, need_w: bool):
     return dx, dwg, dwu
 
 
+def _gated_ffn_check(x, wg, wu):
+    E, shape = _lib.Sca2Error, wg.shape
+    if not x.dtype == wg.dtype == wu.dtype == torch.bfloat16:
+        raise E("gated_ffn: x and the weights must be bfloat16")
+    if x.dim() < 1 or len(shape) != 2 or shape != wu.shape or shape[1] != x.shape[-1]:
+        raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(shape)} and "
+                f"{tuple(wu.shape)}")
+    if not gated_ffn_supported(shape[1], shape[0]):
+        raise E(f"gated_ffn: d and f must be multiples of 8, got {shape[1]} and {shape[0]}")
+
+
 @torch.library.custom_op("sca2b200::gated_ffn_fwd", mutates_args=())
 def _gated_ffn_fwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, act: int) -> torch.Tensor:
     """sca2_gated_ffn_fwd: h (..., f)."""
+    _device_of(x, wg, wu)
+    _gated_ffn_check(x, wg, wu)
     return _gated_ffn_run(x, wg, wu, act)
 
 
@@ -1377,6 +1390,10 @@ def _(x, wg, wu, act):
 def _gated_ffn_bwd(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, act: int, dh: torch.Tensor, need_x: bool,
                    need_w: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """sca2_gated_ffn_bwd: dx, dw_gate, dw_up (empty where not needed)."""
+    _device_of(x, wg, wu, dh)
+    _gated_ffn_check(x, wg, wu)
+    if dh.shape != (*x.shape[:-1], wg.shape[0]):
+        raise _lib.Sca2Error(f"gated_ffn: dh must have the shape of h, got {tuple(dh.shape)}")
     return tuple(x.new_empty(0) if t is None else t for t in _gated_ffn_bwd_run(x, wg, wu, act, dh, need_x, need_w))
 
 
@@ -1463,17 +1480,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: st
     inputs is kept.  The weights may be the halves of one (2 f, d) tensor."""
     _device_of(x, w_gate, w_up)
     _no_tangents("gated_ffn", x, w_gate, w_up)
-    E = _lib.Sca2Error
     if act not in _ACT:
-        raise E(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
-    if not x.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16:
-        raise E("gated_ffn: x and the weights must be bfloat16")
-    shape = w_gate.shape
-    if x.dim() < 1 or len(shape) != 2 or shape != w_up.shape or shape[1] != x.shape[-1]:
-        raise E(f"gated_ffn: x (..., d) and weights (f, d), got {tuple(x.shape)}, {tuple(shape)} and "
-                f"{tuple(w_up.shape)}")
-    if not gated_ffn_supported(shape[1], shape[0]):
-        raise E(f"gated_ffn: d and f must be multiples of 8, got {shape[1]} and {shape[0]}")
+        raise _lib.Sca2Error(f"gated_ffn: act must be 'silu' or 'gelu', not {act!r}")
+    _gated_ffn_check(x, w_gate, w_up)
     if _traced(x, w_gate, w_up):
         return torch.ops.sca2b200.gated_ffn_fwd(x, w_gate, w_up, _ACT[act])
     if _wants_grad(x, w_gate, w_up):
@@ -1547,12 +1556,44 @@ def _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind: int, eps: floa
     return dx, du, dw, db, dgate, dscale, dpw, dpb
 
 
+def _residual_norm_check(x, u, gate, params, zdt):
+    """params: weight, bias, scale, post_weight, post_bias."""
+    E, shape = _lib.Sca2Error, x.shape
+    d = shape[-1] if shape else 0
+    if d < 1 or u.shape != shape:
+        raise E(f"residual_norm: x and u must have one shape (..., d), got {tuple(shape)} and {tuple(u.shape)}")
+    if gate is not None and gate.shape != shape and gate.shape != (*shape[:-1], 1):
+        raise E(f"residual_norm: gate must be (..., d) or (..., 1), got {tuple(gate.shape)}")
+    if x.dtype not in _DT or u.dtype not in _DT or zdt not in _DT:
+        raise E("residual_norm: x, u and out_dtype must be float32 or bfloat16")
+    w, b, _, pw, pb = params
+    if (b is not None and w is None) or (pb is not None and pw is None):
+        raise E("residual_norm: a bias needs its weight")
+    for t in params:
+        if t is not None and t.shape != (d,):
+            raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
+
+
+def _residual_norm_op_check(x, u, w, b, gate, scale, pw, pb, zdt):
+    """What the public function has seen to before it calls a registered operator.  Returns the parameters
+    (vmap's slices of them need not be contiguous)."""
+    params = (w, b, scale, pw, pb)
+    _residual_norm_check(x, u, gate, params, zdt)
+    if any(t is not None and t.dtype != torch.float32 for t in params):
+        raise _lib.Sca2Error("residual_norm: the operator takes float32 weights, biases and scale")
+    if gate is not None and gate.dtype != u.dtype:
+        raise _lib.Sca2Error("residual_norm: the operator takes a gate of u's type")
+    return [None if t is None else t.contiguous() for t in params]
+
+
 @torch.library.custom_op("sca2b200::residual_norm_fwd", mutates_args=())
 def _residual_norm_fwd(x: torch.Tensor, u: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor],
                        gate: Optional[torch.Tensor], scale: Optional[torch.Tensor], pw: Optional[torch.Tensor],
                        pb: Optional[torch.Tensor], kind: int, eps: float, zdt: torch.dtype, save: bool
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """sca2_residual_norm_fwd: y, z (empty without w) and, with save, the rows' means and deviations."""
+    _device_of(x, u, w, b, gate, scale, pw, pb)
+    w, b, scale, pw, pb = _residual_norm_op_check(x, u, w, b, gate, scale, pw, pb, zdt)
     y, z, stats = _residual_norm_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, save)
     return y, z, x.new_empty((0, 4), dtype=torch.float32) if stats is None else stats
 
@@ -1571,6 +1612,12 @@ def _residual_norm_bwd(x: torch.Tensor, u: torch.Tensor, w: Optional[torch.Tenso
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                                   torch.Tensor, torch.Tensor]:
     """sca2_residual_norm_bwd: dx, du, dw, db, dgate, dscale, dpw, dpb (empty where there is no input)."""
+    _device_of(x, u, w, b, gate, scale, pw, pb, stats, dy, dz)
+    w, b, scale, pw, pb = _residual_norm_op_check(x, u, w, b, gate, scale, pw, pb, zdt)
+    if stats.shape != (x.numel() // x.shape[-1], 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise _lib.Sca2Error("residual_norm: the operator takes the statistics that its forward kept (save)")
+    if any(t is not None and t.shape != x.shape for t in (dy, dz)):
+        raise _lib.Sca2Error("residual_norm: dy and dz must have the shape of x")
     out = _residual_norm_bwd_run(x, u, w, b, gate, scale, pw, pb, kind, eps, zdt, stats, dy, dz)
     return tuple(x.new_empty(0) if t is None else t for t in out)
 
@@ -1645,29 +1692,17 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
     arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
     _device_of(x, u, weight, bias, gate, scale, post_weight, post_bias)
     _no_tangents("residual_norm", x, u, weight, bias, gate, scale, post_weight, post_bias)
-    E, shape = _lib.Sca2Error, x.shape
-    d = shape[-1] if shape else 0
     if kind not in _NORM_KIND:
-        raise E(f"residual_norm: kind must be 'layer' or 'rms', not {kind!r}")
-    if d < 1 or u.shape != shape:
-        raise E(f"residual_norm: x and u must have one shape (..., d), got {tuple(shape)} and {tuple(u.shape)}")
-    if gate is not None and gate.shape != shape and gate.shape != (*shape[:-1], 1):
-        raise E(f"residual_norm: gate must be (..., d) or (..., 1), got {tuple(gate.shape)}")
-    zdt = x.dtype if out_dtype is None else out_dtype
-    if x.dtype not in _DT or u.dtype not in _DT or zdt not in _DT:
-        raise E("residual_norm: x, u and out_dtype must be float32 or bfloat16")
-    if (bias is not None and weight is None) or (post_bias is not None and post_weight is None):
-        raise E("residual_norm: a bias needs its weight")
-    par = []
-    for t in (weight, bias, scale, post_weight, post_bias):
+        raise _lib.Sca2Error(f"residual_norm: kind must be 'layer' or 'rms', not {kind!r}")
+    zdt, d = x.dtype if out_dtype is None else out_dtype, x.shape[-1] if x.shape else 0
+    par = [weight, bias, scale, post_weight, post_bias]
+    _residual_norm_check(x, u, gate, par, zdt)
+    for k, t in enumerate(par):
         if t is not None:
-            if t.shape != (d,):
-                raise E(f"residual_norm: weights, biases and scale must have shape ({d},), got {tuple(t.shape)}")
             if t.dtype != torch.float32 or not t.is_contiguous():
-                t = t.float().contiguous()
+                par[k] = t = t.float().contiguous()
             if d == 1 and not torch.compiler.is_compiling():  # one value needs no copy for its strides
-                t = t.resolve_neg()
-        par.append(t)
+                par[k] = t.resolve_neg()
     if gate is not None and gate.dtype != u.dtype:
         gate = gate.to(u.dtype)
     w, b, sc, pw, pb = par

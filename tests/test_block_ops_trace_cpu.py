@@ -200,3 +200,52 @@ def test_a_tensor_that_overlaps_itself_is_not_clipped_in_place(stub):
     for good in (x.t(), x[::2, 3:9], x.view(2, 4, 16).permute(2, 0, 1), x[:1, 2:3].expand(1, 1, 1), x[:0].expand(3, 0, 16)):
         ops.clip_grads([good], 1.0)
     assert len(stub) == 5
+
+
+def _op_calls():
+    """Calls of the registered operators with one argument that does not fit the others."""
+    o = torch.ops.sca2b200
+    z = lambda *s, t=H: torch.zeros(*s, dtype=t)
+    x, w, dh = z(4, 16), z(24, 16), z(4, 24)
+    for a in ((x, w, z(16, 16)), (x, z(24, 8), z(24, 8)), (x.float(), w, w), (x, w.half(), w), (z(4, 12), z(24, 12), z(24, 12)),
+              (x, z(16), z(16))):
+        yield lambda a=a: o.gated_ffn_fwd(*a, 0)
+        yield lambda a=a: o.gated_ffn_bwd(*a, 0, dh, True, True)
+    for bad in (z(3, 24), z(4, 16), z(24)):
+        yield lambda bad=bad: o.gated_ffn_bwd(x, w, w, 0, bad, True, True)
+    f = torch.float32
+    x, v, st = z(4, 16, t=f), z(16, t=f), z(4, 4, t=f)
+    ins = dict(x=x, u=x, w=v, b=v, gate=x, scale=v, pw=v, pb=v)
+    for k, bad in (("u", z(4, 8, t=f)), ("u", z(3, 16, t=f)), ("w", z(8, t=f)), ("b", z(16)), ("gate", z(4, 2, t=f)), ("gate", z(4, 16)),
+                   ("gate", z(4, t=f)), ("scale", z(1, t=f)), ("pw", z(16, t=torch.double)), ("pb", z(16, 1, t=f)), ("x", z(4, 16, t=torch.half)),
+                   ("w", None), ("pw", None)):
+        a = [*{**ins, k: bad}.values(), 0, 1e-5, f]
+        yield lambda a=a: o.residual_norm_fwd(*a, True)
+        yield lambda a=a: o.residual_norm_bwd(*a, st, x, x)
+    a = [*ins.values(), 0, 1e-5, f]
+    yield lambda: o.residual_norm_fwd(*ins.values(), 0, 1e-5, torch.half, True)
+    for st2, dy, dz in ((z(0, 4, t=f), x, x), (z(3, 4, t=f), x, x), (z(4, 4), x, x), (z(4, 8, t=f)[:, ::2], x, x), (st, z(3, 16, t=f), x),
+                        (st, x, z(4, 8, t=f))):
+        yield lambda s=st2, p=dy, q=dz: o.residual_norm_bwd(*a, s, p, q)
+
+
+def test_registered_operators_check_their_arguments(stub):
+    for k, call in enumerate(_op_calls()):
+        with pytest.raises(ops._lib.Sca2Error):
+            call()
+        assert not stub, k
+
+
+def test_registered_operators_refuse_cpu_tensors(monkeypatch):
+    """Without the stub of the device check: no host address reaches a launch."""
+    made = []
+    monkeypatch.setattr(ops, "_launch", lambda *a: made.append(a))
+    o, (x, w, _), n = torch.ops.sca2b200, _ffn(), torch.zeros(4, 16)
+    v, dh = torch.zeros(16), torch.zeros(4, 24, dtype=H)
+    for call in (lambda: o.gated_ffn_fwd(x, w, w, 0), lambda: o.gated_ffn_bwd(x, w, w, 0, dh, True, True),
+                 lambda: o.residual_norm_fwd(n, n, v, v, None, None, None, None, 0, 1e-5, torch.float32, True),
+                 lambda: o.residual_norm_bwd(n, n, v, v, None, None, None, None, 0, 1e-5, torch.float32, torch.zeros(4, 4), n, n),
+                 lambda: o.grad_norm([n]), lambda: o.clip_grads_([n], 1.0), lambda: o.clip_grads_out([n], [n], 1.0)):
+        with pytest.raises(ops._lib.Sca2Error, match="CUDA"):
+            call()
+    assert not made

@@ -90,3 +90,19 @@ def test_vmap_backward(kind):
         ref = sum(o[k].double() for o in one)
         size = sum(o[k].double().abs() for o in one)
         assert bool(((t.double() - ref).abs() <= 2.02 * torch.finfo(t.dtype).eps / 2 * size + 1e-30).all())
+
+
+def test_vmap_over_parameters():
+    """Slices that are not contiguous, of parameters too."""
+    from sca2_b200 import ops
+    x, u = _randn(70, 64), _randn(70, 64, seed=1)
+    ws = [_randn(64, 3, seed=2 + k, grad=True) for k in range(3)]
+    f = lambda w, s, p: ops.residual_norm(x, u, w, scale=s, post_weight=p)
+    y, z = torch.func.vmap(f, in_dims=1)(*ws)
+    got = torch.autograd.grad(z, ws, torch.ones_like(z))
+    for k in range(3):
+        one = [w.detach()[:, k].contiguous().requires_grad_(True) for w in ws]
+        ry, rz = f(*one)
+        assert torch.equal(y[k], ry) and torch.equal(z[k], rz)
+        for g, r in zip(got, torch.autograd.grad(rz, one, torch.ones_like(rz))):
+            assert torch.equal(g[:, k], r)
