@@ -1686,7 +1686,8 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
         p = N_post(u) if post_weight is given, else u
         y = x + scale * sigmoid(gate) * p          z = N(y) if weight is given, else None
 
-    x, u (..., d) fp32 or bf16 (their types may differ), d <= 4096; gate (..., d) or (..., 1) logits;
+    x, u (..., d) fp32 or bf16 (their types may differ), d <= 4096; gate (..., d) or (..., 1) logits
+    (of another type than u's, both are read as fp32);
     weight, bias, post_weight, post_bias, scale (d) (computed with in fp32).  kind: "layer"
     (LayerNorm) or "rms" (no bias), for both norms.  y has x's type, z out_dtype (default: x's);
     arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
@@ -1703,8 +1704,8 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
                 par[k] = t = t.float().contiguous()
             if d == 1 and not torch.compiler.is_compiling():  # one value needs no copy for its strides
                 par[k] = t.resolve_neg()
-    if gate is not None and gate.dtype != u.dtype:
-        gate = gate.to(u.dtype)
+    if gate is not None and gate.dtype != u.dtype:  # the kernels have one type for both
+        gate, u = gate.float(), u.float()
     w, b, sc, pw, pb = par
     kid, eps = _NORM_KIND[kind], float(eps)
     if _traced(x, u, w, b, gate, sc, pw, pb):

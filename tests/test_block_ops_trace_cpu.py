@@ -5,7 +5,7 @@ import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from sca2_b200 import ops
+from sca2_b200 import _lib, ops
 
 H = torch.bfloat16
 
@@ -249,3 +249,12 @@ def test_registered_operators_refuse_cpu_tensors(monkeypatch):
         with pytest.raises(ops._lib.Sca2Error, match="CUDA"):
             call()
     assert not made
+
+
+def test_a_gate_of_another_type_keeps_its_bits(stub):
+    x, u = torch.zeros(4, 16), torch.zeros(4, 16, dtype=H)
+    for gate in (torch.zeros(4, 1), torch.zeros(4, 16), torch.zeros(4, 16, dtype=torch.half)):
+        ops.residual_norm(x, u, gate=gate)
+    assert [args[0].u_dtype for _, args in stub] == [_lib.SCA2_F32] * 3
+    ops.residual_norm(x, u, gate=u)
+    assert stub[-1][1][0].u_dtype == _lib.SCA2_BF16
