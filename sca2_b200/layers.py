@@ -135,9 +135,14 @@ class GatedFFN(nn.Module):
         return self.down(h)
 
 
+_JOINED = (torch.float32, torch.bfloat16)  # ops.residual_norm's types
+
+
 class ResidualJoin(nn.Module):
     """x + scale * sigmoid(gate(z)) * norm(u) for a branch's output u and its normed input z, and
-    the norm of the sum for the next branch, in one kernel (ops.residual_norm)."""
+    the norm of the sum for the next branch: one kernel (ops.residual_norm) for fp32 and bf16 streams
+    of widths that it covers, with an fp16 branch read as fp32; torch's operations, in fp32 at least,
+    for others."""
 
     def __init__(self, d: int, tail: TailCfg, eps: float):
         super().__init__()
@@ -148,11 +153,23 @@ class ResidualJoin(nn.Module):
 
     def forward(self, x, u, z, next_norm: Optional[nn.LayerNorm] = None):
         dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else x.dtype
+        dt = dt if dt == torch.bfloat16 else x.dtype
+        gate = self.gate(z) if self.gate is not None else None
+        if not (x.is_cuda and x.dtype in _JOINED and u.dtype != torch.float64 and ops.residual_norm_supported(x.shape[-1])):
+            return self._join(x, u, gate, next_norm, dt)
         w, b = (next_norm.weight, next_norm.bias) if next_norm is not None else (None, None)
         pw, pb = (self.norm.weight, self.norm.bias) if self.norm is not None else (None, None)
-        return ops.residual_norm(x, u, w, b, gate=self.gate(z) if self.gate is not None else None, scale=self.scale,
-                                 post_weight=pw, post_bias=pb, eps=self.eps,
-                                 out_dtype=dt if dt == torch.bfloat16 else x.dtype)
+        return ops.residual_norm(x, u if u.dtype in _JOINED else u.float(), w, b, gate=gate, scale=self.scale,
+                                 post_weight=pw, post_bias=pb, eps=self.eps, out_dtype=dt)
+
+    def _join(self, x, u, gate, next_norm, dt):
+        wide = torch.float64 if torch.float64 in (x.dtype, u.dtype) else torch.float32
+        norm = lambda v, n: F.layer_norm(v, v.shape[-1:], n.weight.to(wide), n.bias.to(wide), self.eps)
+        with torch.autocast(x.device.type, enabled=False):
+            p = u.to(wide) if self.norm is None else norm(u.to(wide), self.norm)
+            p = p if self.scale is None else p * self.scale.to(wide)
+            y = x.to(wide) + (p if gate is None else p * torch.sigmoid(gate.to(wide)))
+            return y.to(x.dtype), None if next_norm is None else norm(y, next_norm).to(dt)
 
 
 Slot = Tuple[str, str]  # (module attribute, state key)

@@ -1675,6 +1675,11 @@ class _ResidualNorm(torch.autograd.Function):
     once = staticmethod(once_differentiable(grads.__func__))  # with create_graph
 
 
+def residual_norm_supported(d: int) -> bool:
+    """Widths that residual_norm takes: up to 4096."""
+    return 1 <= d <= 4096
+
+
 def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tensor] = None,
                   bias: Optional[torch.Tensor] = None, *, gate: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
