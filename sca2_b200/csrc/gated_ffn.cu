@@ -33,7 +33,8 @@
 // Up to FEW_ROWS rows (decode) the forward is bound by reading the weights and by latency:
 // `ffn_few` keeps no tiles, each warp streams weight rows straight into mma.sync fragments.
 //
-// Every wait is bounded: a wait that runs out sets the fault word and the kernel leaves.
+// Every wait is bounded: a wait that runs out sets the fault word, and the kernel leaves once its copies
+// and products in flight are done (waits that are bounded too).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -174,11 +175,11 @@ __device__ __forceinline__ void mma2(uint32_t d, uint64_t a, uint64_t b, uint32_
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// arrive on the barrier at this offset in both CTAs once the products issued so far are done
-__device__ __forceinline__ void commit2(uint32_t bar) {
+// arrive on the barrier at this offset in the CTAs of `mask` (both) once the products issued so far are done
+__device__ __forceinline__ void commit2(uint32_t bar, uint16_t mask = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
+      "h"(mask)
       : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t t, uint32_t* r) {
@@ -330,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;  // the same offset in both CTAs
   const uint32_t stg0 = base + L::RING, bars = base + L::BARS;
   const uint32_t full = bars, empty = bars + 8 * ST, tfull = bars + 16 * ST, tempty = tfull + 16, dhbar = tempty + 16,
-                 slot = dhbar + 8 * EPI_WARPS;
+                 slot = dhbar + 8 * EPI_WARPS, done = slot + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -342,6 +343,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
     for (int s = 0; s < ST; ++s) init(full + 8 * s, 1), init(empty + 8 * s, 1);
     for (int s = 0; s < 2; ++s) init(tfull + 8 * s, 1), init(tempty + 8 * s, 2 * EPI_WARPS);
     for (int s = 0; s < EPI_WARPS; ++s) init(dhbar + 8 * s, 1);
+    init(done, 1);
     umma::fence_mbar_init();
   }
   if (warp == 2) {
@@ -390,7 +392,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
         }
         return true;
       });
-      if (!ok && rank == 0)  // leave no copy in flight: both CTAs' copies complete on these
+      if (rank == 0)  // leave no copy in flight, whichever wait ran out: both CTAs' copies complete on these
         for (; issued > 0; --issued) {
           if (--s < 0) s = ST - 1, ph ^= 1;
           if (!wait_for(full + 8 * s, ph ^ 1)) break;
@@ -421,6 +423,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
         ++n;
         return true;
       });
+      commit2(done, 1);  // nor a product, whose operands and accumulator are about to be given up
+      wait_for(done, 0);
     }
   } else if (warp >= 4) {  // ---- epilogue: 32 rows (the warp's quarter of TMEM) x a quarter of the columns
     const int e = warp - 4, q = warp & 3, part = e >> 2;
@@ -439,7 +443,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1) ffn_gemm(cons
           load1(stg, &maps.dh, hc, row, dhb);
         }
       }
-      if (!__all_sync(0xffffffffu, wait_for(tfull + 8 * acc, (n >> 1) & 1))) return false;
+      if (!__all_sync(0xffffffffu, wait_for(tfull + 8 * acc, (n >> 1) & 1))) {
+        if constexpr (MODE == BACK) wait_for(dhb, n & 1);  // the copy of dh is in flight
+        return false;
+      }
       umma::fence_after_sync();
       if constexpr (MODE == FWD || MODE == BACK) {
         uint32_t rg[32], ru[32];
