@@ -44,3 +44,57 @@ def test_layer_under_fp16_autocast():
     assert relerr(y, ref) < 2e-2
     y.sum().backward()
     assert all(bool(torch.isfinite(p.grad).all()) for n, p in layer.named_parameters() if n.split(".")[0] in ("ff", "join1", "join2"))
+
+
+@pytest.mark.parametrize("kind", ["gated", "lapa"])
+@pytest.mark.parametrize("batch", [1, 3])
+def test_bf16_graph_decoder_gives_the_eager_tokens(kind, batch):
+    """The few-row kernels inside a decode graph: token for token, and logit for logit, what eager steps
+    give under the same autocast."""
+    from sca2_b200 import _lib, lm as L
+    from tests.test_block_tail_gpu import _lm
+    m = _lm(kind, dict(ffn_act="silu", post_norm=True, gate="channel", res_scale=0.5)).eval()
+    tok = torch.randint(0, 128, (batch, 24), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+        logits, st = m.prefill(tok)
+        first = logits[:, -1].argmax(-1)
+        dec = L.GraphDecoder(m, st)
+        got, t, e = [], first, first
+        for _ in range(8):
+            t = dec.step(t).clone()
+            lg, st = m.step(e, st)
+            e = lg.argmax(-1)
+            assert bool(torch.isfinite(lg).all()) and torch.equal(dec.logits, lg)
+            got.append((t, e))
+    assert all(torch.equal(a, b) for a, b in got)
+    assert _lib.device_faults() == 0
+
+
+def test_capture_while_an_eager_graph_of_the_leaves_lives():
+    """The tail, its backward and the clip captured on detached aliases while an eager graph of the
+    parameters is kept, which is differentiated afterwards."""
+    from sca2_b200 import layers, ops
+    torch.manual_seed(7)
+    ffn = layers.GatedFFN(64, 128).cuda().bfloat16()
+    join = layers.ResidualJoin(64, layers.TailCfg(post_norm=True, gate="channel", res_scale=0.5), 1e-5).cuda().bfloat16()
+    names = [("ffn", n) for n, _ in ffn.named_parameters()] + [("join", n) for n, _ in join.named_parameters()]
+    ps = [*ffn.parameters(), *join.parameters()]
+    x = torch.randn(300, 64, device="cuda").bfloat16()
+
+    def forward(params):
+        of = lambda part: {n: p for (q, n), p in zip(names, params) if q == part}
+        h = torch.func.functional_call(ffn, of("ffn"), (x,))
+        return torch.func.functional_call(join, of("join"), (x, h, x))[0]
+
+    def step(params, y):
+        grads = torch.autograd.grad(y, params, torch.ones_like(y))
+        return (*grads, ops.clip_grads(grads, 0.5))
+    eager = forward(ps)
+    own = [p.detach().requires_grad_(True) for p in ps]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(own, forward(own))
+    g.replay()
+    ref = step(ps, eager)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(ref, out))
