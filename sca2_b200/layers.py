@@ -283,7 +283,8 @@ class SCA2Layer(MixerLayer):
         dv = _dv(cfg)
         c = _c_head(cfg, c_cls or heads.CHeadRef, cfg.d, dv)
         dh = _d_head(cfg, d_cls or heads.DHeadRef, cfg.d, dv)
-        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, conv, cfg.tail)
+        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, conv,
+                         getattr(cfg, "tail", None))
         self.cfg = cfg
 
 
@@ -311,7 +312,8 @@ class ShortLayer(MixerLayer):
         dv = _dv(cfg)
         c = _c_head(cfg, self.C_CLS, cfg.d, dv)
         dh = heads.CHeadShort(cfg.d, cfg.Ls, dv, theta_scale=cfg.theta_scale or 0.02)
-        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff, tail=cfg.tail)
+        super().__init__(cfg.d, [("c", "c", c), ("dh", "d", dh)], 4 * dv, cfg.ff,
+                         tail=getattr(cfg, "tail", None))
         self.cfg = cfg
         if hasattr(c, "lam_raw"):
             c.LAM_MAX = cfg.lam_max if cfg.lam_max is not None else 1.0 / cfg.Ls
