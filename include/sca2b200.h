@@ -424,7 +424,8 @@ SCA2_API int sca2_gated_ffn_fwd(const sca2_ffn_args* a, void* h, void* stream);
 SCA2_API int64_t sca2_gated_ffn_work_bytes(int64_t rows, int32_t d, int32_t f);
 
 /* Gradients from dh (rows, f) dense: dx (rows, d) dense or NULL, dw_gate and dw_up (f, d) dense or
- * both NULL, all written.  g and u are recomputed.  work 256-byte aligned. */
+ * both NULL, all written.  g and u are recomputed with fp32 accumulators; dg and du are rounded to bf16
+ * as operands of the gradients' products, and the gradients once more.  work 256-byte aligned. */
 SCA2_API int sca2_gated_ffn_bwd(const sca2_ffn_args* a, const void* dh, void* dx, void* dw_gate, void* dw_up,
                    void* work, int64_t work_bytes, void* stream);
 

@@ -13,8 +13,10 @@
 //         Wg's rows and CTA 1 Wu's, so one accumulator row holds g and u of a column and the
 //         epilogue forms h without a trip to memory.
 //   BACK  the same product again with dh: g and u are recomputed in fp32 rather than kept (which
-//         would cost 2 rows f bf16 values of memory for the whole step and a rounding of both),
-//         dg and du are rounded to bf16 once, as operands of the next two products.
+//         would cost 2 rows f bf16 values of memory for the whole step and a rounding of both).
+//         dg and du are rounded to bf16 once, as operands of the next two products (two bf16 terms of
+//         each would double those).  That shows in the gradients: in the 2-norm they are 0.0023 off 64
+//         bits, 0.0017 if dg and du kept 32 bits until the gradients themselves are rounded.
 //   DX    contraction over f twice, (dg, Wg) then (du, Wu), one accumulator; the weights are read
 //         as they lie (MN-major operand), no transposed copy.
 //   DW    contraction over the rows, both operands MN-major; split over the rows where the tiles
@@ -24,8 +26,9 @@
 //         65536 x 768 -> 2048 555 us for both, 580 as two launches and a pass over split parts.
 // Ragged sizes: TMA fills what lies outside with zeros and clips what is stored there.
 //
-// Measured (one B200, device time in short bursts): 32768 x 1024 -> 4096 forward 360 us (1530 TFLOP/s,
-// 91% of the measured cuBLAS burst); 65536 x 768 -> 2048 forward 290 us, BACK 340, GRADS 555.  Bound by
+// Measured (one B200): 32768 x 1024 -> 4096 forward 420 to 430 us called back to back (1280 to 1310
+// TFLOP/s, 92% of what cuBLAS sustains under the power limit), 360 us in short bursts (1530, 91% of its
+// burst).  In short bursts 65536 x 768 -> 2048: forward 290 us, BACK 340, GRADS 555.  Bound by
 // the tensor cores under the power limit: a contraction block of a tile takes 0.37 us at any width,
 // which is cuBLAS's rate; at d = 768 the epilogue and the switch of tiles add 15%, in BACK 30% (half of
 // that its stores).  L2 prefetches of the operands by TMA slowed every product (360 -> 400 us).

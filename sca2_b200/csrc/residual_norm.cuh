@@ -1028,10 +1028,12 @@ cudaError_t fwd_wide_launch(const Args& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 // A CTA a row (fwd_wide) for rows wider than fwd_ring takes, for odd rows from 513 values, and for few rows,
-// each by more threads (against fwd_ring, everything on: 1184 and 1776 rows of 256 values 5.5 / 4.7 and 7.2 /
-// 4.7 us, of 768 6.2 / 8.8 and 8.1 / 9.0; 64 rows 2.7 / 7.1).  Beyond 768 values fwd_ring's slots leave two
-// CTAs an SM, and few means more rows (3552, 7104, 10656 rows of 1024 values 15.0 / 21.0, 27.0 / 28.2,
-// 38.9 / 38.1 us; of 896 14.3 / 19.1, 26.1 / 26.1, 37.4 / 35.2).
+// each by more threads (against fwd_ring, everything on: 1184 and 1776 rows of 768 values 6.2 / 8.8 and 8.1 /
+// 9.0 us; 64 rows 2.7 / 7.1).  The bound is one for all widths to 768 and too high for narrow rows, most of
+// whose threads hold no column: 1184 and 1776 rows of 256 values take 5.5 / 4.7 and 7.2 / 4.7 us.  Beyond 768
+// values fwd_ring's slots leave two CTAs an SM (one where x and u are fp32 with a channel gate and all five
+// parameters), and few means more rows (3552, 7104, 10656 rows of 1024 values 15.0 / 21.0, 27.0 / 28.2,
+// 38.9 / 38.1 us; of 896 14.3 / 19.1, 26.1 / 26.1, 37.4 / 35.2; measured where two fit).
 inline int few_rows(int d) { return 148 * (d > 768 ? 48 : 8); }
 template <int GATE, bool POST, bool ANY, class TX, class TU>
 cudaError_t fwd_width(const Args& a, cudaStream_t st) {
@@ -1082,7 +1084,8 @@ cudaError_t bwd_ring_gate(const Args& a, cudaStream_t st) {
 template <bool CONTIG, class TX, class TU>
 cudaError_t bwd_launch(const Args& a, cudaStream_t st) {
   const int d = a.d, grid = bwd_grid(a.rows, d), T = bwd_threads(d, 1);
-  // rows near 4096 values with everything on and no type of 16 bits, or of any alignment, do not fit
+  // The slots are counted for a channel gate and z, whatever the call has: above 3840 values rows with no
+  // type of 16 bits, and those of any alignment, count as too large.
   using L = BwdRing<2, 2, true, !CONTIG, TX, TU>;
   const bool fits = d <= 1024 || L::thread(L::z_bytes(a.zdt == SCA2_BF16)) * bwd_threads(d, 2) <= SMEM_MOST;
   if ((many(a.rows, d) || many_wide(a.rows, d, !CONTIG)) && fits)

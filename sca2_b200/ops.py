@@ -1475,9 +1475,11 @@ def gated_ffn_supported(d: int, f: int) -> bool:
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu") -> torch.Tensor:
     """h = act(x w_gate^T) * (x w_up^T): both projections of a gated feed-forward block, the
     activation ("silu", or "gelu" in its exact form) and the product in one kernel.  x (..., d),
-    weights (f, d), all bf16 with fp32 accumulation, d and f multiples of 8; returns h (..., f).
-    Differentiable once in all three; the backward recomputes the projections, so nothing but the
-    inputs is kept.  The weights may be the halves of one (2 f, d) tensor."""
+    weights (f, d), all bf16 with fp32 accumulation, d and f multiples of 8; returns h (..., f),
+    rounded once.  Differentiable once in all three, in reverse; the backward recomputes the
+    projections, so nothing but the inputs is kept, and rounds the gradients of both projections to
+    bf16 before the products that give dx, dw_gate and dw_up, which are rounded too.  The weights may
+    be the halves of one (2 f, d) tensor."""
     _device_of(x, w_gate, w_up)
     _no_tangents("gated_ffn", x, w_gate, w_up)
     if act not in _ACT:
@@ -1695,7 +1697,8 @@ def residual_norm(x: torch.Tensor, u: torch.Tensor, weight: Optional[torch.Tenso
     (of another type than u's, both are read as fp32);
     weight, bias, post_weight, post_bias, scale (d) (computed with in fp32).  kind: "layer"
     (LayerNorm) or "rms" (no bias), for both norms.  y has x's type, z out_dtype (default: x's);
-    arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor."""
+    arithmetic is fp32 and z is formed from the unrounded y.  Differentiable once in every tensor, in
+    reverse."""
     _device_of(x, u, weight, bias, gate, scale, post_weight, post_bias)
     _no_tangents("residual_norm", x, u, weight, bias, gate, scale, post_weight, post_bias)
     if kind not in _NORM_KIND:
