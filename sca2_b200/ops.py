@@ -1865,12 +1865,12 @@ def grad_norm(grads) -> torch.Tensor:
     grads = [grads] if isinstance(grads, _T) else list(grads)
     if not grads:
         return torch.zeros((), device="cuda")
-    if torch.compiler.is_compiling():
-        return torch.ops.sca2b200.grad_norm(grads)
-    grads, outs, types, dev = _grad_list("grad_norm", grads)
-    if _traced(*grads):
-        return torch.ops.sca2b200.grad_norm(grads)
     with torch.no_grad():
+        if torch.compiler.is_compiling():
+            return torch.ops.sca2b200.grad_norm(grads)
+        grads, outs, types, dev = _grad_list("grad_norm", grads)
+        if _traced(*grads):
+            return torch.ops.sca2b200.grad_norm(grads)
         return _clip_run(grads, outs, types, None, dev)
 
 
@@ -1892,13 +1892,13 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     compiling = torch.compiler.is_compiling()
     if not compiling:
         grads, outs, types, dev = _grad_list("clip_grads", grads, out)
-    if compiling or _traced(*grads, *(out or ())):
-        if out is None:
-            return torch.ops.sca2b200.clip_grads_(grads, max_norm)
-        if not compiling:  # else found out by the operator
-            _same_sizes([g.numel() for g in grads], out)
-        return torch.ops.sca2b200.clip_grads_out(grads, out, max_norm)
     with torch.no_grad():
+        if compiling or _traced(*grads, *(out or ())):
+            if out is None:
+                return torch.ops.sca2b200.clip_grads_(grads, max_norm)
+            if not compiling:  # else found out by the operator
+                _same_sizes([g.numel() for g in grads], out)
+            return torch.ops.sca2b200.clip_grads_out(grads, out, max_norm)
         norm = _clip_run(grads, outs, types, max_norm, dev)
     try:
         torch.autograd.graph.increment_version(outs)

@@ -4,10 +4,16 @@ nothing), so only structure is compared, never values."""
 import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from sca2_b200 import _lib, ops
 
 H = torch.bfloat16
+
+
+class Mode(TorchDispatchMode):
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
 
 
 @pytest.fixture
@@ -77,8 +83,6 @@ def test_jit_trace_records_the_operators(stub, case):
 
 
 def test_dispatch_modes_see_the_operators(stub):
-    from torch.utils._python_dispatch import TorchDispatchMode
-
     class Seen(TorchDispatchMode):
         def __init__(self):
             super().__init__()
@@ -258,3 +262,15 @@ def test_a_gate_of_another_type_keeps_its_bits(stub):
     assert [args[0].u_dtype for _, args in stub] == [_lib.SCA2_F32] * 3
     ops.residual_norm(x, u, gate=u)
     assert stub[-1][1][0].u_dtype == _lib.SCA2_BF16
+
+
+@pytest.mark.parametrize("case", ["grad_norm", "clip", "clip_out"])
+def test_not_differentiable_in_a_trace_either(stub, case):
+    """Tensors that require gradients: the norm and what is written do not become part of a graph."""
+    f, ins, _ = CASES[case]
+    for leaf in (True, False):
+        ts = [t if leaf else t * 1 for t in ins(True)]
+        nodes = [t.grad_fn for t in ts]
+        with Mode():
+            n = f(*ts)
+        assert not n.requires_grad and [t.grad_fn for t in ts] == nodes

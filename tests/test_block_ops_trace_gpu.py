@@ -106,3 +106,15 @@ def test_vmap_over_parameters():
         assert torch.equal(y[k], ry) and torch.equal(z[k], rz)
         for g, r in zip(got, torch.autograd.grad(rz, one, torch.ones_like(rz))):
             assert torch.equal(g[:, k], r)
+
+
+def test_clip_of_parameters_compiled():
+    """Leaves that require gradients, as in the plain call: nothing becomes part of a graph."""
+    from sca2_b200 import ops
+    a, b = _randn(40, grad=True), _randn(3, 5, grad=True)
+    x, y = a.detach().clone().requires_grad_(True), b.detach().clone().requires_grad_(True)
+    n = ops.clip_grads([a, b], 0.1)
+    m = torch.compile(lambda u, v: ops.clip_grads([u, v], 0.1), fullgraph=True, backend="aot_eager")(x, y)
+    assert torch.equal(n, m) and not m.requires_grad and torch.equal(a, x) and torch.equal(b, y) and x.is_leaf
+    r = torch.compile(lambda u, v: ops.grad_norm([u, v]), fullgraph=True, backend="aot_eager")(x, y)
+    assert torch.equal(r, ops.grad_norm([a, b])) and not r.requires_grad
