@@ -43,7 +43,7 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent where torch has no CUDA
 
 
 def _launch(what: str, fn, dev: int, *args):
